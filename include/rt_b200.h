@@ -635,6 +635,80 @@ int rt_mla_sparse_decode(const void* q_abs, const void* q_pe, const void* kv, co
                          int64_t idx_batch_stride, int64_t splits, float softmax_scale,
                          void* stream);
 
+/* ------------------------------------------------------------------------ */
+/* Paged caches                                                                */
+/* ------------------------------------------------------------------------ */
+
+/*
+ * Upkeep of a paged cache. Its rows lie in page buffers [pages, page_size, row bytes] (up to
+ * RT_PAGE_MAX_BUFFERS of them: `bases`, the bytes from page to page `page_strides`, `row_bytes`; host
+ * arrays) under one table: table int32 [n_seqs, width] (row pitch table_stride), table[s, m] = the
+ * page of positions [m * page_size, (m + 1) * page_size) of sequence s or -1; lens int32 [n_seqs];
+ * refs int32 [pages] = how many table entries name a page (0: free). Full pages may have several
+ * holders, a partial last page has one. A fresh cache is table -1, lens 0, refs 0. At most 32768
+ * sequences; pages * page_size and width * page_size below 2^31; rows multiples of 4 bytes, pages and
+ * their stride multiples of 16, buffers 16-byte aligned. Lists of sequences are int32 on the device;
+ * negative entries are padding and do nothing. An entry that cannot be served is left as it was and
+ * counted in status[0] (int32 [2], never cleared here); status[1] counts the pages that were lacking.
+ * Page numbers outside [0, pages) in the table are never followed. Nothing is read back, nothing
+ * allocated; every call can be captured in a graph.
+ * No reference counterpart: racetrack's caches are [batch, max_len, dim] tensors
+ * (racetrack/models/deepseek.py:735-736).
+ */
+#define RT_PAGE_MAX_BUFFERS 128
+
+/*
+ * Sequence seqs[i] (NULL: i) grows by offsets[i + 1] - offsets[i] tokens (NULL: one each), tokens
+ * [offsets[i], offsets[i + 1]) of the list: takes the lowest free pages, in the order of the list, and
+ * writes where the rows of the tokens go: slots int32 [tokens], page * page_size + row, -1 for the tokens of
+ * entries that were not served (a number out of range, one that an earlier entry has named, more than
+ * width pages, no free page left) and for padding. workspace: rt_page_extend_workspace_ints(n, tokens) ints.
+ */
+int64_t rt_page_extend_workspace_ints(int64_t n, int64_t tokens);
+int rt_page_extend(int32_t* table, int64_t table_stride, int32_t* lens, int32_t* refs, int32_t* status,
+                   const int32_t* seqs, const int32_t* offsets, int32_t* slots, int32_t* workspace,
+                   int64_t n_seqs, int64_t width, int64_t pages, int64_t page_size, int64_t n, int64_t tokens,
+                   void* stream);
+
+/* Row t of rows[b] (row_strides[b] bytes apart) goes to slots[t] of buffer b; slots outside the pool are
+ * skipped. */
+int rt_page_write(void* const* bases, const int64_t* page_strides, const int64_t* row_bytes,
+                  const void* const* rows, const int64_t* row_strides, int64_t n_buffers,
+                  const int32_t* slots, int64_t tokens, int64_t pages, int64_t page_size, void* stream);
+
+/* The sequences of the list give their pages back and are empty (a second mention does nothing). */
+int rt_page_free(int32_t* table, int64_t table_stride, int32_t* lens, int32_t* refs, const int32_t* seqs,
+                 int64_t n_seqs, int64_t width, int64_t pages, int64_t n, void* stream);
+
+/*
+ * dst[i] becomes a copy of src[i]: it shares the full pages and gets the used rows of a partial last
+ * page in a page of its own; what dst[i] held before is given back. All entries take effect at once, so a
+ * sequence may be a source and a destination of one call (beams that change places); a destination
+ * is named once (later mentions are refused), src[i] == dst[i] does nothing. Pages are handed out before any
+ * are given back. workspace: rt_page_fork_workspace_ints(n, width) ints, 16-byte aligned.
+ */
+int64_t rt_page_fork_workspace_ints(int64_t n, int64_t width);
+int rt_page_fork(void* const* bases, const int64_t* page_strides, const int64_t* row_bytes, int64_t n_buffers,
+                 int32_t* table, int64_t table_stride, int32_t* lens, int32_t* refs, int32_t* status,
+                 const int32_t* src, const int32_t* dst, int32_t* workspace, int64_t n_seqs, int64_t width,
+                 int64_t pages, int64_t page_size, int64_t n, void* stream);
+
+/*
+ * Packs the pages in use into [0, live): the k-th lowest one outside that range moves into the k-th
+ * lowest free page inside it; table and refs follow. workspace: rt_page_compact_workspace_ints(pages)
+ * ints, 16-byte aligned; its first two ints are then live and the number of pages moved.
+ */
+int64_t rt_page_compact_workspace_ints(int64_t pages);
+int rt_page_compact(void* const* bases, const int64_t* page_strides, const int64_t* row_bytes,
+                    int64_t n_buffers, int32_t* table, int64_t table_stride, int32_t* refs, int32_t* workspace,
+                    int64_t n_seqs, int64_t width, int64_t pages, int64_t page_size, void* stream);
+
+/* Page from[i] of every buffer to page to[i] (int32 on the device; pairs with a number outside the pool are
+ * skipped). No page may be both read and written, and none written twice: the order is not defined. */
+int rt_page_copy(void* const* bases, const int64_t* page_strides, const int64_t* row_bytes, int64_t n_buffers,
+                 const int32_t* from, const int32_t* to, int64_t n, int64_t pages, int64_t page_size,
+                 void* stream);
+
 /*
  * Causal attention of the prefill stack on the tensor cores (flash-style: scores and
  * probabilities never leave the SM):

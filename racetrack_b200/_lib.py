@@ -72,6 +72,15 @@ SIGNATURES: dict[str, tuple] = {
     "rt_index_topk": (_I, [_P, _P, _L, _L, _L, _L, _P]),
     "rt_mla_sparse_decode_splits": (_L, [_L, _L, _L]),
     "rt_mla_sparse_decode": (_I, [_P] * 8 + [_L] * 14 + [_F, _P]),
+    "rt_page_extend_workspace_ints": (_L, [_L, _L]),
+    "rt_page_extend": (_I, [_P, _L] + [_P] * 7 + [_L] * 6 + [_P]),
+    "rt_page_write": (_I, [_P] * 5 + [_L, _P, _L, _L, _L, _P]),
+    "rt_page_free": (_I, [_P, _L, _P, _P, _P, _L, _L, _L, _L, _P]),
+    "rt_page_fork_workspace_ints": (_L, [_L, _L]),
+    "rt_page_fork": (_I, [_P] * 3 + [_L, _P, _L] + [_P] * 6 + [_L] * 5 + [_P]),
+    "rt_page_compact_workspace_ints": (_L, [_L]),
+    "rt_page_compact": (_I, [_P] * 3 + [_L, _P, _L, _P, _P] + [_L] * 4 + [_P]),
+    "rt_page_copy": (_I, [_P] * 3 + [_L, _P, _P, _L, _L, _L, _P]),
     "rt_attn_causal_prefill": (_I, [_P] * 5 + [_L] * 15 + [_F, _P]),
     "rt_attn_causal_prefill_fp8": (_I, [_P] * 6 + [_L] * 13 + [_F, _P]),
     "rt_attn_causal_prefill_share": (_I, [_P] * 7 + [_L] * 16 + [_F, _P]),

@@ -34,6 +34,7 @@ SOURCES = {
     "rt_moe.cu": ["-fmad=false"],
     "rt_gemm.cu": [],
     "rt_attn.cu": [],
+    "rt_page.cu": [],
     "rt_peer.cu": ["-fmad=false"],
 }
 

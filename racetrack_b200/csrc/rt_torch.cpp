@@ -5,6 +5,7 @@
 //
 // The module links against torch only. The kernel library's functions arrive as addresses
 // (bind()), so whatever library racetrack_b200/_lib.py has loaded is the one that runs.
+#include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/extension.h>
 
@@ -25,7 +26,10 @@ using OptTensor = std::optional<Tensor>;
     X(rt_moe_tile_map) X(rt_moe_plan) X(rt_absmax_onto) X(rt_swiglu_absmax_rows_onto) X(rt_moe_gather_nvfp4) X(rt_moe_quant_nvfp4) X(rt_moe_combine)             \
     X(rt_gemm_bf16) X(rt_gemm_bf16_splitk_splits) X(rt_gemm_bf16_splitk) X(rt_gemm_bf16_batched)  \
     X(rt_gemm_fp8) X(rt_gemm_nvfp4_grouped) X(rt_index_prep_into) X(rt_index_head_weights) X(rt_fp8_index_batched)              \
-    X(rt_index_topk) X(rt_mla_sparse_decode_splits) X(rt_mla_sparse_decode)
+    X(rt_index_topk) X(rt_mla_sparse_decode_splits) X(rt_mla_sparse_decode)                       \
+    X(rt_page_extend_workspace_ints) X(rt_page_extend) X(rt_page_write) X(rt_page_free)           \
+    X(rt_page_fork_workspace_ints) X(rt_page_fork) X(rt_page_compact_workspace_ints)              \
+    X(rt_page_compact) X(rt_page_copy)
 
 #define RT_POINTER(name) decltype(&::name) p_##name = nullptr;
 RT_TABLE(RT_POINTER)
@@ -796,6 +800,225 @@ Tensor mla_sparse_decode(const Tensor& q_abs, const Tensor& q_pe, const Tensor& 
     return out;
 }
 
+// ---- paged caches -----------------------------------------------------------------------------
+// These calls run on the device of their tensors, whichever is current, and on its current stream.
+
+// The tables of a paged cache: block_table [sequences, width], seq_lens [sequences], refcount [pages].
+struct Tables {
+    const Tensor &table, &lens, &refs;
+    int64_t seqs() const { return table.size(0); }
+    int64_t width() const { return table.size(1); }
+    int64_t pages() const { return refs.numel(); }
+    int64_t stride() const { return table.size(0) > 1 ? table.stride(0) : table.size(1); }
+};
+
+void require_ints(const std::string& who, const char* name, const Tensor& t, const Tensor& like, int64_t dims) {
+    if (t.scalar_type() != at::kInt || t.dim() != dims || t.device() != like.device())
+        fail(who + ": " + name + " must be int32 with " + std::to_string(dims) +
+             (dims == 1 ? " dimension" : " dimensions") + " on the device of the table");
+    if (t.numel() > 0 && t.size(-1) > 1 && t.stride(-1) != 1) fail(who + ": " + name + " must have a contiguous last dimension");
+}
+
+Tables page_tables(const std::string& who, const Tensor& table, const Tensor& lens, const Tensor& refs) {
+    require_cuda({&table});
+    require_ints(who, "block_table", table, table, 2);
+    require_ints(who, "seq_lens", lens, table, 1);
+    require_ints(who, "refcount", refs, table, 1);
+    if (lens.numel() != table.size(0)) fail(who + ": seq_lens must have one entry for each row of block_table");
+    if (table.size(0) > 1 && table.stride(0) < table.size(1)) fail(who + ": rows of block_table must not overlap");
+    return {table, lens, refs};
+}
+
+void require_status(const std::string& who, const Tensor& status, const Tensor& table) {
+    require_ints(who, "status", status, table, 1);
+    if (status.numel() != 2) fail(who + ": status must have two entries");
+}
+
+// A list of sequences or pages on the table's device.
+void require_list(const std::string& who, const char* name, const Tensor& t, const Tensor& table) {
+    require_ints(who, name, t, table, 1);
+}
+
+// Page buffers [pages, page_size, ...], rows contiguous within a page.
+struct PageBuffers {
+    std::vector<void*> bases;
+    std::vector<int64_t> strides, row_bytes;
+    int64_t n = 0, pages = 0, page = 1;
+};
+
+PageBuffers page_buffers(const std::string& who, const std::vector<Tensor>& buffers, const Tensor& like, int64_t pages) {
+    PageBuffers p;
+    p.n = static_cast<int64_t>(buffers.size());
+    p.pages = pages;
+    if (buffers.empty()) fail(who + ": at least one page buffer is required");
+    p.page = buffers[0].dim() >= 2 ? buffers[0].size(1) : 0;
+    for (const Tensor& b : buffers) {
+        if (!b.defined() || !b.is_cuda() || b.device() != like.device()) fail(who + ": page buffers must be on the device of the other tensors");
+        if (b.dim() < 2 || b.size(0) != pages || b.size(1) != p.page || p.page < 1)
+            fail(who + ": page buffers must be [pages, page_size, ...] with one entry of refcount a page");
+        int64_t row = 1, expect = 1;
+        for (int64_t d = b.dim() - 1; d >= 1; --d) {
+            if (b.size(d) > 1 && b.stride(d) != expect) fail(who + ": the rows of a page must be contiguous");
+            expect *= b.size(d);
+            if (d > 1) row *= b.size(d);
+        }
+        p.bases.push_back(b.data_ptr());
+        p.row_bytes.push_back(row * b.element_size());
+        p.strides.push_back((pages > 1 ? b.stride(0) : expect) * b.element_size());
+    }
+    return p;
+}
+
+Tensor extend(const std::string& who, const Tables& t, const Tensor& status, int64_t tokens, int64_t page,
+              const OptTensor& seqs, const OptTensor& offsets) {
+    require_status(who, status, t.table);
+    if (tokens < 0 || page < 1) fail(who + ": tokens and page_size must not be negative or zero");
+    if (seqs) require_list(who, "seqs", *seqs, t.table);
+    if (offsets) {
+        require_list(who, "offsets", *offsets, t.table);
+        if (offsets->numel() < 1) fail(who + ": offsets has one entry more than there are sequences");
+    }
+    const int64_t n = offsets ? offsets->numel() - 1 : seqs ? seqs->numel() : tokens;
+    if (seqs && seqs->numel() != n) fail(who + ": offsets must have one entry more than seqs");
+    if (!offsets && tokens != n) fail(who + ": without offsets every sequence of the list gets one token");
+    if (!seqs && n > t.seqs()) fail(who + ": more entries than the table has sequences");
+    Tensor slots = empty({tokens}, at::kInt, t.table);
+    Tensor work = empty({std::max<int64_t>(1, p_rt_page_extend_workspace_ints(n, tokens))}, at::kInt, t.table);
+    check(p_rt_page_extend(data<int32_t>(t.table), t.stride(), data<int32_t>(t.lens), data<int32_t>(t.refs),
+                           data<int32_t>(status), data<int32_t>(seqs), data<int32_t>(offsets), data<int32_t>(slots),
+                           data<int32_t>(work), t.seqs(), t.width(), t.pages(), page, n, tokens, stream()),
+          "rt_page_extend");
+    return slots;
+}
+
+Tensor page_extend(const Tensor& table, const Tensor& lens, const Tensor& refs, const Tensor& status, int64_t tokens,
+                   int64_t page_size, const OptTensor& seqs, const OptTensor& offsets) {
+    const Tables t = page_tables("page_extend", table, lens, refs);
+    const c10::cuda::CUDAGuard guard(table.device());
+    return extend("page_extend", t, status, tokens, page_size, seqs, offsets);
+}
+
+// The rows of a call, one tensor [tokens, ...] a buffer, and the copies that keep them alive.
+struct PageRows {
+    std::vector<Tensor> held;
+    std::vector<const void*> bases;
+    std::vector<int64_t> strides;
+    int64_t tokens = 0;
+};
+
+PageRows page_rows(const std::string& who, const std::vector<Tensor>& buffers, const std::vector<Tensor>& rows) {
+    PageRows r;
+    if (rows.size() != buffers.size()) fail(who + ": one tensor of rows for each page buffer is required");
+    r.tokens = rows[0].dim() >= 1 ? rows[0].size(0) : -1;
+    for (size_t i = 0; i < rows.size(); ++i) {
+        const Tensor &x = rows[i], &b = buffers[i];
+        if (!x.defined() || x.device() != b.device() || x.scalar_type() != b.scalar_type())
+            fail(who + ": rows must have the type and device of their page buffer");
+        if (x.dim() != b.dim() - 1 || x.size(0) != r.tokens || !x.sizes().slice(1).equals(b.sizes().slice(2)))
+            fail(who + ": rows must be [tokens, ...] with the rows of their page buffer");
+        int64_t expect = 1;
+        bool whole = true;
+        for (int64_t d = x.dim() - 1; d >= 1; --d) {
+            if (x.size(d) > 1 && x.stride(d) != expect) whole = false;
+            expect *= x.size(d);
+        }
+        const int64_t step = (r.tokens > 1 ? x.stride(0) : expect) * x.element_size();
+        if (!whole || step < 0 || step % 4 != 0 || reinterpret_cast<uintptr_t>(x.data_ptr()) % 4 != 0) {
+            r.held.push_back(x.contiguous());
+            if (r.held.back().data_ptr() == x.data_ptr()) r.held.back() = x.clone(at::MemoryFormat::Contiguous);
+            r.strides.push_back(expect * x.element_size());
+        } else {
+            r.held.push_back(x);
+            r.strides.push_back(step);
+        }
+        r.bases.push_back(r.held.back().data_ptr());
+    }
+    return r;
+}
+
+void write(const PageBuffers& p, const PageRows& r, const Tensor& slots) {
+    check(p_rt_page_write(p.bases.data(), p.strides.data(), p.row_bytes.data(), r.bases.data(), r.strides.data(), p.n,
+                          data<int32_t>(slots), r.tokens, p.pages, p.page, stream()),
+          "rt_page_write");
+}
+
+void page_write(const std::vector<Tensor>& buffers, const std::vector<Tensor>& rows, const Tensor& slots) {
+    require_cuda({&slots});
+    if (buffers.empty()) fail("page_write: at least one page buffer is required");
+    const PageBuffers p = page_buffers("page_write", buffers, slots, buffers[0].dim() ? buffers[0].size(0) : 0);
+    require_list("page_write", "slots", slots, slots);
+    const c10::cuda::CUDAGuard guard(slots.device());
+    const PageRows r = page_rows("page_write", buffers, rows);
+    if (slots.numel() != r.tokens) fail("page_write: one slot for each row is required");
+    write(p, r, slots);
+}
+
+Tensor page_append(const std::vector<Tensor>& buffers, const std::vector<Tensor>& rows, const Tensor& table,
+                   const Tensor& lens, const Tensor& refs, const Tensor& status, const OptTensor& seqs,
+                   const OptTensor& offsets) {
+    const Tables t = page_tables("page_append", table, lens, refs);
+    const PageBuffers p = page_buffers("page_append", buffers, table, t.pages());
+    const c10::cuda::CUDAGuard guard(table.device());
+    const PageRows r = page_rows("page_append", buffers, rows);
+    const Tensor slots = extend("page_append", t, status, r.tokens, p.page, seqs, offsets);
+    write(p, r, slots);
+    return slots;
+}
+
+void page_free(const Tensor& table, const Tensor& lens, const Tensor& refs, const Tensor& seqs) {
+    const Tables t = page_tables("page_free", table, lens, refs);
+    require_list("page_free", "seqs", seqs, table);
+    const c10::cuda::CUDAGuard guard(table.device());
+    check(p_rt_page_free(data<int32_t>(table), t.stride(), data<int32_t>(lens), data<int32_t>(refs), data<int32_t>(seqs),
+                         t.seqs(), t.width(), t.pages(), seqs.numel(), stream()),
+          "rt_page_free");
+}
+
+void page_fork(const std::vector<Tensor>& buffers, const Tensor& table, const Tensor& lens, const Tensor& refs,
+               const Tensor& status, const Tensor& src, const Tensor& dst) {
+    const Tables t = page_tables("page_fork", table, lens, refs);
+    const PageBuffers p = page_buffers("page_fork", buffers, table, t.pages());
+    require_status("page_fork", status, table);
+    require_list("page_fork", "src", src, table);
+    require_list("page_fork", "dst", dst, table);
+    if (src.numel() != dst.numel()) fail("page_fork: src and dst must have as many entries");
+    const c10::cuda::CUDAGuard guard(table.device());
+    Tensor work = empty({std::max<int64_t>(4, p_rt_page_fork_workspace_ints(src.numel(), t.width()))}, at::kInt, table);
+    check(p_rt_page_fork(p.bases.data(), p.strides.data(), p.row_bytes.data(), p.n, data<int32_t>(table), t.stride(),
+                         data<int32_t>(lens), data<int32_t>(refs), data<int32_t>(status), data<int32_t>(src),
+                         data<int32_t>(dst), data<int32_t>(work), t.seqs(), t.width(), t.pages(), p.page, src.numel(),
+                         stream()),
+          "rt_page_fork");
+}
+
+Tensor page_compact(const std::vector<Tensor>& buffers, const Tensor& table, const Tensor& refs) {
+    require_cuda({&table});
+    require_ints("page_compact", "block_table", table, table, 2);
+    require_ints("page_compact", "refcount", refs, table, 1);
+    if (table.size(0) > 1 && table.stride(0) < table.size(1)) fail("page_compact: rows of block_table must not overlap");
+    const Tables t{table, refs, refs};
+    const PageBuffers p = page_buffers("page_compact", buffers, table, t.pages());
+    const c10::cuda::CUDAGuard guard(table.device());
+    Tensor work = empty({p_rt_page_compact_workspace_ints(t.pages())}, at::kInt, table);
+    check(p_rt_page_compact(p.bases.data(), p.strides.data(), p.row_bytes.data(), p.n, data<int32_t>(table), t.stride(),
+                            data<int32_t>(refs), data<int32_t>(work), t.seqs(), t.width(), t.pages(), p.page, stream()),
+          "rt_page_compact");
+    return work.narrow(0, 0, 2);
+}
+
+void page_copy(const std::vector<Tensor>& buffers, const Tensor& src, const Tensor& dst) {
+    require_cuda({&src});
+    if (buffers.empty()) fail("page_copy: at least one page buffer is required");
+    const PageBuffers p = page_buffers("page_copy", buffers, src, buffers[0].dim() ? buffers[0].size(0) : 0);
+    require_list("page_copy", "src", src, src);
+    require_list("page_copy", "dst", dst, src);
+    if (src.numel() != dst.numel()) fail("page_copy: src and dst must have as many entries");
+    const c10::cuda::CUDAGuard guard(src.device());
+    check(p_rt_page_copy(p.bases.data(), p.strides.data(), p.row_bytes.data(), p.n, data<int32_t>(src),
+                         data<int32_t>(dst), src.numel(), p.pages, p.page, stream()),
+          "rt_page_copy");
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_rt_torch, m) {
@@ -836,5 +1059,12 @@ PYBIND11_MODULE(_rt_torch, m) {
     RT_DEF(fp8_index);
     RT_DEF(index_topk);
     RT_DEF(mla_sparse_decode);
+    RT_DEF(page_extend);
+    RT_DEF(page_write);
+    RT_DEF(page_append);
+    RT_DEF(page_free);
+    RT_DEF(page_fork);
+    RT_DEF(page_compact);
+    RT_DEF(page_copy);
 #undef RT_DEF
 }

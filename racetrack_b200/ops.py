@@ -504,6 +504,69 @@ def mla_sparse_decode(q_abs: torch.Tensor, q_pe: torch.Tensor, kv_cache: torch.T
     return _native().mla_sparse_decode(q_abs, q_pe, kv_cache, pe_cache, indices, softmax_scale)
 
 
+# ---------------------------------------------------------------------------
+# paged caches
+# ---------------------------------------------------------------------------
+# One block table serves any number of page buffers [n_pages, page_size, ...] (a layer's latent rows
+# and rope keys, all layers' at once): block_table int32 [S, M], block_table[s, m] the page of
+# positions [m * page_size, (m + 1) * page_size) of sequence s or -1; seq_lens int32 [S]; refcount
+# int32 [n_pages], how many table entries name a page (0: free); status int32 [2], entries refused so
+# far and pages that were lacking. A fresh cache is -1, 0, 0, 0 (paging.PagedCaches makes one). Lists
+# of sequences are int32 on the device, negative entries are padding. The calls change the tables
+# in place, between calls nothing else should; they read nothing back and can be captured in a graph. racetrack's
+# caches are [batch, max_len, dim] tensors (racetrack/models/deepseek.py:735-736): no counterpart.
+
+def page_extend(block_table: torch.Tensor, seq_lens: torch.Tensor, refcount: torch.Tensor, status: torch.Tensor,
+                tokens: int, page_size: int, seqs: Optional[torch.Tensor] = None, *,
+                offsets: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Sequence seqs[i] (default: i) grows by offsets[i + 1] - offsets[i] tokens (default: one each;
+    offsets ascending from 0 to at most `tokens`). Takes the lowest free pages in the order of the list
+    and returns slots int32 [tokens], the row page * page_size + r where each token's rows go (page_write).
+    An entry that cannot grow (out of range, named before in the list, beyond M pages, no free page left)
+    stays as it was, its tokens get slot -1, and status[0] counts it."""
+    return _native().page_extend(block_table, seq_lens, refcount, status, tokens, page_size, seqs, offsets)
+
+
+def page_write(pages, rows, slots: torch.Tensor) -> None:
+    """rows[b][t] into row slots[t] of every buffer pages[b]; slots outside the pool are skipped.
+    rows[b] is [tokens, ...] of the buffer's type, its rows at any pitch."""
+    _native().page_write(list(pages), list(rows), slots)
+
+
+def page_append(pages, rows, block_table: torch.Tensor, seq_lens: torch.Tensor, refcount: torch.Tensor,
+                status: torch.Tensor, seqs: Optional[torch.Tensor] = None, *,
+                offsets: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """page_extend by the rows given, and page_write of them; returns the slots."""
+    return _native().page_append(list(pages), list(rows), block_table, seq_lens, refcount, status, seqs, offsets)
+
+
+def page_free(block_table: torch.Tensor, seq_lens: torch.Tensor, refcount: torch.Tensor, seqs: torch.Tensor) -> None:
+    """The sequences of the list give their pages back and are empty; one that is named twice does so once."""
+    _native().page_free(block_table, seq_lens, refcount, seqs)
+
+
+def page_fork(pages, block_table: torch.Tensor, seq_lens: torch.Tensor, refcount: torch.Tensor, status: torch.Tensor,
+              src: torch.Tensor, dst: torch.Tensor) -> None:
+    """Sequence dst[i] becomes a copy of src[i]: it shares the full pages, gets the used rows of a partial
+    last page in a page of its own, and gives back what it held. All entries take effect at once, so a
+    sequence may be source and destination of one call (beams that change places). A destination is named
+    once, later mentions are refused; src[i] == dst[i] does nothing. New pages are taken, lowest first in the
+    order of the list, before any return."""
+    _native().page_fork(list(pages), block_table, seq_lens, refcount, status, src, dst)
+
+
+def page_compact(pages, block_table: torch.Tensor, refcount: torch.Tensor) -> torch.Tensor:
+    """Packs the n pages in use into [0, n): the k-th lowest one outside moves into the k-th lowest free one
+    inside, in every buffer; table and refcount follow. Returns int32 [2]: n and the pages moved."""
+    return _native().page_compact(list(pages), block_table, refcount)
+
+
+def page_copy(pages, src: torch.Tensor, dst: torch.Tensor) -> None:
+    """Page src[i] of every buffer to page dst[i] (int32 lists; pairs outside the pool are skipped). A page
+    may be read any number of times; none is both read and written, or written twice."""
+    _native().page_copy(list(pages), src, dst)
+
+
 def attention_prefill(q: torch.Tensor, k_nope: torch.Tensor, k_pe: Optional[torch.Tensor],
                       v: torch.Tensor, softmax_scale: Optional[float] = None, *,
                       quantized: bool = False, out: Optional[tuple] = None,
