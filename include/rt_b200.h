@@ -658,6 +658,33 @@ int rt_mla_sparse_decode(const void* q_abs, const void* q_pe, const void* kv, co
 #define RT_PAGE_MAX_BUFFERS 128
 
 /*
+ * Attention of one new token a sequence over the pages of a latent cache (MLA decode, tcgen05):
+ *   s_j      = softmax_scale * (q_abs[b, h, :] . kv[j, :] + q_pe[b, h, :] . pe[j, :])
+ *   out[b, h] = sum_j softmax(s)_j * kv[j, :]
+ * over the positions j of row b's sequence that its newest token sees: j < L, and with window > 0 those with
+ * j >= L - window or j < sinks. Row b is sequence seqs[b] (NULL: b); L = lens[seq], cut to width * page_size;
+ * a sequence out of [0, slots), a length of zero and positions whose page number lies outside [0, pages) give
+ * and weigh nothing (a row without any position is zero). What memory holds behind a sequence's end, or at
+ * positions it does not see, NaN included, does not reach the output. An infinite or NaN value of a row that is
+ * seen may reach all 512 dims of the output.
+ * q_abs bf16 [batch, heads, 512], q_pe bf16 [batch, heads, 64], kv bf16 [pages, page_size, 512], pe bf16
+ * [pages, page_size, 64] (strides in elements, multiples of 8, pointers 16-byte aligned), table int32 [slots,
+ * width], out bf16 [batch, heads, 512] contiguous. page_size: a power of two, 16 or more; heads up to 1024;
+ * batch up to 65535. The sequences' tiles are cut evenly over the SMs on the device; a second kernel joins
+ * what was cut, in the order of the positions. workspace: rt_mla_paged_decode_workspace_bytes(heads), 16-byte
+ * aligned, of one call at a time. No allocation, no host synchronisation.
+ * ref: racetrack/models/deepseek.py:793-810 (MLA.forward, "MQA decode", without the indexer's mask).
+ */
+int64_t rt_mla_paged_decode_workspace_bytes(int64_t heads);
+int rt_mla_paged_decode(const void* q_abs, const void* q_pe, const void* kv, const void* pe,
+                        const int32_t* table, const int32_t* lens, const int32_t* seqs, void* out,
+                        void* workspace, int64_t batch, int64_t heads, int64_t slots, int64_t width,
+                        int64_t pages, int64_t page_size, int64_t qa_batch_stride, int64_t qa_head_stride,
+                        int64_t qp_batch_stride, int64_t qp_head_stride, int64_t kv_page_stride,
+                        int64_t kv_row_stride, int64_t pe_page_stride, int64_t pe_row_stride,
+                        int64_t table_stride, int64_t window, int64_t sinks, float softmax_scale, void* stream);
+
+/*
  * Sequence seqs[i] (NULL: i) grows by offsets[i + 1] - offsets[i] tokens (NULL: one each), tokens
  * [offsets[i], offsets[i + 1]) of the list: takes the lowest free pages, in the order of the list, and
  * writes where the rows of the tokens go: slots int32 [tokens], page * page_size + row, -1 for the tokens of

@@ -72,6 +72,8 @@ SIGNATURES: dict[str, tuple] = {
     "rt_index_topk": (_I, [_P, _P, _L, _L, _L, _L, _P]),
     "rt_mla_sparse_decode_splits": (_L, [_L, _L, _L]),
     "rt_mla_sparse_decode": (_I, [_P] * 8 + [_L] * 14 + [_F, _P]),
+    "rt_mla_paged_decode_workspace_bytes": (_L, [_L]),
+    "rt_mla_paged_decode": (_I, [_P] * 9 + [_L] * 17 + [_F, _P]),
     "rt_page_extend_workspace_ints": (_L, [_L, _L]),
     "rt_page_extend": (_I, [_P, _L] + [_P] * 7 + [_L] * 6 + [_P]),
     "rt_page_write": (_I, [_P] * 5 + [_L, _P, _L, _L, _L, _P]),

@@ -35,6 +35,7 @@ SOURCES = {
     "rt_gemm.cu": [],
     "rt_attn.cu": [],
     "rt_page.cu": [],
+    "rt_paged_attn.cu": [],
     "rt_peer.cu": ["-fmad=false"],
 }
 

@@ -1890,21 +1890,32 @@ int make_tmap_rows128_batched(CUtensorMap* map, const void* ptr, uint64_t rows, 
 
 // 4-D bf16 tensor map with the 128-byte swizzle for the attention kernels (rt_attn.cu): dims and
 // box are given fastest dimension first, strides in bytes for dimensions 1..3.
-int make_tmap_bf16_4d(CUtensorMap* map, const void* ptr, const uint64_t dims_in[4],
-                      const uint64_t strides_in[3], const uint32_t box_in[4]) {
+// Tensor map of bf16 data, 128-byte swizzle, reads outside it as zeros: `rank` dims (the first contiguous),
+// strides in bytes of the others.
+int make_tmap_bf16(CUtensorMap* map, const void* ptr, int rank, const uint64_t* dims_in, const uint64_t* strides_in,
+                   const uint32_t* box_in) {
     EncodeTiledFn fn = encode_fn();
     RT_REQUIRE(fn, RT_ERR_CUDA, "cuTensorMapEncodeTiled is not available from this driver");
-    const cuuint64_t dims[4] = {dims_in[0], dims_in[1], dims_in[2], dims_in[3]};
-    const cuuint64_t strides[3] = {strides_in[0], strides_in[1], strides_in[2]};
-    const cuuint32_t box[4] = {box_in[0], box_in[1], box_in[2], box_in[3]};
-    const cuuint32_t estr[4] = {1, 1, 1, 1};
-    const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(ptr), dims,
+    cuuint64_t dims[5], strides[4];
+    cuuint32_t box[5], estr[5];
+    for (int i = 0; i < rank; ++i) {
+        dims[i] = dims_in[i];
+        box[i] = box_in[i];
+        estr[i] = 1;
+        if (i > 0) strides[i - 1] = strides_in[i - 1];
+    }
+    const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, static_cast<cuuint32_t>(rank), const_cast<void*>(ptr), dims,
                           strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
                           CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    RT_REQUIRE(r == CUDA_SUCCESS, RT_ERR_CUDA, "cuTensorMapEncodeTiled (4-D) failed with CUresult %d",
+    RT_REQUIRE(r == CUDA_SUCCESS, RT_ERR_CUDA, "cuTensorMapEncodeTiled (%d-D) failed with CUresult %d", rank,
                static_cast<int>(r));
     return RT_OK;
+}
+
+int make_tmap_bf16_4d(CUtensorMap* map, const void* ptr, const uint64_t dims[4], const uint64_t strides[3],
+                      const uint32_t box[4]) {
+    return make_tmap_bf16(map, ptr, 4, dims, strides, box);
 }
 
 int sm_count() {
@@ -2528,7 +2539,7 @@ extern "C" int rt_gemm_bf16_splitk(const void* a, const void* b, float* workspac
                                   static_cast<int>(splits), as_stream(stream));
 }
 
-namespace rt { namespace tc { int attn_error_take(); } }   // the flag of the attention kernels (rt_attn.cu)
+namespace rt { namespace tc { int attn_error_take(); int paged_attn_error_take(); } }   // the flags of the attention kernels (rt_attn.cu, rt_paged_attn.cu)
 
 extern "C" int rt_tc_error_state(void) {
     int v = 0;
@@ -2536,7 +2547,9 @@ extern "C" int rt_tc_error_state(void) {
         cudaGetLastError();
         return fail(RT_ERR_CUDA, "rt_tc_error_state: cannot read the device flag");
     }
-    const int va = tc::attn_error_take();
+    const int vp = tc::paged_attn_error_take();
+    int va = tc::attn_error_take();
+    if (va == 0 || vp < 0) va = vp;
     if (va < 0) return fail(RT_ERR_CUDA, "rt_tc_error_state: cannot read the device flag");
     if (v == 0 && va > 0)
         return fail(RT_ERR_TIMEOUT, "a tensor-core kernel abandoned wait #%d (bounded spin expired)", va);

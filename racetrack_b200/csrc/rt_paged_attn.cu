@@ -1,0 +1,821 @@
+// Attention of one new token a sequence over a paged latent cache (the MLA decode step):
+//
+//   out[b, h, :] = sum_j p_j kv[j, :],   p = softmax_j( scale * (q_abs[b, h, :] . kv[j, :] + q_pe[b, h, :] . pe[j, :]) )
+//
+// over the positions j of sequence b that its newest token (position L - 1) sees: all j < L, or under a
+// window of W positions with s sinks those with j >= L - W or j < s. kv [pages, page, 512] and pe [pages,
+// page, 64] hold the rows, block_table their pages. The dense counterpart of mla_sparse_decode_kernel
+// (racetrack/models/deepseek.py:793-810 without the indexer's mask).
+//
+// A row of 1152 bytes serves 2 * 1088 flops for each head, 242 flop/B at 128 heads: with few heads the
+// kernel is bound by reading the cache once, with all of them memory and tensor cores take about the same.
+#include "rt_tc.cuh"
+
+namespace rt {
+namespace tc {
+
+constexpr int kPTile = 64;                          // positions per tile
+constexpr uint32_t kPLatBytes = kPTile * 1024;      // latent part of a tile
+constexpr uint32_t kPTileBytes = kPTile * 1152;
+constexpr int kPMaxBatch = 65535;
+
+// ---- which CTA walks which tiles --------------------------------------------------------------
+// The visible positions of row b are the tiles {0 .. na - 1} (sinks) and {b0 .. b0 + nb - 1} of 64
+// positions. All rows' tiles in one line are cut into as many equal ranges as there are CTAs, so
+// ragged lengths keep every SM busy alike; a row that crosses from one range into the next is finished by
+// the merge kernel. The host knows no length: each CTA sums them itself.
+struct PagedArgs {
+    const int32_t* table;         // [slots, width]
+    const int32_t* lens;          // [slots]
+    const int32_t* seqs;          // [batch] or null: row b is slot b
+    __nv_bfloat16* out;           // [batch, heads, 512]
+    int4* ranges;                 // [ranges]: row, tile within it, its tiles, tiles per range
+    float* part_ml;               // [2 ranges, heads, 2]: running maximum, denominator
+    float* part_o;                // [2 ranges, heads, 512], not normalised
+    int64_t table_stride;
+    int batch, heads, slots, width, pages;
+    int page_log;                 // log2(page size)
+    int window, sinks;            // window 0: none
+    int n_ranges;
+    int group;                    // heads of a CTA
+    float scale_log2;
+};
+
+struct RowTiles {
+    int len, na, b0, n;           // length, sink tiles, first window tile, all tiles
+};
+
+__device__ __forceinline__ int row_slot(const PagedArgs& a, int b) {
+    const int s = a.seqs ? __ldg(a.seqs + b) : b;
+    return s >= 0 && s < a.slots ? s : -1;
+}
+
+__device__ __forceinline__ RowTiles row_tiles(const PagedArgs& a, int b) {
+    const int s = row_slot(a, b);
+    const int most = a.width << a.page_log;
+    RowTiles t;
+    t.len = s < 0 ? 0 : min(max(__ldg(a.lens + s), 0), most);
+    const int all = (t.len + kPTile - 1) / kPTile;
+    if (a.window == 0 || a.window >= t.len) {
+        t.na = 0;
+        t.b0 = 0;
+        t.n = all;
+    } else {
+        t.na = (min(a.sinks, t.len) + kPTile - 1) / kPTile;
+        t.b0 = max(t.na, (t.len - a.window) / kPTile);
+        t.n = t.na + max(0, all - t.b0);
+    }
+    return t;
+}
+
+__device__ __forceinline__ int tile_of(const RowTiles& t, int j) { return j < t.na ? j : t.b0 + (j - t.na); }
+
+// Bit i: position 64 * tile + i is visible (by its position alone).
+__device__ __forceinline__ uint64_t tile_mask(const PagedArgs& a, const RowTiles& t, int tile) {
+    const int p0 = tile * kPTile;
+    auto below = [&](int x) {                        // positions p0 .. x - 1
+        const int n = x - p0;
+        return n <= 0 ? 0ull : n >= 64 ? ~0ull : (1ull << n) - 1;
+    };
+    uint64_t m = below(t.len);
+    if (a.window != 0 && a.window < t.len) m &= ~below(t.len - a.window) | below(a.sinks);
+    return m;
+}
+
+// The range of this CTA: its first row and tile, and how many tiles it walks. All threads (kPThreads) call
+// it; every thread sums the rows of one slice of the batch.
+struct RangeStart {
+    int row, tile, count;
+};
+template <int THREADS>
+__device__ RangeStart find_range(const PagedArgs& a, int range) {
+    __shared__ int warp_sum[THREADS / 32];
+    __shared__ int found[3];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int per = (a.batch + THREADS - 1) / THREADS;
+    const int b0 = min(static_cast<int>(threadIdx.x) * per, a.batch), b1 = min(b0 + per, a.batch);
+    int mine = 0;
+    for (int b = b0; b < b1; ++b) mine += row_tiles(a, b).n;
+    int x = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= o) x += y;
+    }
+    if (lane == 31) warp_sum[warp] = x;
+    if (threadIdx.x == 0) {
+        found[0] = -1;
+        found[1] = found[2] = 0;
+    }
+    __syncthreads();
+    int before = x - mine, total = 0;
+#pragma unroll
+    for (int w = 0; w < THREADS / 32; ++w) {
+        if (w < warp) before += warp_sum[w];
+        total += warp_sum[w];
+    }
+    const int per_range = (total + a.n_ranges - 1) / a.n_ranges;
+    const int first = range * per_range;             // below 2^31: the host bounds batch * tiles
+    if (first >= before && first < before + mine) {
+        int at = before, b = b0;
+        RowTiles t = row_tiles(a, b);
+        while (at + t.n <= first) {
+            at += t.n;
+            t = row_tiles(a, ++b);
+        }
+        found[0] = b;
+        found[1] = first - at;
+        found[2] = t.n;
+    }
+    __syncthreads();
+    RangeStart r{found[0], found[1], 0};
+    if (r.row >= 0) r.count = min(per_range, total - first);
+    if (threadIdx.x == 0) a.ranges[range] = make_int4(r.row, found[1], found[2], per_range);
+    return r;
+}
+
+// ---- one CTA, up to 32 heads --------------------------------------------------------------------
+// Work of a CTA: its range of tiles for one group of G <= 32 heads. Per tile of 64 positions:
+//   producer  one TMA box a page brings the latent rows as [8-row groups][8 blocks of 64 dims][8 rows][128
+//             B] (128-byte swizzle), one the rope keys: a page of any size lands in the same
+//             layout, of which both products read their operand (the group stride is a field of the
+//             descriptor), so the rows are staged once. Two tiles in flight (144 KB: what an SM's share
+//             of the memory rate needs, some 44 KB, three times over);
+//   S = Q K^T 36 tcgen05.mma (M = 128 rows of which G are heads, N = 64, K = 16), K-major operands;
+//   softmax   one thread a head: running maximum with a lazy rescale (only when it grows by more than
+//             2^8), P = 2^(s - m) as bf16 into shared memory. Sums, maxima and O stay fp32; P is rounded to
+//             bf16 because the tensor core multiplies it with bf16 rows (relative 2^-9 a
+//             probability, no more than the rows' own rounding);
+//   O += P V  the tile again as the MN-major operand. 512 dims would fill tensor memory as columns;
+//             they are folded into the lanes: P lies between zero rows, and the MMA whose A operand starts
+//             32 f rows before P puts dims [128 f, 128 f + 128) of head r into lane 32 f + r, all four in the
+//             same 128 columns. Only the 16-position steps that hold a visible position are multiplied.
+// Positions that are not visible weigh exactly nothing whatever their memory holds: their scores are never
+// looked at, and their rows are zeroed in shared memory between the two products (0 * NaN).
+// A page number outside the pool reads as zeros (the TMA unit's bounds) and its positions are not visible.
+constexpr int kPThreads = 256;                       // 0 MMA, 1 producer, 4-7 softmax / lanes
+constexpr int kPMaxG = 32;
+constexpr uint32_t kPQRow = 9 * 128;                 // bytes of a staged head
+constexpr uint32_t kPQOff = 0;                       // two of up to 16 heads or one of up to 32
+constexpr uint32_t kPKOff = kPMaxG * kPQRow;
+constexpr uint32_t kPPOff = kPKOff + 2 * kPTileBytes;        // 96 zero rows | P: 32 rows of 128 B | 96 zero rows
+constexpr uint32_t kPBarOff = kPPOff + 224 * 128;
+constexpr int kPBars = 15;      // qfull[2] qfree[2] kfull[2] kfree[2] sfull[2] afull[2] pfull pfree ofree
+constexpr uint32_t kPInfoOff = kPBarOff + kPBars * 8 + 24;   // (tensor memory slot, abort flag before it)
+constexpr uint32_t kPAlphaOff = kPInfoOff + 2 * 16;          // rescale factors [2][32], grow flags [2]
+constexpr uint32_t kPMlOff = kPAlphaOff + (2 * 32 + 2) * 4;  // denominators [2][32]
+constexpr uint32_t kPSmemBytes = kPMlOff + 2 * 32 * 4 + 1024;
+static_assert(kPKOff % 1024 == 0 && kPPOff % 1024 == 0 && kPInfoOff % 16 == 0, "alignment");
+static_assert(kPSmemBytes <= 232448, "shared memory budget");
+constexpr uint32_t kPTmemS = 128;                    // O: columns [0, 128); S: two buffers of 64
+constexpr uint32_t kPSIdesc = (1u << 4) | (1u << 7) | (1u << 10) | ((kPTile >> 3) << 17) | (8u << 24);
+constexpr uint32_t kPOIdesc = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | (16u << 17) | (8u << 24);
+
+struct TileInfo {
+    uint64_t mask;
+    int32_t row;
+    int32_t flags;                // 1: first tile of the row in this range, 2: last one, 4: the row's first, 8: its last
+};
+
+// Descriptor with a stride between 8-row groups of its own (K-major: rows of one 64-dim block; MN-major: K
+// indices, `lbo` between 64-element blocks).
+__device__ __forceinline__ uint64_t smem_desc_groups(uint32_t addr, uint32_t lbo, uint32_t sbo) {
+    return static_cast<uint64_t>((addr & 0x3ffffu) >> 4) | (static_cast<uint64_t>(lbo >> 4) << 16) |
+           (static_cast<uint64_t>(sbo >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+
+__device__ __forceinline__ void tma_load_5d(uint32_t dst, const CUtensorMap* m, int c0, int c1, int c2, int c3,
+                                            int c4, uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.5d.shared::cluster.global.mbarrier::complete_tx::bytes "
+        "[%0], [%1, {%3, %4, %5, %6, %7}], [%2];" ::"r"(dst),
+        "l"(m), "r"(bar), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(c4)
+        : "memory");
+}
+
+__device__ __forceinline__ float exp2_fast(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// mbar_wait of a whole warp: all lanes go on or none does (a lane whose cycle budget runs out while another
+// still sees the phase complete must not leave the warp's shuffles behind).
+__device__ __forceinline__ bool mbar_wait_warp(uint32_t bar, uint32_t parity, volatile int* abort, int code) {
+    return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort, code));
+}
+
+// Where the result of a row's tiles in a range goes: the row's own output if they are all of its tiles, else
+// the range's slot for a row that began in an earlier range (2 r) or ends in a later one (2 r + 1).
+__device__ __forceinline__ int part_slot(int flags, int range) {
+    return (flags & 12) == 12 ? -1 : 2 * range + ((flags & 4) ? 1 : 0);
+}
+
+__global__ void __launch_bounds__(kPThreads, 1) mla_paged_kernel(const __grid_constant__ CUtensorMap tm_qa,
+                                                                 const __grid_constant__ CUtensorMap tm_qp,
+                                                                 const __grid_constant__ CUtensorMap tm_kv,
+                                                                 const __grid_constant__ CUtensorMap tm_pe,
+                                                                 const PagedArgs a) {
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    uint8_t* base_ptr = smem_raw + (base - smem_u32(smem_raw));
+    const uint32_t bars = base + kPBarOff;
+    auto qfull = [&](int s) { return bars + 8u * s; };
+    auto qfree = [&](int s) { return bars + 8u * (2 + s); };
+    auto kfull = [&](int s) { return bars + 8u * (4 + s); };
+    auto kfree = [&](int s) { return bars + 8u * (6 + s); };
+    auto sfull = [&](int s) { return bars + 8u * (8 + s); };
+    auto afull = [&](int s) { return bars + 8u * (10 + s); };
+    const uint32_t pfull = bars + 8u * 12, pfree = bars + 8u * 13, ofree = bars + 8u * 14;
+    const uint32_t slot = bars + 8u * kPBars;
+    volatile uint32_t* slot_ptr = reinterpret_cast<volatile uint32_t*>(base_ptr + kPBarOff + 8 * kPBars);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(slot_ptr + 1);
+    volatile TileInfo* info_s = reinterpret_cast<volatile TileInfo*>(base_ptr + kPInfoOff);
+
+    const int warp = uniform_warp_id(), lane = threadIdx.x & 31;
+    const int groups = (a.heads + a.group - 1) / a.group;
+    const int hg = blockIdx.x % groups, range = blockIdx.x / groups;
+    const int G = a.group;                                     // multiple of 8
+    const int q_bufs = G <= 16 ? 2 : 1;
+
+    if (threadIdx.x == 0) {
+        *abort_flag = 0;
+        for (int s = 0; s < 2; ++s) {
+            mbar_init(qfull(s), 1);
+            mbar_init(qfree(s), 1);
+            mbar_init(kfull(s), 1);
+            mbar_init(kfree(s), 1);
+            mbar_init(sfull(s), 1);
+            mbar_init(afull(s), 1);
+        }
+        mbar_init(pfull, 4);
+        mbar_init(pfree, 1);
+        mbar_init(ofree, 4);
+        fence_mbar_init();
+        tma_prefetch_desc(&tm_qa);
+        tma_prefetch_desc(&tm_qp);
+        tma_prefetch_desc(&tm_kv);
+        tma_prefetch_desc(&tm_pe);
+    }
+    if (warp == 0) {
+        tmem_alloc(slot, 256);
+        tmem_relinquish();
+    }
+    // zero rows around P (P's own rows are written before they are read)
+    for (int c = threadIdx.x; c < 224 * 8; c += kPThreads)
+        *reinterpret_cast<uint4*>(base_ptr + kPPOff + c * 16) = make_uint4(0u, 0u, 0u, 0u);
+    fence_proxy_async();
+    const RangeStart start = find_range<kPThreads>(a, range);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem_base = *slot_ptr;
+    const int n_tiles = start.count;
+
+    if (warp == 0) {
+        if (n_tiles > 0 && elect_one()) {
+            bool ok = true;
+            int q = 0, v = 0, q_seg = 0, v_seg = 0;            // tiles scored and accumulated, and their rows
+            bool q_open = false, v_open = false;               // the current row's first tile has been taken
+            uint32_t acc = 0;
+            long long t0 = 0;
+            uint32_t spins = 0;
+            // scores of the next landed tile or P V of the tile whose probabilities are written, whichever
+            // is ready first
+            while (ok && v < n_tiles) {
+                bool progressed = false;
+                if (q < n_tiles && q - v < 2 && mbar_try_wait(kfull(q & 1), (q >> 1) & 1)) {
+                    const int flags = info_s[q & 1].flags;
+                    const int qb = q_bufs == 2 ? (q_seg & 1) : 0;
+                    if (q_open || mbar_try_wait(qfull(qb), (q_bufs == 2 ? q_seg >> 1 : q_seg) & 1)) {
+                        tc_fence_after();
+                        const uint32_t kb = base + kPKOff + (q & 1) * kPTileBytes;
+                        const uint32_t qa = base + kPQOff + qb * (16 * kPQRow);
+                        const uint32_t d = tmem_base + kPTmemS + static_cast<uint32_t>(q & 1) * kPTile;
+#pragma unroll
+                        for (int c = 0; c < 9; ++c) {
+                            const uint64_t adesc = smem_desc_sw128(qa + c * G * 128);
+                            const uint64_t bdesc = c < 8 ? smem_desc_groups(kb + c * 1024, 16, 8192)
+                                                         : smem_desc_sw128(kb + kPLatBytes);
+#pragma unroll
+                            for (int j = 0; j < 4; ++j)
+                                mma_f16(d, adesc + 2u * j, bdesc + 2u * j, kPSIdesc, (c | j) != 0 ? 1u : 0u);
+                        }
+                        mma_commit(sfull(q & 1));
+                        q_open = true;
+                        if (flags & 2) {
+                            mma_commit(qfree(qb));
+                            ++q_seg;
+                            q_open = false;
+                        }
+                        ++q;
+                        progressed = true;
+                    }
+                }
+                if (v < q && mbar_try_wait(pfull, v & 1) &&
+                    (v_open || v_seg == 0 || mbar_try_wait(ofree, (v_seg - 1) & 1))) {
+                    tc_fence_after();
+                    const uint64_t mask = info_s[v & 1].mask;
+                    const int flags = info_s[v & 1].flags;
+                    if (!v_open) acc = 0;
+                    const uint32_t kb = base + kPKOff + (v & 1) * kPTileBytes;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        if ((mask >> (16 * j) & 0xffffu) == 0) continue;
+#pragma unroll
+                        for (int f = 0; f < 4; ++f) {
+                            const uint64_t adesc = smem_desc_sw128(base + kPPOff + (96 - 32 * f) * 128);
+                            const uint64_t bdesc = smem_desc_groups(kb + j * 16384 + f * 2048, 1024, 8192);
+                            mma_f16(tmem_base, adesc + 2u * j, bdesc, kPOIdesc, acc);
+                            acc = 1;
+                        }
+                    }
+                    mma_commit(kfree(v & 1));
+                    mma_commit(pfree);
+                    v_open = true;
+                    if (flags & 2) {
+                        ++v_seg;
+                        v_open = false;
+                    }
+                    ++v;
+                    progressed = true;
+                }
+                if (progressed) {
+                    spins = 0;
+                } else if ((++spins & 63u) == 0) {
+                    if (spins == 64) t0 = clock64();
+                    if (*abort_flag) ok = false;
+                    else if (clock64() - t0 > kWaitCycles) {
+                        *abort_flag = 81;
+                        atomicCAS(&g_tc_error, 0, 81);
+                        ok = false;
+                    }
+                }
+            }
+        }
+        __syncwarp();
+    } else if (warp == 1) {
+        // the whole warp walks the range (lanes fetch page numbers), one thread issues the loads
+        int b = start.row, j = start.tile, seg = 0;
+        RowTiles t{};
+        int row_at = -1;
+        int slot_row = -1;
+        const int page = 1 << a.page_log;
+        const int boxes = page < kPTile ? kPTile / page : 1;   // pages of a tile
+        bool ok = true;
+        int32_t fetched = -1;                                   // lane: page number of entry fetched0 + lane
+        int fetched0 = -1, fetched_row = -1;
+        for (int g = 0; ok && g < n_tiles; ++g) {
+            if (row_at != b) {
+                t = row_tiles(a, b);
+                while (j >= t.n) {                              // rows without a tile
+                    t = row_tiles(a, ++b);
+                    j = 0;
+                }
+                row_at = b;
+                slot_row = row_slot(a, b);
+            }
+            const bool first = g == 0 || j == 0;
+            const bool last = g == n_tiles - 1 || j == t.n - 1;
+            const int tile = tile_of(t, j);
+            const int m0 = (tile * kPTile) >> a.page_log;       // first entry of the row's table
+            if (fetched_row != b || m0 < fetched0 || m0 + boxes > fetched0 + 32) {
+                fetched0 = m0;
+                fetched_row = b;
+                const int m = m0 + lane;
+                fetched = m < a.width ? __ldg(a.table + slot_row * a.table_stride + m) : -1;
+            }
+            uint64_t mask = tile_mask(a, t, tile);
+            const int used = (t.len + page - 1) >> a.page_log;  // entries behind the sequence's end are not read
+            const uint64_t page_bits = page < 64 ? (1ull << page) - 1 : ~0ull;
+            int id[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                id[i] = -1;
+                if (i < boxes) {
+                    id[i] = __shfl_sync(0xffffffffu, fetched, m0 - fetched0 + i);
+                    if (m0 + i >= used || id[i] < 0 || id[i] >= a.pages) {
+                        id[i] = -1;
+                        mask &= ~(page_bits << (i * page & 63));
+                    }
+                }
+            }
+            const int st = g & 1;
+            if (!(ok = mbar_wait_warp(kfree(st), ((g >> 1) & 1) ^ 1u, abort_flag, 82))) break;
+            const int qb = q_bufs == 2 ? (seg & 1) : 0;
+            if (first && !(ok = mbar_wait_warp(qfree(qb), ((q_bufs == 2 ? seg >> 1 : seg) & 1) ^ 1u, abort_flag, 83))) break;
+            if (elect_one()) {
+                if (first) {
+                    const uint32_t dst = base + kPQOff + qb * (16 * kPQRow);
+                    mbar_arrive_expect_tx(qfull(qb), G * kPQRow);
+                    tma_load_4d(dst, &tm_qa, 0, hg * G, 0, b, qfull(qb));
+                    tma_load_3d(dst + G * 1024, &tm_qp, 0, hg * G, b, qfull(qb));
+                }
+                info_s[st].mask = mask;
+                info_s[st].row = b;
+                info_s[st].flags = (first ? 1 : 0) | (last ? 2 : 0) | (j == 0 ? 4 : 0) | (j == t.n - 1 ? 8 : 0);
+                mbar_arrive_expect_tx(kfull(st), kPTileBytes);
+                const uint32_t dst = base + kPKOff + st * kPTileBytes;
+                const int row0 = (tile * kPTile) & (page - 1);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    if (i >= boxes) break;
+                    tma_load_5d(dst + i * page * 1024, &tm_kv, 0, 0, 0, row0 >> 3, id[i], kfull(st));
+                    tma_load_3d(dst + kPLatBytes + i * page * 128, &tm_pe, 0, row0, id[i], kfull(st));
+                }
+            }
+            __syncwarp();
+            if (last) ++seg;
+            if (++j == t.n) {
+                ++b;
+                j = 0;
+            }
+        }
+    } else if (warp >= 4) {
+        const int quad = warp & 3;
+        const uint32_t lane_base = static_cast<uint32_t>(quad * 32) << 16;
+        const float ninf = __int_as_float(0xff800000);
+        float* alpha_s = reinterpret_cast<float*>(base_ptr + kPAlphaOff);
+        volatile int* grow_s = reinterpret_cast<volatile int*>(alpha_s + 64);
+        float* l_s = reinterpret_cast<float*>(base_ptr + kPMlOff);
+        const int head = hg * G + lane;
+        const bool live = lane < G && head < a.heads;
+        // rows without a visible tile are nobody's: zeros, shared out over the CTAs
+        if (hg == 0)
+            for (int b = range; b < a.batch; b += a.n_ranges)
+                if (row_tiles(a, b).n == 0)
+                    for (int c = threadIdx.x - 128; c < a.heads * 64; c += 128)
+                        reinterpret_cast<uint4*>(a.out + static_cast<int64_t>(b) * a.heads * 512)[c] = make_uint4(0u, 0u, 0u, 0u);
+        float m_ref = ninf, l = 0.f;
+        int flags4 = 0;
+        bool ok = true;
+        for (int g = 0; g < n_tiles; ++g) {
+            const int st = g & 1;
+            if (!(ok = mbar_wait_warp(kfull(st), (g >> 1) & 1, abort_flag, 84))) break;
+            const uint64_t mask = info_s[st].mask;
+            const int flags = info_s[st].flags, b = info_s[st].row;
+            const bool first = flags & 1, last = flags & 2;
+            flags4 = (first ? 0 : flags4) | (flags & 12);
+            if (!(ok = mbar_wait_warp(sfull(st), (g >> 1) & 1, abort_flag, 85))) break;
+            tc_fence_after();
+            uint32_t pk[32];
+            if (quad == 0) {
+                if (first) {
+                    m_ref = ninf;
+                    l = 0.f;
+                }
+                uint32_t r0[32], r1[32];
+                const uint32_t ts = tmem_base + kPTmemS + static_cast<uint32_t>(st) * kPTile;
+                tmem_ld_32x32(ts, r0);
+                tmem_ld_32x32(ts + 32, r1);
+                tmem_ld_wait(r0);
+                tmem_ld_wait(r1);
+                const uint64_t seen = live ? mask : 0ull;
+#pragma unroll
+                for (int i = 0; i < 32; ++i) {
+                    r0[i] = __float_as_uint(__uint_as_float(r0[i]) * a.scale_log2);
+                    r1[i] = __float_as_uint(__uint_as_float(r1[i]) * a.scale_log2);
+                }
+                if (seen != ~0ull) {
+                    const uint32_t lo = static_cast<uint32_t>(seen), hi = static_cast<uint32_t>(seen >> 32);
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) {
+                        if (!(lo >> i & 1)) r0[i] = 0xff800000u;
+                        if (!(hi >> i & 1)) r1[i] = 0xff800000u;
+                    }
+                }
+                float mx[4] = {ninf, ninf, ninf, ninf};
+#pragma unroll
+                for (int i = 0; i < 32; ++i) {
+                    mx[i & 1] = fmaxf(mx[i & 1], __uint_as_float(r0[i]));
+                    mx[2 + (i & 1)] = fmaxf(mx[2 + (i & 1)], __uint_as_float(r1[i]));
+                }
+                const float mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+                const bool grow = mt > m_ref + 8.f;          // false while mt is -inf
+                const float m_new = grow ? mt : m_ref;
+                const float alpha = grow ? exp2_fast(m_ref - m_new) : 1.f;
+                const float m_use = m_new == ninf ? 0.f : m_new;
+                float sum[2] = {0.f, 0.f};
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const float p0 = exp2_fast(__uint_as_float(r0[2 * i]) - m_use), p1 = exp2_fast(__uint_as_float(r0[2 * i + 1]) - m_use);
+                    const float p2 = exp2_fast(__uint_as_float(r1[2 * i]) - m_use), p3 = exp2_fast(__uint_as_float(r1[2 * i + 1]) - m_use);
+                    sum[0] += p0 + p1;
+                    sum[1] += p2 + p3;
+                    pk[i] = pack_bf16x2(p0, p1);
+                    pk[16 + i] = pack_bf16x2(p2, p3);
+                }
+                l = l * alpha + (sum[0] + sum[1]);
+                m_ref = m_new;
+                alpha_s[st * 32 + lane] = alpha;
+                const bool any = __any_sync(0xffffffffu, grow);
+                if (lane == 0) grow_s[st] = any ? 1 : 0;
+                if (last) l_s[st * 32 + lane] = l;
+                __syncwarp();
+                if (lane == 0) mbar_arrive(afull(st));
+            } else if (mask != ~0ull) {
+                // rows of the steps that are multiplied, but not visible
+                uint64_t z = 0;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const uint64_t step = 0xffffull << (16 * k);
+                    if (mask & step) z |= step & ~mask;
+                }
+                uint8_t* kt = base_ptr + kPKOff + st * kPTileBytes;
+                const int t = threadIdx.x - 160;                 // 96 threads, 64 pieces of a row
+                while (z) {
+                    const int r = __ffsll(static_cast<long long>(z)) - 1;
+                    z &= z - 1;
+                    if (t < 64)
+                        *reinterpret_cast<uint4*>(kt + (r >> 3) * 8192 + (t >> 3) * 1024 + (r & 7) * 128 + (t & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
+                }
+                fence_proxy_async();
+            }
+            if (!(ok = mbar_wait_warp(afull(st), (g >> 1) & 1, abort_flag, 86))) break;
+            // read before this warp's arrival on pfull, behind which the slot may be written again
+            const float den = last ? l_s[st * 32 + lane] : 0.f;
+            if (g > 0) {
+                // P V of the tile before has retired: P may be overwritten, O is at rest
+                if (!(ok = mbar_wait_warp(pfree, (g - 1) & 1, abort_flag, 87))) break;
+                tc_fence_after();
+                if (!first && grow_s[st]) {
+                    const float al = alpha_s[st * 32 + lane];
+#pragma unroll 1
+                    for (int c = 0; c < 4; ++c) {
+                        uint32_t o[32];
+                        tmem_ld_32x32(tmem_base + lane_base + c * 32, o);
+                        tmem_ld_wait(o);
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * al);
+                        tmem_st_32x32(tmem_base + lane_base + c * 32, o);
+                    }
+                    tmem_st_wait();
+                }
+            }
+            if (quad == 0) {
+                // P row: 64 bf16 = 8 pieces of 16 bytes in a 128-byte swizzled row
+                uint8_t* prow = base_ptr + kPPOff + (96 + lane) * 128;
+#pragma unroll
+                for (int c = 0; c < 8; ++c)
+                    *reinterpret_cast<uint4*>(prow + ((c ^ (lane & 7)) << 4)) =
+                        make_uint4(pk[4 * c], pk[4 * c + 1], pk[4 * c + 2], pk[4 * c + 3]);
+                fence_proxy_async();
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(pfull);
+            if (last) {
+                if (!(ok = mbar_wait_warp(pfree, g & 1, abort_flag, 88))) break;
+                tc_fence_after();
+                const int part = part_slot(flags4, range);
+                if (part < 0) {
+                    // the row's only part: a row of no weight at all (every page out of the pool, every score
+                    // -infinity) is zero
+                    const float inv = 1.f / den;
+                    __nv_bfloat16* orow = a.out + (static_cast<int64_t>(b) * a.heads + head) * 512 + quad * 128;
+#pragma unroll 1
+                    for (int c = 0; c < 4; ++c) {
+                        uint32_t o[32];
+                        tmem_ld_32x32(tmem_base + lane_base + c * 32, o);
+                        tmem_ld_wait(o);
+                        if (live) {
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                uint32_t w[4];
+#pragma unroll
+                                for (int k = 0; k < 4; ++k)
+                                    w[k] = den == 0.f ? 0u
+                                                      : pack_bf16x2(__uint_as_float(o[8 * i + 2 * k]) * inv,
+                                                                    __uint_as_float(o[8 * i + 2 * k + 1]) * inv);
+                                *reinterpret_cast<uint4*>(orow + c * 32 + 8 * i) = make_uint4(w[0], w[1], w[2], w[3]);
+                            }
+                        }
+                    }
+                } else {
+                    const int64_t prt = static_cast<int64_t>(part) * a.heads + head;
+                    float* po = a.part_o + prt * 512 + quad * 128;
+#pragma unroll 1
+                    for (int c = 0; c < 4; ++c) {
+                        uint32_t o[32];
+                        tmem_ld_32x32(tmem_base + lane_base + c * 32, o);
+                        tmem_ld_wait(o);
+                        if (live) {
+#pragma unroll
+                            for (int i = 0; i < 32; i += 4)
+                                *reinterpret_cast<uint4*>(po + c * 32 + i) =
+                                    den == 0.f ? make_uint4(0u, 0u, 0u, 0u) : make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+                        }
+                    }
+                    if (live && quad == 0) *reinterpret_cast<float2*>(a.part_ml + prt * 2) = make_float2(m_ref, l);
+                }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(ofree);
+            }
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 0) {
+        tc_fence_after();
+        tmem_dealloc(tmem_base, 256);
+    }
+}
+
+// Joins the parts of every row that crosses ranges: blockIdx.y + 1 is a range whose first tile lies inside a
+// row, and the block does the row if that is the row's first crossing. out = sum_s o_s 2^(m_s - M) / sum_s l_s
+// 2^(m_s - M), the parts in the order of their positions. Four threads share a group of four dims and take
+// every fourth part; their sums are added in order, so the result does not depend on timing.
+constexpr int kJoinThreads = 512;
+constexpr int kJoinMaxParts = 160;
+__global__ void __launch_bounds__(kJoinThreads) mla_paged_join_kernel(const PagedArgs a) {
+    const int r = blockIdx.y + 1, head = blockIdx.x;
+    const int4 rg = a.ranges[r];
+    if (rg.x < 0 || rg.y == 0) return;
+    const int per = rg.w, t0 = r * per - rg.y, r0 = t0 / per;
+    if (r0 != r - 1) return;
+    const int r1 = (t0 + rg.z - 1) / per, parts = r1 - r0 + 1;
+    __shared__ float w_s[kJoinMaxParts], red[kJoinThreads / 32][2];
+    __shared__ float4 acc_s[3][128];
+    const float ninf = __int_as_float(0xff800000);
+    auto row_of = [&](int s) { return (static_cast<int64_t>(s == 0 ? 2 * r0 + 1 : 2 * (r0 + s)) * a.heads + head); };
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    float ms = ninf, ls = 0.f;
+    if (tid < parts) {
+        const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + row_of(tid) * 2);
+        ms = ml.x;
+        ls = ml.y;
+    }
+    float m = warp_max(ms);
+    if (lane == 0) red[warp][0] = m;
+    __syncthreads();
+    m = red[0][0];
+#pragma unroll
+    for (int w = 1; w < kJoinMaxParts / 32; ++w) m = fmaxf(m, red[w][0]);
+    const float weight = ms == ninf ? (ls != 0.f ? ls : 0.f) : exp2f(ms - m);
+    if (tid < parts) w_s[tid] = weight;
+    const float d = warp_sum(tid < parts ? ls * weight : 0.f);
+    if (lane == 0) red[warp][1] = d;
+    __syncthreads();
+    float den = 0.f;
+#pragma unroll
+    for (int w = 0; w < kJoinMaxParts / 32; ++w) den += red[w][1];
+    const int q = tid >> 7, c = tid & 127;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int s0 = q; s0 < parts; s0 += 16) {
+        float4 o[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            o[i] = __ldg(reinterpret_cast<const float4*>(a.part_o + row_of(min(s0 + 4 * i, parts - 1)) * 512) + c);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int s = s0 + 4 * i;
+            if (s < parts) {
+                const float w = w_s[s];
+                acc.x += o[i].x * w; acc.y += o[i].y * w; acc.z += o[i].z * w; acc.w += o[i].w * w;
+            }
+        }
+    }
+    if (q > 0) acc_s[q - 1][c] = acc;
+    __syncthreads();
+    if (q == 0) {
+#pragma unroll
+        for (int i = 0; i < 3; ++i) {
+            const float4 o = acc_s[i][c];
+            acc.x += o.x; acc.y += o.y; acc.z += o.z; acc.w += o.w;
+        }
+        const float inv = 1.f / den;
+        uint2 v = make_uint2(pack_bf16x2(acc.x * inv, acc.y * inv), pack_bf16x2(acc.z * inv, acc.w * inv));
+        if (den == 0.f) v = make_uint2(0u, 0u);
+        *reinterpret_cast<uint2*>(a.out + (static_cast<int64_t>(rg.x) * a.heads + head) * 512 + c * 4) = v;
+    }
+}
+
+int sm_count();                                      // rt_gemm.cu
+int make_tmap_bf16(CUtensorMap* map, const void* ptr, int rank, const uint64_t* dims, const uint64_t* strides,
+                   const uint32_t* box);
+
+int paged_attn_error_take() {
+    int v = 0;
+    if (cudaMemcpyFromSymbol(&v, g_tc_error, sizeof(int)) != cudaSuccess) {
+        cudaGetLastError();
+        return -1;
+    }
+    if (v != 0) {
+        const int zero = 0;
+        cudaMemcpyToSymbol(g_tc_error, &zero, sizeof(int));
+    }
+    return v;
+}
+
+// Heads of a CTA, and the ranges that the tiles are cut into.
+static int paged_group(int64_t heads) {
+    return static_cast<int>(heads >= kPMaxG ? kPMaxG : (heads + 7) / 8 * 8);
+}
+static int paged_ranges(int64_t heads) {
+    const int64_t groups = (heads + paged_group(heads) - 1) / paged_group(heads);
+    const int64_t sms = sm_count();
+    int64_t r = sms / groups;
+    if (r < 1) r = 1;
+    return static_cast<int>(r < kJoinMaxParts ? r : kJoinMaxParts);
+}
+
+}  // namespace tc
+}  // namespace rt
+
+using namespace rt;
+
+extern "C" int64_t rt_mla_paged_decode_workspace_bytes(int64_t heads) {
+    if (heads < 1) return 0;
+    const int64_t r = tc::paged_ranges(heads);
+    return r * 16 + 2 * r * heads * (2 + 512) * 4;
+}
+
+extern "C" int rt_mla_paged_decode(const void* q_abs, const void* q_pe, const void* kv, const void* pe,
+                                   const int32_t* table, const int32_t* lens, const int32_t* seqs, void* out,
+                                   void* workspace, int64_t batch, int64_t heads, int64_t slots, int64_t width,
+                                   int64_t pages, int64_t page_size, int64_t qa_batch_stride, int64_t qa_head_stride,
+                                   int64_t qp_batch_stride, int64_t qp_head_stride, int64_t kv_page_stride,
+                                   int64_t kv_row_stride, int64_t pe_page_stride, int64_t pe_row_stride,
+                                   int64_t table_stride, int64_t window, int64_t sinks, float softmax_scale, void* stream) {
+    RT_REQUIRE(batch >= 0 && heads > 0 && slots >= 0 && width >= 0 && pages >= 0, RT_ERR_BAD_ARG, "rt_mla_paged_decode: bad shape");
+    if (batch == 0) return RT_OK;
+    RT_REQUIRE(page_size >= 16 && page_size <= (1 << 20) && (page_size & (page_size - 1)) == 0, RT_ERR_UNSUPPORTED,
+               "rt_mla_paged_decode: page_size must be a power of two, 16 or more");
+    RT_REQUIRE(q_abs && q_pe && kv && pe && out && workspace && (table || slots * width == 0) && (lens || slots == 0),
+               RT_ERR_BAD_ARG, "rt_mla_paged_decode: null pointer");
+    RT_REQUIRE(aligned16(q_abs) && aligned16(q_pe) && aligned16(kv) && aligned16(pe) && aligned16(out) && aligned16(workspace),
+               RT_ERR_BAD_ARG, "rt_mla_paged_decode: pointers must be 16-byte aligned");
+    const int64_t strides[] = {qa_batch_stride, qa_head_stride, qp_batch_stride, qp_head_stride, kv_page_stride,
+                               kv_row_stride, pe_page_stride, pe_row_stride};
+    for (int64_t s : strides)
+        RT_REQUIRE(s >= 0 && s % 8 == 0 && s < (1ll << 38), RT_ERR_BAD_ARG,
+                   "rt_mla_paged_decode: strides must be non-negative multiples of 8 elements");
+    RT_REQUIRE(window >= 0 && sinks >= 0, RT_ERR_BAD_ARG, "rt_mla_paged_decode: window and sinks must not be negative");
+    RT_REQUIRE(pages > 0, RT_ERR_BAD_ARG, "rt_mla_paged_decode: the pool has no page");
+    const int64_t tiles = (width * page_size + tc::kPTile - 1) / tc::kPTile;
+    RT_REQUIRE(batch <= tc::kPMaxBatch && heads <= 1024 && pages < (1ll << 31) && slots < (1ll << 31) &&
+                   width * page_size < (1ll << 31) - 64 && batch * tiles < (1ll << 31) - 65536,
+               RT_ERR_UNSUPPORTED, "rt_mla_paged_decode: dimension too large");
+    tc::PagedArgs a;
+    a.table = table; a.lens = lens; a.seqs = seqs;
+    a.out = static_cast<__nv_bfloat16*>(out);
+    a.table_stride = table_stride;
+    a.batch = static_cast<int>(batch); a.heads = static_cast<int>(heads); a.slots = static_cast<int>(slots);
+    a.width = static_cast<int>(width); a.pages = static_cast<int>(pages);
+    a.page_log = 0;
+    while ((1ll << a.page_log) < page_size) ++a.page_log;
+    const int64_t longest = width * page_size;
+    a.window = static_cast<int>(window > longest ? 0 : window);
+    a.sinks = static_cast<int>(sinks > longest ? longest : sinks);
+    a.scale_log2 = softmax_scale * 1.4426950408889634f;
+    a.group = tc::paged_group(heads);
+    a.n_ranges = tc::paged_ranges(heads);
+    a.ranges = static_cast<int4*>(workspace);
+    a.part_ml = reinterpret_cast<float*>(a.ranges + a.n_ranges);
+    a.part_o = a.part_ml + 2ll * a.n_ranges * heads * 2;
+
+    // one row of dims as eight blocks of 64: {dims, heads, blocks, rows} and {dims, 8 rows, blocks, groups of
+    // rows, pages}
+    CUtensorMap tm_qa, tm_qp, tm_kv, tm_pe;
+    const uint32_t box_rows = static_cast<uint32_t>(page_size < tc::kPTile ? page_size : tc::kPTile);
+    const int64_t u = 2;
+    {
+        const uint64_t dims[] = {64, static_cast<uint64_t>(heads), 8, static_cast<uint64_t>(batch)};
+        const uint64_t st[] = {static_cast<uint64_t>(u * qa_head_stride), 128, static_cast<uint64_t>(u * qa_batch_stride)};
+        const uint32_t box[] = {64, static_cast<uint32_t>(a.group), 8, 1};
+        if (int rc = tc::make_tmap_bf16(&tm_qa, q_abs, 4, dims, st, box)) return rc;
+    }
+    {
+        const uint64_t dims[] = {64, static_cast<uint64_t>(heads), static_cast<uint64_t>(batch)};
+        const uint64_t st[] = {static_cast<uint64_t>(u * qp_head_stride), static_cast<uint64_t>(u * qp_batch_stride)};
+        const uint32_t box[] = {64, static_cast<uint32_t>(a.group), 1};
+        if (int rc = tc::make_tmap_bf16(&tm_qp, q_pe, 3, dims, st, box)) return rc;
+    }
+    {
+        const uint64_t dims[] = {64, 8, 8, static_cast<uint64_t>(page_size / 8), static_cast<uint64_t>(pages)};
+        const uint64_t st[] = {static_cast<uint64_t>(u * kv_row_stride), 128, static_cast<uint64_t>(8 * u * kv_row_stride), static_cast<uint64_t>(u * kv_page_stride)};
+        const uint32_t box[] = {64, 8, 8, box_rows / 8, 1};
+        if (int rc = tc::make_tmap_bf16(&tm_kv, kv, 5, dims, st, box)) return rc;
+    }
+    {
+        const uint64_t dims[] = {64, static_cast<uint64_t>(page_size), static_cast<uint64_t>(pages)};
+        const uint64_t st[] = {static_cast<uint64_t>(u * pe_row_stride), static_cast<uint64_t>(u * pe_page_stride)};
+        const uint32_t box[] = {64, box_rows, 1};
+        if (int rc = tc::make_tmap_bf16(&tm_pe, pe, 3, dims, st, box)) return rc;
+    }
+    if (int rc = ensure_dynamic_smem(reinterpret_cast<const void*>(&tc::mla_paged_kernel),
+                                     static_cast<int>(tc::kPSmemBytes), "rt_mla_paged_decode"))
+        return rc;
+    const int groups = (a.heads + a.group - 1) / a.group;
+    cudaStream_t s = as_stream(stream);
+    tc::mla_paged_kernel<<<static_cast<unsigned>(a.n_ranges * groups), tc::kPThreads, tc::kPSmemBytes, s>>>(
+        tm_qa, tm_qp, tm_kv, tm_pe, a);
+    count_launch();
+    if (int rc = check_launch("mla_paged_kernel")) return rc;
+    if (a.n_ranges == 1) return RT_OK;
+    dim3 grid(static_cast<unsigned>(heads), static_cast<unsigned>(a.n_ranges - 1));
+    tc::mla_paged_join_kernel<<<grid, tc::kJoinThreads, 0, s>>>(a);
+    count_launch();
+    return check_launch("mla_paged_join_kernel");
+}

@@ -29,7 +29,7 @@ using OptTensor = std::optional<Tensor>;
     X(rt_index_topk) X(rt_mla_sparse_decode_splits) X(rt_mla_sparse_decode)                       \
     X(rt_page_extend_workspace_ints) X(rt_page_extend) X(rt_page_write) X(rt_page_free)           \
     X(rt_page_fork_workspace_ints) X(rt_page_fork) X(rt_page_compact_workspace_ints)              \
-    X(rt_page_compact) X(rt_page_copy)
+    X(rt_page_compact) X(rt_page_copy) X(rt_mla_paged_decode_workspace_bytes) X(rt_mla_paged_decode)
 
 #define RT_POINTER(name) decltype(&::name) p_##name = nullptr;
 RT_TABLE(RT_POINTER)
@@ -1019,6 +1019,53 @@ void page_copy(const std::vector<Tensor>& buffers, const Tensor& src, const Tens
           "rt_page_copy");
 }
 
+Tensor mla_paged_decode(const Tensor& q_abs_in, const Tensor& q_pe_in, const Tensor& kv, const Tensor& pe,
+                        const Tensor& table, const Tensor& lens, double softmax_scale, const OptTensor& seqs,
+                        std::optional<int64_t> window, int64_t sinks) {
+    const std::string who = "mla_paged_decode";
+    require_cuda({&q_abs_in});
+    require_ints(who, "block_table", table, q_abs_in, 2);
+    require_ints(who, "seq_lens", lens, q_abs_in, 1);
+    if (seqs) require_ints(who, "seqs", *seqs, q_abs_in, 1);
+    for (const Tensor* t : {&q_abs_in, &q_pe_in, &kv, &pe})
+        if (t->scalar_type() != at::kBFloat16 || t->dim() != 3 || t->device() != q_abs_in.device())
+            fail(who + ": q_abs, q_pe, kv_pages and pe_pages must be bf16 with three dimensions on one device");
+    const int64_t batch = q_abs_in.size(0), heads = q_abs_in.size(1), pages = kv.size(0), page = kv.size(1);
+    if (q_abs_in.size(2) != 512 || !same_shape(q_pe_in, {batch, heads, 64}) || kv.size(2) != 512 ||
+        !same_shape(pe, {pages, page, 64}))
+        fail(who + ": shapes must be q_abs [B, H, 512], q_pe [B, H, 64], kv_pages [P, page, 512], pe_pages [P, page, 64]");
+    if (lens.numel() != table.size(0)) fail(who + ": seq_lens must have one entry for each row of block_table");
+    if (table.size(0) > 1 && table.stride(0) < 0) fail(who + ": block_table strides must not be negative");
+    if (seqs ? seqs->numel() != batch : table.size(0) < batch)
+        fail(who + ": without seqs block_table must have a row for each query, with it seqs an entry");
+    if (window && *window < 1) fail(who + ": window must be positive");
+    if (sinks < 0 || (sinks > 0 && !window)) fail(who + ": sinks go with a window and must not be negative");
+    for (const Tensor* t : {&kv, &pe})
+        if (t->stride(2) != 1 || (pages > 1 && (t->stride(0) % 8 != 0 || t->stride(0) < 0)) || t->stride(1) % 8 != 0 ||
+            t->stride(1) < 0 || !aligned16(*t))
+            fail(who + ": kv_pages and pe_pages must have contiguous, 16-byte aligned rows");
+    const c10::cuda::CUDAGuard guard(q_abs_in.device());
+    // queries are a few rows: what the kernel cannot take as it lies is copied
+    auto rows = [](const Tensor& t) {
+        const bool fits = t.stride(2) == 1 && t.stride(0) % 8 == 0 && t.stride(1) % 8 == 0 && t.stride(0) > 0 &&
+                          t.stride(1) > 0 && aligned16(t);
+        return fits ? t : t.clone(at::MemoryFormat::Contiguous);
+    };
+    const Tensor q_abs = rows(q_abs_in), q_pe = rows(q_pe_in);
+    Tensor out = empty({batch, heads, 512}, at::kBFloat16, q_abs);
+    if (out.numel() == 0) return out;
+    Tensor work = empty({p_rt_mla_paged_decode_workspace_bytes(heads)}, at::kByte, q_abs);
+    check(p_rt_mla_paged_decode(q_abs.data_ptr(), q_pe.data_ptr(), kv.data_ptr(), pe.data_ptr(), data<int32_t>(table),
+                                data<int32_t>(lens), data<int32_t>(seqs), out.data_ptr(), work.data_ptr(), batch, heads,
+                                table.size(0), table.size(1), pages, page, q_abs.stride(0), q_abs.stride(1),
+                                q_pe.stride(0), q_pe.stride(1), pages > 1 ? kv.stride(0) : page * kv.stride(1), kv.stride(1),
+                                pages > 1 ? pe.stride(0) : page * pe.stride(1), pe.stride(1),
+                                table.size(0) > 1 ? table.stride(0) : table.size(1), window.value_or(0), sinks,
+                                static_cast<float>(softmax_scale), stream()),
+          "rt_mla_paged_decode");
+    return out;
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_rt_torch, m) {
@@ -1059,6 +1106,7 @@ PYBIND11_MODULE(_rt_torch, m) {
     RT_DEF(fp8_index);
     RT_DEF(index_topk);
     RT_DEF(mla_sparse_decode);
+    RT_DEF(mla_paged_decode);
     RT_DEF(page_extend);
     RT_DEF(page_write);
     RT_DEF(page_append);

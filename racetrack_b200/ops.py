@@ -567,6 +567,21 @@ def page_copy(pages, src: torch.Tensor, dst: torch.Tensor) -> None:
     _native().page_copy(list(pages), src, dst)
 
 
+def mla_paged_decode(q_abs: torch.Tensor, q_pe: torch.Tensor, kv_pages: torch.Tensor, pe_pages: torch.Tensor,
+                     block_table: torch.Tensor, seq_lens: torch.Tensor, softmax_scale: float, *,
+                     seqs: Optional[torch.Tensor] = None, window: Optional[int] = None, sinks: int = 0) -> torch.Tensor:
+    """Attention of one new token a sequence over a paged latent cache (racetrack/models/deepseek.py:793-810
+    without the indexer's mask): q_abs bf16 [B, H, 512] (q_nope times the key half of wkv_b), q_pe bf16 [B, H,
+    64], kv_pages bf16 [P, page, 512], pe_pages bf16 [P, page, 64] -> bf16 [B, H, 512].
+
+    Row b attends to the seq_lens[s] positions of sequence s = seqs[b] (int32 [B]; default: b), its own among
+    them (append first), or with `window` to the last `window` of them and the first `sinks`. A row whose
+    sequence is out of range (padding: -1) or empty is zero. Lengths stay on the device, so one captured
+    graph serves a growing cache. page: a power of two, 16 or more."""
+    return _native().mla_paged_decode(q_abs, q_pe, kv_pages, pe_pages, block_table, seq_lens, softmax_scale, seqs,
+                                      window, sinks)
+
+
 def attention_prefill(q: torch.Tensor, k_nope: torch.Tensor, k_pe: Optional[torch.Tensor],
                       v: torch.Tensor, softmax_scale: Optional[float] = None, *,
                       quantized: bool = False, out: Optional[tuple] = None,
