@@ -797,6 +797,22 @@ int rt_attn_causal_prefill_share(const void* q, const void* k_nope, const void* 
                                  int64_t v_token_stride, int64_t v_head_stride, int64_t o_token_stride,
                                  int64_t o_head_stride, float softmax_scale, void* stream);
 
+/*
+ * rt_attn_causal_prefill_share under a sliding window with sinks: query i sees the keys j <= i with j > i -
+ * window or j < sinks, and only key tiles that hold such keys are loaded and multiplied. window >= tokens is
+ * the causal call. The key of a token that a query does not see weighs nothing, NaN included; an infinite or
+ * NaN value of such a token may reach it (0 * inf), as in a product with a masked softmax. There is one
+ * schedule, so the bits do not depend on layer_heads below the window.
+ */
+int rt_attn_window_prefill(const void* q, const void* k_nope, const void* k_pe, const void* v, void* out,
+                           void* out_codes, float* out_scales, int64_t tokens, int64_t heads,
+                           int64_t layer_heads, int64_t nope_dim, int64_t rope_dim, int64_t v_dim,
+                           int64_t q_token_stride, int64_t q_head_stride, int64_t kn_token_stride,
+                           int64_t kn_head_stride, int64_t kp_token_stride, int64_t kp_head_stride,
+                           int64_t v_token_stride, int64_t v_head_stride, int64_t o_token_stride,
+                           int64_t o_head_stride, int64_t window, int64_t sinks, float softmax_scale,
+                           void* stream);
+
 /* ------------------------------------------------------------------------ */
 /* Collective steps over NVLink peer memory (one process per GPU)              */
 /* ------------------------------------------------------------------------ */

@@ -544,6 +544,8 @@ struct PrefillArgs {
     // [tokens, heads * 128] and one fp32 scale per token and head (= per 128-wide group)
     uint8_t* out_codes;
     float* out_scales;
+    // the windowed kernel: query i sees keys j <= i with j > i - window or j < sinks
+    int window, sinks;
 };
 
 // Two fp32 -> two e4m3 (RNE, saturating), `lo` in the low byte.
@@ -624,6 +626,11 @@ __device__ __forceinline__ void softmax_chunk(const uint32_t (&r)[32], uint32_t 
     }
 }
 
+// kWindow: under a sliding window with sinks a block of 256 queries walks the key tiles that hold sinks and
+// then those from the first key its first query sees on; both query tiles walk the same list. A tile that
+// not every query of a query tile sees whole is masked by 64 bits a thread; a row may meet a tile that it
+// sees nothing of before its first key, so its maximum may still be -infinity.
+template <bool kWindow>
 __global__ void __launch_bounds__(kFThreads, 1) attn_prefill_kernel(
     const __grid_constant__ CUtensorMap tm_qn, const __grid_constant__ CUtensorMap tm_qp,
     const __grid_constant__ CUtensorMap tm_kn, const __grid_constant__ CUtensorMap tm_kp,
@@ -647,7 +654,12 @@ __global__ void __launch_bounds__(kFThreads, 1) attn_prefill_kernel(
     const int qb = static_cast<int>(gridDim.x) - 1 - static_cast<int>(blockIdx.x);   // heaviest first
     const int h = blockIdx.y;
     const int q0 = qb * 256;
-    const int n0 = q0 / 128 + 1;                        // key tiles of query tile 0 (the last one is diagonal)
+    // key tiles left out between those of the sinks and the window's first one
+    const int w0 = kWindow ? max(0, q0 - a.window + 1) / 128 : 0;
+    const int n_sink = kWindow ? min((a.sinks + 127) / 128, w0) : 0;
+    const int gap = w0 - n_sink;
+    auto key_tile = [&](int j) { return kWindow && j >= n_sink ? j + gap : j; };
+    const int n0 = q0 / 128 + 1 - gap;                  // key tiles of query tile 0 (the last one is diagonal)
     const bool has1 = q0 + 128 < a.tokens;
     const int n1 = has1 ? n0 + 1 : 0;
     const int n_max = has1 ? n1 : n0;
@@ -703,13 +715,13 @@ __global__ void __launch_bounds__(kFThreads, 1) attn_prefill_kernel(
                 if (!(ok = mbar_wait(k_empty(st), ((j >> 1) & 1) ^ 1u, abort_flag, 71))) return;
                 const uint32_t dst = base + kFKOff + st * 3 * kFChunk;
                 mbar_arrive_expect_tx(k_full(st), nk * kFChunk);
-                load(&tm_kn, a.one_op & 4, a.cn, dst, 128 * j, h, k_full(st));
-                if (a.cp) load(&tm_kp, a.one_op & 8, a.cp, dst + a.cn * kFChunk, 128 * j, pe_head, k_full(st));
+                load(&tm_kn, a.one_op & 4, a.cn, dst, 128 * key_tile(j), h, k_full(st));
+                if (a.cp) load(&tm_kp, a.one_op & 8, a.cp, dst + a.cn * kFChunk, 128 * key_tile(j), pe_head, k_full(st));
             };
             auto load_v = [&](int j) {
                 if (!(ok = mbar_wait(v_empty, (j & 1) ^ 1u, abort_flag, 72))) return;
                 mbar_arrive_expect_tx(v_full, a.cv * kFChunk);
-                load(&tm_v, a.one_op & 16, a.cv, base + kFVOff, 128 * j, h, v_full);
+                load(&tm_v, a.one_op & 16, a.cv, base + kFVOff, 128 * key_tile(j), h, v_full);
             };
             // in the order the buffers become free: K_0 V_0 K_1, then K_(j+2) V_(j+1)
             load_k(0);
@@ -825,7 +837,24 @@ __global__ void __launch_bounds__(kFThreads, 1) attn_prefill_kernel(
             tmem_ld_wait(r0);
             tmem_ld_wait(r1);
             if (threadIdx.x == 64) RT_FTRACE(7, j);
-            if (j == n_t - 1) {                               // diagonal tile: keys beyond the row's own are masked
+            if constexpr (kWindow) {
+                const int k0 = 128 * key_tile(j), r0_abs = q0 + 128 * t;
+                if (j == n_t - 1 || !(k0 > r0_abs + 127 - a.window || k0 + 127 < a.sinks)) {
+                    // bit c: this row sees key k0 + 64 hh + c
+                    const int i = r0_abs + row, first = k0 + 64 * hh;
+                    auto below = [&](int x) {                 // keys first .. x - 1
+                        const int n = x - first;
+                        return n <= 0 ? 0ull : n >= 64 ? ~0ull : (1ull << n) - 1;
+                    };
+                    const uint64_t seen = below(i + 1) & (~below(i + 1 - a.window) | below(a.sinks));
+                    const uint32_t lo = static_cast<uint32_t>(seen), hi = static_cast<uint32_t>(seen >> 32);
+#pragma unroll
+                    for (int c = 0; c < 32; ++c) {
+                        if (!(lo >> c & 1)) r0[c] = 0xff800000u;
+                        if (!(hi >> c & 1)) r1[c] = 0xff800000u;
+                    }
+                }
+            } else if (j == n_t - 1) {                        // diagonal tile: keys beyond the row's own are masked
                 const int c0 = 64 * hh;
 #pragma unroll
                 for (int i = 0; i < 32; ++i) {
@@ -863,8 +892,12 @@ __global__ void __launch_bounds__(kFThreads, 1) attn_prefill_kernel(
                 }
             }
             m_ref = m_new;
+            auto neg_max = [&](float m) {
+                if (kWindow && m == ninf) m = 0.f;            // nothing seen yet: every probability is 2^-inf
+                return pack_f32x2(-m, -m);
+            };
             // P = exp2(s * scale - m) as bf16 pairs into columns [32 hh, 32 hh + 32) of S_t
-            const uint64_t scale2 = pack_f32x2(a.scale_log2, a.scale_log2), neg_m2 = pack_f32x2(-m_new, -m_new);
+            const uint64_t scale2 = pack_f32x2(a.scale_log2, a.scale_log2), neg_m2 = neg_max(m_new);
             uint64_t sums[2] = {0u, 0u};
             uint32_t pk[16];
             softmax_chunk<RT_FA_POLY_EVERY>(r0, pk, scale2, neg_m2, sums);
@@ -1491,7 +1524,8 @@ static int attn_causal_prefill(const void* q, const void* k_nope, const void* k_
                                int64_t q_token_stride, int64_t q_head_stride, int64_t kn_token_stride,
                                int64_t kn_head_stride, int64_t kp_token_stride, int64_t kp_head_stride,
                                int64_t v_token_stride, int64_t v_head_stride, int64_t o_token_stride,
-                               int64_t o_head_stride, float softmax_scale, void* stream);
+                               int64_t o_head_stride, float softmax_scale, void* stream, int64_t window = 0,
+                               int64_t sinks = 0);
 
 extern "C" int rt_attn_causal_prefill(const void* q, const void* k_nope, const void* k_pe, const void* v,
                                       void* out, int64_t tokens, int64_t heads, int64_t nope_dim,
@@ -1544,6 +1578,29 @@ extern "C" int rt_attn_causal_prefill_share(const void* q, const void* k_nope, c
                                v_head_stride, o_token_stride, o_head_stride, softmax_scale, stream);
 }
 
+extern "C" int rt_attn_window_prefill(const void* q, const void* k_nope, const void* k_pe, const void* v, void* out,
+                                      void* out_codes, float* out_scales, int64_t tokens, int64_t heads,
+                                      int64_t layer_heads, int64_t nope_dim, int64_t rope_dim, int64_t v_dim,
+                                      int64_t q_token_stride, int64_t q_head_stride, int64_t kn_token_stride,
+                                      int64_t kn_head_stride, int64_t kp_token_stride, int64_t kp_head_stride,
+                                      int64_t v_token_stride, int64_t v_head_stride, int64_t o_token_stride,
+                                      int64_t o_head_stride, int64_t window, int64_t sinks, float softmax_scale,
+                                      void* stream) {
+    RT_REQUIRE(window > 0 && sinks >= 0, RT_ERR_BAD_ARG,
+               "rt_attn_window_prefill: window must be positive and sinks not negative");
+    RT_REQUIRE(layer_heads >= heads, RT_ERR_BAD_ARG, "rt_attn_window_prefill: layer_heads below heads");
+    if (out == nullptr) {
+        RT_REQUIRE(out_codes && out_scales, RT_ERR_BAD_ARG, "rt_attn_window_prefill: null pointer");
+        RT_REQUIRE(nope_dim == 128 && rope_dim == 64 && v_dim == 128, RT_ERR_UNSUPPORTED,
+                   "rt_attn_window_prefill: the FP8 epilogue exists for the 128 + 64 / 128 head shape");
+        RT_REQUIRE(aligned16(out_codes), RT_ERR_BAD_ARG, "rt_attn_window_prefill: codes must be 16-byte aligned");
+    }
+    return attn_causal_prefill(q, k_nope, k_pe, v, out, out ? nullptr : out_codes, out ? nullptr : out_scales, tokens,
+                               heads, layer_heads, nope_dim, rope_dim, v_dim, q_token_stride, q_head_stride,
+                               kn_token_stride, kn_head_stride, kp_token_stride, kp_head_stride, v_token_stride,
+                               v_head_stride, o_token_stride, o_head_stride, softmax_scale, stream, window, sinks);
+}
+
 // Whether CTA pairs take a prefill of the 128 + 64 / 128 head shape: where every pair has its SMs at once
 // (one B200, single CTA / pairs: 16 heads x 1024 tokens 26 / 20 us, 8 x 2048 42 / 27, 32 x 512 18 / 16),
 // and from 3072 tokens on while the longest CTA takes a good part of what an SM has to do in all, its n
@@ -1563,7 +1620,8 @@ static int attn_causal_prefill(const void* q, const void* k_nope, const void* k_
                                       int64_t kn_head_stride, int64_t kp_token_stride,
                                       int64_t kp_head_stride, int64_t v_token_stride,
                                       int64_t v_head_stride, int64_t o_token_stride,
-                                      int64_t o_head_stride, float softmax_scale, void* stream) {
+                                      int64_t o_head_stride, float softmax_scale, void* stream, int64_t window,
+                                      int64_t sinks) {
     RT_REQUIRE(tokens >= 0 && heads > 0, RT_ERR_BAD_ARG, "rt_attn_causal_prefill: bad shape");
     if (tokens == 0) return RT_OK;
     RT_REQUIRE(q && k_nope && v && (out || out_codes) && (k_pe || rope_dim == 0), RT_ERR_BAD_ARG,
@@ -1596,6 +1654,9 @@ static int attn_causal_prefill(const void* q, const void* k_nope, const void* k_
     a.scale_log2 = softmax_scale * 1.4426950408889634f;
     a.out_codes = static_cast<uint8_t*>(out_codes);
     a.out_scales = out_scales;
+    if (window >= tokens) window = 0;                  // every query sees all keys before it
+    a.window = static_cast<int>(window);
+    a.sinks = static_cast<int>(sinks < tokens ? sinks : tokens);
     CUtensorMap tm_qn, tm_qp, tm_kn, tm_kp, tm_v;
     bool one[5] = {false, false, false, false, false};
     const __nv_bfloat16* qb = static_cast<const __nv_bfloat16*>(q);
@@ -1619,6 +1680,16 @@ static int attn_causal_prefill(const void* q, const void* k_nope, const void* k_
     }
     a.one_op = (one[0] ? 1 : 0) | (one[1] ? 2 : 0) | (one[2] ? 4 : 0) | (one[3] ? 8 : 0) | (one[4] ? 16 : 0);
     const bool mla_shape = nope_dim == 128 && rope_dim == 64 && v_dim == 128;
+    if (window > 0) {
+        if (int rc = ensure_dynamic_smem(reinterpret_cast<const void*>(&tc::attn_prefill_kernel<true>),
+                                         static_cast<int>(tc::kFSmemBytes), "rt_attn_window_prefill"))
+            return rc;
+        dim3 wgrid(static_cast<unsigned>((tokens + 255) / 256), static_cast<unsigned>(heads));
+        tc::attn_prefill_kernel<true><<<wgrid, tc::kFThreads, tc::kFSmemBytes, as_stream(stream)>>>(
+            tm_qn, tm_qp, tm_kn, tm_kp, tm_v, a);
+        count_launch();
+        return check_launch("attn_prefill_kernel<window>");
+    }
     if (mla_shape && (tc::g_attn_schedule == 2 || (tc::g_attn_schedule == 0 && attn_pairs_pay(tokens, layer_heads)))) {
         // the MLA head shape on CTA pairs with key tiles of 256 keys: a CTA brings 128 keys of a
         // tile (the boxes above) and 64 of the value dims for all of its 256 keys
@@ -1635,11 +1706,11 @@ static int attn_causal_prefill(const void* q, const void* k_nope, const void* k_
         count_launch();
         return check_launch("attn_prefill_pair_kernel");
     }
-    if (int rc = ensure_dynamic_smem(reinterpret_cast<const void*>(&tc::attn_prefill_kernel),
+    if (int rc = ensure_dynamic_smem(reinterpret_cast<const void*>(&tc::attn_prefill_kernel<false>),
                                      static_cast<int>(tc::kFSmemBytes), "rt_attn_causal_prefill"))
         return rc;
     dim3 grid(static_cast<unsigned>((tokens + 255) / 256), static_cast<unsigned>(heads));
-    tc::attn_prefill_kernel<<<grid, tc::kFThreads, tc::kFSmemBytes, as_stream(stream)>>>(
+    tc::attn_prefill_kernel<false><<<grid, tc::kFThreads, tc::kFSmemBytes, as_stream(stream)>>>(
         tm_qn, tm_qp, tm_kn, tm_kp, tm_v, a);
     count_launch();
     return check_launch("attn_prefill_kernel");

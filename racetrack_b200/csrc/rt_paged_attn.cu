@@ -448,15 +448,14 @@ __global__ void __launch_bounds__(kPThreads, 1) mla_paged_kernel(const __grid_co
                         reinterpret_cast<uint4*>(a.out + static_cast<int64_t>(b) * a.heads * 512)[c] = make_uint4(0u, 0u, 0u, 0u);
         float m_ref = ninf, l = 0.f;
         int flags4 = 0;
-        bool ok = true;
         for (int g = 0; g < n_tiles; ++g) {
             const int st = g & 1;
-            if (!(ok = mbar_wait_warp(kfull(st), (g >> 1) & 1, abort_flag, 84))) break;
+            if (!mbar_wait_warp(kfull(st), (g >> 1) & 1, abort_flag, 84)) break;
             const uint64_t mask = info_s[st].mask;
             const int flags = info_s[st].flags, b = info_s[st].row;
             const bool first = flags & 1, last = flags & 2;
             flags4 = (first ? 0 : flags4) | (flags & 12);
-            if (!(ok = mbar_wait_warp(sfull(st), (g >> 1) & 1, abort_flag, 85))) break;
+            if (!mbar_wait_warp(sfull(st), (g >> 1) & 1, abort_flag, 85)) break;
             tc_fence_after();
             uint32_t pk[32];
             if (quad == 0) {
@@ -531,12 +530,12 @@ __global__ void __launch_bounds__(kPThreads, 1) mla_paged_kernel(const __grid_co
                 }
                 fence_proxy_async();
             }
-            if (!(ok = mbar_wait_warp(afull(st), (g >> 1) & 1, abort_flag, 86))) break;
+            if (!mbar_wait_warp(afull(st), (g >> 1) & 1, abort_flag, 86)) break;
             // read before this warp's arrival on pfull, behind which the slot may be written again
             const float den = last ? l_s[st * 32 + lane] : 0.f;
             if (g > 0) {
                 // P V of the tile before has retired: P may be overwritten, O is at rest
-                if (!(ok = mbar_wait_warp(pfree, (g - 1) & 1, abort_flag, 87))) break;
+                if (!mbar_wait_warp(pfree, (g - 1) & 1, abort_flag, 87)) break;
                 tc_fence_after();
                 if (!first && grow_s[st]) {
                     const float al = alpha_s[st * 32 + lane];
@@ -565,7 +564,7 @@ __global__ void __launch_bounds__(kPThreads, 1) mla_paged_kernel(const __grid_co
             __syncwarp();
             if (lane == 0) mbar_arrive(pfull);
             if (last) {
-                if (!(ok = mbar_wait_warp(pfree, g & 1, abort_flag, 88))) break;
+                if (!mbar_wait_warp(pfree, g & 1, abort_flag, 88)) break;
                 tc_fence_after();
                 const int part = part_slot(flags4, range);
                 if (part < 0) {

@@ -585,7 +585,7 @@ def mla_paged_decode(q_abs: torch.Tensor, q_pe: torch.Tensor, kv_pages: torch.Te
 def attention_prefill(q: torch.Tensor, k_nope: torch.Tensor, k_pe: Optional[torch.Tensor],
                       v: torch.Tensor, softmax_scale: Optional[float] = None, *,
                       quantized: bool = False, out: Optional[tuple] = None,
-                      layer_heads: Optional[int] = None):
+                      layer_heads: Optional[int] = None, window: Optional[int] = None, sinks: int = 0):
     """Causal attention over [tokens, heads, dim] tensors on the tensor cores
     (racetrack/runtime/torch_ops.py:97-110; the attention core of
     racetrack/realistic_bench.py:304-313): q bf16 [T, H, nope + rope]; the key of head h is
@@ -599,8 +599,22 @@ def attention_prefill(q: torch.Tensor, k_nope: torch.Tensor, k_pe: Optional[torc
     ``out`` = (codes, scales) to write into (contiguous, 1-byte codes).
 
     layer_heads: the heads of the whole layer where a rank holds a share of them (default: H). The schedule
-    is the one the whole layer would take, so the share has the bits a call with every head gives."""
+    is the one the whole layer would take, so the share has the bits a call with every head gives.
+
+    window: query i sees only the last `window` keys up to its own and the first `sinks` of all; key tiles
+    without such a key are neither loaded nor multiplied. A window of T or more is the causal call. Hidden
+    keys weigh nothing, NaN included; their values must be finite."""
     _require_cuda(q, k_nope, v)
+    if window is not None and int(window) < 1:
+        raise RuntimeError("attention_prefill: window must be positive")
+    if sinks < 0 or (sinks and window is None):
+        raise RuntimeError("attention_prefill: sinks go with a window and must not be negative")
+    if any(t is not None and t.device != q.device for t in (k_nope, k_pe, v)):
+        raise RuntimeError("attention_prefill: operands must be on one device")
+    if q.device.index != torch.cuda.current_device():
+        with torch.cuda.device(q.device):
+            return attention_prefill(q, k_nope, k_pe, v, softmax_scale, quantized=quantized, out=out,
+                                     layer_heads=layer_heads, window=window, sinks=sinks)
     tokens, heads, qk = q.shape
     nope = k_nope.shape[-1]
     rope = qk - nope
@@ -629,6 +643,10 @@ def attention_prefill(q: torch.Tensor, k_nope: torch.Tensor, k_pe: Optional[torc
     if softmax_scale is None:
         softmax_scale = qk ** -0.5
     lib = _lib.load()
+    if window is None:
+        attend, masked = lib.rt_attn_causal_prefill_share, ()
+    else:
+        attend, masked = lib.rt_attn_window_prefill, (min(int(window), max(tokens, 1)), min(int(sinks), tokens))
     if quantized:
         if out is not None:
             codes, scales = out
@@ -638,23 +656,24 @@ def attention_prefill(q: torch.Tensor, k_nope: torch.Tensor, k_pe: Optional[torc
                 raise RuntimeError("attention_prefill: out must be contiguous (1-byte codes [T, H*v], fp32 scales [T, H*v/128])")
         if (nope, rope, v_dim) != (128, 64, 128):
             # no fused epilogue for this head shape: the quantiser runs behind the attention kernel
-            return fused_act_quant(attention_prefill(q, k_nope, k_pe, v, softmax_scale, layer_heads=layer_heads)
+            return fused_act_quant(attention_prefill(q, k_nope, k_pe, v, softmax_scale, layer_heads=layer_heads,
+                                                     window=window, sinks=sinks)
                                    .view(tokens, heads * v_dim), out=out)
         if out is None:
             codes = torch.empty(tokens, heads * v_dim, dtype=torch.float8_e4m3fn, device=q.device)
             scales = torch.empty(tokens, heads, dtype=torch.float32, device=q.device)
-        _lib.check(lib.rt_attn_causal_prefill_share(
+        _lib.check(attend(
             q.data_ptr(), k_nope.data_ptr(), k_pe.data_ptr(), v.data_ptr(), None, codes.data_ptr(),
             scales.data_ptr(), tokens, heads, layer_heads or heads, nope, rope, v_dim, q.stride(0), q.stride(1),
             k_nope.stride(0), k_nope.stride(1), kp_ts, kp_hs, v.stride(0), v.stride(1), 8, 8,
-            float(softmax_scale), _stream()), "rt_attn_causal_prefill_fp8")
+            *masked, float(softmax_scale), _stream()), "rt_attn_causal_prefill_fp8")
         return codes, scales
     out = torch.empty(tokens, heads, v_dim, dtype=torch.bfloat16, device=q.device)
-    _lib.check(lib.rt_attn_causal_prefill_share(
+    _lib.check(attend(
         q.data_ptr(), k_nope.data_ptr(), k_pe.data_ptr() if rope else None, v.data_ptr(),
         out.data_ptr(), None, None, tokens, heads, layer_heads or heads, nope, rope, v_dim, q.stride(0), q.stride(1),
         k_nope.stride(0), k_nope.stride(1), kp_ts, kp_hs, v.stride(0), v.stride(1),
-        out.stride(0), out.stride(1), float(softmax_scale), _stream()), "rt_attn_causal_prefill")
+        out.stride(0), out.stride(1), *masked, float(softmax_scale), _stream()), "rt_attn_causal_prefill")
     return out
 
 
