@@ -37,7 +37,6 @@ struct PagedArgs {
     int page_log;                 // log2(page size)
     int window, sinks;            // window 0: none
     int n_ranges;
-    int group;                    // heads of a CTA
     float scale_log2;
 };
 
@@ -82,15 +81,14 @@ __device__ __forceinline__ uint64_t tile_mask(const PagedArgs& a, const RowTiles
     return m;
 }
 
-// The range of this CTA: its first row and tile, and how many tiles it walks. All threads (kPThreads) call
-// it; every thread sums the rows of one slice of the batch.
+// The range of this CTA: its first row and tile, and how many tiles it walks. All threads call it; every
+// thread sums the rows of one slice of the batch. `scratch`: THREADS / 32 + 3 ints of shared memory.
 struct RangeStart {
     int row, tile, count;
 };
 template <int THREADS>
-__device__ RangeStart find_range(const PagedArgs& a, int range) {
-    __shared__ int warp_sum[THREADS / 32];
-    __shared__ int found[3];
+__device__ RangeStart find_range(const PagedArgs& a, int range, volatile int* scratch) {
+    volatile int* found = scratch + THREADS / 32;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int per = (a.batch + THREADS - 1) / THREADS;
     const int b0 = min(static_cast<int>(threadIdx.x) * per, a.batch), b1 = min(b0 + per, a.batch);
@@ -102,7 +100,7 @@ __device__ RangeStart find_range(const PagedArgs& a, int range) {
         const int y = __shfl_up_sync(0xffffffffu, x, o);
         if (lane >= o) x += y;
     }
-    if (lane == 31) warp_sum[warp] = x;
+    if (lane == 31) scratch[warp] = x;
     if (threadIdx.x == 0) {
         found[0] = -1;
         found[1] = found[2] = 0;
@@ -111,8 +109,9 @@ __device__ RangeStart find_range(const PagedArgs& a, int range) {
     int before = x - mine, total = 0;
 #pragma unroll
     for (int w = 0; w < THREADS / 32; ++w) {
-        if (w < warp) before += warp_sum[w];
-        total += warp_sum[w];
+        const int v = scratch[w];
+        if (w < warp) before += v;
+        total += v;
     }
     const int per_range = (total + a.n_ranges - 1) / a.n_ranges;
     const int first = range * per_range;             // below 2^31: the host bounds batch * tiles
@@ -130,46 +129,49 @@ __device__ RangeStart find_range(const PagedArgs& a, int range) {
     __syncthreads();
     RangeStart r{found[0], found[1], 0};
     if (r.row >= 0) r.count = min(per_range, total - first);
-    if (threadIdx.x == 0) a.ranges[range] = make_int4(r.row, found[1], found[2], per_range);
+    if (threadIdx.x == 0) a.ranges[range] = make_int4(r.row, r.tile, found[2], per_range);
     return r;
 }
 
-// ---- one CTA, up to 32 heads --------------------------------------------------------------------
-// Work of a CTA: its range of tiles for one group of G <= 32 heads. Per tile of 64 positions:
+// ---- the kernel -------------------------------------------------------------------------------
+// Work of a CTA: its range of tiles for one group of G heads (16, 32 or 64; more heads are several groups,
+// whose CTAs run side by side and share the tiles in L2). Positions and dims are the rows of the products,
+// heads the columns: with few heads what the tensor core reads from shared memory is then little
+// more than the tile itself. (Heads as rows, padded to 128, took 2300 + 1400 cycles a tile for 16 heads:
+// 4 KB of mostly empty query rows for each instruction. This form takes about half.) Per tile of 64
+// positions:
 //   producer  one TMA box a page brings the latent rows as [8-row groups][8 blocks of 64 dims][8 rows][128
 //             B] (128-byte swizzle), one the rope keys: a page of any size lands in the same
 //             layout, of which both products read their operand (the group stride is a field of the
-//             descriptor), so the rows are staged once. Two tiles in flight (144 KB: what an SM's share
-//             of the memory rate needs, some 44 KB, three times over);
-//   S = Q K^T 36 tcgen05.mma (M = 128 rows of which G are heads, N = 64, K = 16), K-major operands;
-//   softmax   one thread a head: running maximum with a lazy rescale (only when it grows by more than
-//             2^8), P = 2^(s - m) as bf16 into shared memory. Sums, maxima and O stay fp32; P is rounded to
-//             bf16 because the tensor core multiplies it with bf16 rows (relative 2^-9 a
-//             probability, no more than the rows' own rounding);
-//   O += P V  the tile again as the MN-major operand. 512 dims would fill tensor memory as columns;
-//             they are folded into the lanes: P lies between zero rows, and the MMA whose A operand starts
-//             32 f rows before P puts dims [128 f, 128 f + 128) of head r into lane 32 f + r, all four in the
-//             same 128 columns. Only the 16-position steps that hold a visible position are multiplied.
-// Positions that are not visible weigh exactly nothing whatever their memory holds: their scores are never
-// looked at, and their rows are zeroed in shared memory between the two products (0 * NaN).
-// A page number outside the pool reads as zeros (the TMA unit's bounds) and its positions are not visible.
-constexpr int kPThreads = 256;                       // 0 MMA, 1 producer, 4-7 softmax / lanes
-constexpr int kPMaxG = 32;
+//             descriptor), so the rows are staged once. Two tiles in flight (144 KB);
+//   S = K Q^T 36 tcgen05.mma (M = 64 positions, N = G heads, K = 16 dims), both K-major;
+//   softmax   a thread holds one position's scores of 16 or 32 heads (an M = 64 product lies in lanes 0-15
+//             of each quarter of tensor memory). The maxima it works against change only when a score
+//             exceeds one by 2^8: all warps vote on that, and only then (and at a row's first tile)
+//             look for new maxima, across lanes and warps. P = 2^(s - m) goes as bf16 into shared memory,
+//             one 128-byte line of heads a position; a thread sums its own probabilities in fp32,
+//             and the sums meet at the row's end;
+//   O^T += V^T P^T  tcgen05.mma (M = 128 of the 512 dims, N = G, K = 16 positions): the tile again, as the
+//             MN-major operand, P MN-major too. Only steps that hold a visible position are multiplied.
+// O is 4 blocks of G columns in tensor memory, the two score buffers 2 G behind it. All sums, maxima and O
+// are fp32; P is rounded to bf16 because the tensor core multiplies it with bf16 rows (2^-8 of a
+// probability at most, no more than the rounding of the rows). Positions that are not visible weigh
+// exactly nothing whatever memory holds there: their scores are not looked at, their rows are zeroed in
+// shared memory between the two products (0 * NaN). A page number outside the pool reads as zeros (the
+// TMA unit's bounds) and its positions are not visible.
+constexpr int kPMaxG = 64;
 constexpr uint32_t kPQRow = 9 * 128;                 // bytes of a staged head
-constexpr uint32_t kPQOff = 0;                       // two of up to 16 heads or one of up to 32
-constexpr uint32_t kPKOff = kPMaxG * kPQRow;
-constexpr uint32_t kPPOff = kPKOff + 2 * kPTileBytes;        // 96 zero rows | P: 32 rows of 128 B | 96 zero rows
-constexpr uint32_t kPBarOff = kPPOff + 224 * 128;
-constexpr int kPBars = 15;      // qfull[2] qfree[2] kfull[2] kfree[2] sfull[2] afull[2] pfull pfree ofree
-constexpr uint32_t kPInfoOff = kPBarOff + kPBars * 8 + 24;   // (tensor memory slot, abort flag before it)
-constexpr uint32_t kPAlphaOff = kPInfoOff + 2 * 16;          // rescale factors [2][32], grow flags [2]
-constexpr uint32_t kPMlOff = kPAlphaOff + (2 * 32 + 2) * 4;  // denominators [2][32]
-constexpr uint32_t kPSmemBytes = kPMlOff + 2 * 32 * 4 + 1024;
-static_assert(kPKOff % 1024 == 0 && kPPOff % 1024 == 0 && kPInfoOff % 16 == 0, "alignment");
+constexpr uint32_t kPQBytes = kPMaxG * kPQRow;       // two sets of queries of up to 32 heads, or one of 64
+constexpr uint32_t kPKOff = kPQBytes;
+constexpr uint32_t kPPOff = kPKOff + 2 * kPTileBytes;        // P: [64 positions][64 heads] bf16
+constexpr uint32_t kPBarOff = kPPOff + kPTile * 128;
+constexpr int kPBars = 14;      // qfull[2] qfree[2] kfull[2] kfree[2] sfull[2] vote pfull pfree ofree
+constexpr uint32_t kPInfoOff = kPBarOff + kPBars * 8 + 16;   // (tensor memory slot, abort flag before it)
+constexpr uint32_t kPVoteOff = kPInfoOff + 2 * 16;           // [2][8] ints
+constexpr uint32_t kPMaxOff = kPVoteOff + 2 * 8 * 4;         // m [64], m or 0 [64], per quarter [4][64]
+constexpr uint32_t kPSmemBytes = kPMaxOff + 6 * 64 * 4 + 1024;
+static_assert(kPKOff % 1024 == 0 && kPPOff % 1024 == 0 && kPInfoOff % 16 == 0 && kPMaxOff % 16 == 0, "alignment");
 static_assert(kPSmemBytes <= 232448, "shared memory budget");
-constexpr uint32_t kPTmemS = 128;                    // O: columns [0, 128); S: two buffers of 64
-constexpr uint32_t kPSIdesc = (1u << 4) | (1u << 7) | (1u << 10) | ((kPTile >> 3) << 17) | (8u << 24);
-constexpr uint32_t kPOIdesc = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | (16u << 17) | (8u << 24);
 
 struct TileInfo {
     uint64_t mask;
@@ -205,17 +207,67 @@ __device__ __forceinline__ bool mbar_wait_warp(uint32_t bar, uint32_t parity, vo
     return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort, code));
 }
 
+// 16 or 32 consecutive columns of the warp's lanes, complete on return.
+__device__ __forceinline__ void tmem_ld_cols(uint32_t taddr, uint32_t (&r)[32]) {
+    tmem_ld_32x32(taddr, r);
+    tmem_ld_wait(r);
+}
+__device__ __forceinline__ void tmem_ld_cols(uint32_t taddr, uint32_t (&r)[16]) {
+    uint32_t lo[8], hi[8];
+    tmem_ld_32x8(taddr, lo);
+    tmem_ld_32x8(taddr + 8, hi);
+    tmem_ld_wait(lo);
+    tmem_ld_wait(hi);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        r[i] = lo[i];
+        r[8 + i] = hi[i];
+    }
+}
+__device__ __forceinline__ void tmem_st_cols(uint32_t taddr, const uint32_t (&r)[32]) { tmem_st_32x32(taddr, r); }
+__device__ __forceinline__ void tmem_st_cols(uint32_t taddr, const uint32_t (&r)[16]) { tmem_st_32x16(taddr, r); }
+
+// Combines 16 values over lanes 0-15 with 15 shuffles: lane i is left with value i of all of them.
+template <typename F>
+__device__ __forceinline__ float reduce16(float (&v)[16], F f) {
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) {
+        const bool up = lane & o;
+#pragma unroll
+        for (int i = 0; i < o; ++i) {
+            const float give = up ? v[i] : v[i + o], keep = up ? v[i + o] : v[i];
+            v[i] = f(keep, __shfl_xor_sync(0xffffffffu, give, o));
+        }
+    }
+    return v[0];
+}
+
 // Where the result of a row's tiles in a range goes: the row's own output if they are all of its tiles, else
 // the range's slot for a row that began in an earlier range (2 r) or ends in a later one (2 r + 1).
 __device__ __forceinline__ int part_slot(int flags, int range) {
     return (flags & 12) == 12 ? -1 : 2 * range + ((flags & 4) ? 1 : 0);
 }
 
-__global__ void __launch_bounds__(kPThreads, 1) mla_paged_kernel(const __grid_constant__ CUtensorMap tm_qa,
-                                                                 const __grid_constant__ CUtensorMap tm_qp,
-                                                                 const __grid_constant__ CUtensorMap tm_kv,
-                                                                 const __grid_constant__ CUtensorMap tm_pe,
-                                                                 const PagedArgs a) {
+// Softmax warps: one a quarter of tensor memory, two (each half of the heads) for 64 heads.
+template <int G>
+constexpr int kPHalves = G > 32 ? 2 : 1;
+template <int G>
+constexpr int kPThreads = 128 + 128 * kPHalves<G>;   // 0 MMA, 1 producer, 4.. softmax
+
+template <int G>
+__global__ void __launch_bounds__(kPThreads<G>, 1) mla_paged_kernel(const __grid_constant__ CUtensorMap tm_qa,
+                                                                    const __grid_constant__ CUtensorMap tm_qp,
+                                                                    const __grid_constant__ CUtensorMap tm_kv,
+                                                                    const __grid_constant__ CUtensorMap tm_pe,
+                                                                    const PagedArgs a) {
+    constexpr int kHalves = kPHalves<G>, kHT = G / kHalves, kWarps = 4 * kHalves;
+    constexpr int kQBufs = G > 32 ? 1 : 2;
+    constexpr uint32_t kTmemS = 4 * G, kTmemCols = G == 16 ? 128 : G == 32 ? 256 : 512;
+    // fp32 accumulate, bf16 x bf16; S: both K-major, M = 64; O: both MN-major, M = 128
+    constexpr uint32_t kSIdesc = (1u << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(G >> 3) << 17) | (4u << 24);
+    constexpr uint32_t kOIdesc = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 15) | (1u << 16) |
+                                 (static_cast<uint32_t>(G >> 3) << 17) | (8u << 24);
     extern __shared__ uint8_t smem_raw[];
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     uint8_t* base_ptr = smem_raw + (base - smem_u32(smem_raw));
@@ -225,18 +277,18 @@ __global__ void __launch_bounds__(kPThreads, 1) mla_paged_kernel(const __grid_co
     auto kfull = [&](int s) { return bars + 8u * (4 + s); };
     auto kfree = [&](int s) { return bars + 8u * (6 + s); };
     auto sfull = [&](int s) { return bars + 8u * (8 + s); };
-    auto afull = [&](int s) { return bars + 8u * (10 + s); };
-    const uint32_t pfull = bars + 8u * 12, pfree = bars + 8u * 13, ofree = bars + 8u * 14;
+    const uint32_t vote = bars + 8u * 10, pfull = bars + 8u * 11, pfree = bars + 8u * 12, ofree = bars + 8u * 13;
     const uint32_t slot = bars + 8u * kPBars;
     volatile uint32_t* slot_ptr = reinterpret_cast<volatile uint32_t*>(base_ptr + kPBarOff + 8 * kPBars);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(slot_ptr + 1);
     volatile TileInfo* info_s = reinterpret_cast<volatile TileInfo*>(base_ptr + kPInfoOff);
+    float* const m_s = reinterpret_cast<float*>(base_ptr + kPMaxOff);        // running maxima
+    float* const mu_s = m_s + 64;                                            // the same, 0 for -infinity
+    float* const w_s = mu_s + 64;                                            // [4][64]
 
     const int warp = uniform_warp_id(), lane = threadIdx.x & 31;
-    const int groups = (a.heads + a.group - 1) / a.group;
+    const int groups = (a.heads + G - 1) / G;
     const int hg = blockIdx.x % groups, range = blockIdx.x / groups;
-    const int G = a.group;                                     // multiple of 8
-    const int q_bufs = G <= 16 ? 2 : 1;
 
     if (threadIdx.x == 0) {
         *abort_flag = 0;
@@ -246,11 +298,11 @@ __global__ void __launch_bounds__(kPThreads, 1) mla_paged_kernel(const __grid_co
             mbar_init(kfull(s), 1);
             mbar_init(kfree(s), 1);
             mbar_init(sfull(s), 1);
-            mbar_init(afull(s), 1);
         }
-        mbar_init(pfull, 4);
+        mbar_init(vote, kWarps);
+        mbar_init(pfull, kWarps);
         mbar_init(pfree, 1);
-        mbar_init(ofree, 4);
+        mbar_init(ofree, kWarps);
         fence_mbar_init();
         tma_prefetch_desc(&tm_qa);
         tma_prefetch_desc(&tm_qp);
@@ -258,14 +310,10 @@ __global__ void __launch_bounds__(kPThreads, 1) mla_paged_kernel(const __grid_co
         tma_prefetch_desc(&tm_pe);
     }
     if (warp == 0) {
-        tmem_alloc(slot, 256);
+        tmem_alloc(slot, kTmemCols);
         tmem_relinquish();
     }
-    // zero rows around P (P's own rows are written before they are read)
-    for (int c = threadIdx.x; c < 224 * 8; c += kPThreads)
-        *reinterpret_cast<uint4*>(base_ptr + kPPOff + c * 16) = make_uint4(0u, 0u, 0u, 0u);
-    fence_proxy_async();
-    const RangeStart start = find_range<kPThreads>(a, range);
+    const RangeStart start = find_range<kPThreads<G>>(a, range, reinterpret_cast<volatile int*>(w_s));
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -286,20 +334,20 @@ __global__ void __launch_bounds__(kPThreads, 1) mla_paged_kernel(const __grid_co
                 bool progressed = false;
                 if (q < n_tiles && q - v < 2 && mbar_try_wait(kfull(q & 1), (q >> 1) & 1)) {
                     const int flags = info_s[q & 1].flags;
-                    const int qb = q_bufs == 2 ? (q_seg & 1) : 0;
-                    if (q_open || mbar_try_wait(qfull(qb), (q_bufs == 2 ? q_seg >> 1 : q_seg) & 1)) {
+                    const int qb = kQBufs == 2 ? (q_seg & 1) : 0;
+                    if (q_open || mbar_try_wait(qfull(qb), (kQBufs == 2 ? q_seg >> 1 : q_seg) & 1)) {
                         tc_fence_after();
                         const uint32_t kb = base + kPKOff + (q & 1) * kPTileBytes;
-                        const uint32_t qa = base + kPQOff + qb * (16 * kPQRow);
-                        const uint32_t d = tmem_base + kPTmemS + static_cast<uint32_t>(q & 1) * kPTile;
+                        const uint32_t qa = base + qb * (G * kPQRow);
+                        const uint32_t d = tmem_base + kTmemS + static_cast<uint32_t>(q & 1) * G;
 #pragma unroll
                         for (int c = 0; c < 9; ++c) {
-                            const uint64_t adesc = smem_desc_sw128(qa + c * G * 128);
-                            const uint64_t bdesc = c < 8 ? smem_desc_groups(kb + c * 1024, 16, 8192)
+                            const uint64_t adesc = c < 8 ? smem_desc_groups(kb + c * 1024, 16, 8192)
                                                          : smem_desc_sw128(kb + kPLatBytes);
+                            const uint64_t bdesc = smem_desc_sw128(qa + c * G * 128);
 #pragma unroll
                             for (int j = 0; j < 4; ++j)
-                                mma_f16(d, adesc + 2u * j, bdesc + 2u * j, kPSIdesc, (c | j) != 0 ? 1u : 0u);
+                                mma_f16(d, adesc + 2u * j, bdesc + 2u * j, kSIdesc, (c | j) != 0 ? 1u : 0u);
                         }
                         mma_commit(sfull(q & 1));
                         q_open = true;
@@ -322,13 +370,12 @@ __global__ void __launch_bounds__(kPThreads, 1) mla_paged_kernel(const __grid_co
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
                         if ((mask >> (16 * j) & 0xffffu) == 0) continue;
+                        const uint64_t bdesc = smem_desc_groups(base + kPPOff + j * 2048, 16, 1024);
 #pragma unroll
-                        for (int f = 0; f < 4; ++f) {
-                            const uint64_t adesc = smem_desc_sw128(base + kPPOff + (96 - 32 * f) * 128);
-                            const uint64_t bdesc = smem_desc_groups(kb + j * 16384 + f * 2048, 1024, 8192);
-                            mma_f16(tmem_base, adesc + 2u * j, bdesc, kPOIdesc, acc);
-                            acc = 1;
-                        }
+                        for (int f = 0; f < 4; ++f)
+                            mma_f16(tmem_base + f * G, smem_desc_groups(kb + j * 16384 + f * 2048, 1024, 8192), bdesc,
+                                    kOIdesc, acc);
+                        acc = 1;
                     }
                     mma_commit(kfree(v & 1));
                     mma_commit(pfree);
@@ -362,10 +409,9 @@ __global__ void __launch_bounds__(kPThreads, 1) mla_paged_kernel(const __grid_co
         int slot_row = -1;
         const int page = 1 << a.page_log;
         const int boxes = page < kPTile ? kPTile / page : 1;   // pages of a tile
-        bool ok = true;
         int32_t fetched = -1;                                   // lane: page number of entry fetched0 + lane
         int fetched0 = -1, fetched_row = -1;
-        for (int g = 0; ok && g < n_tiles; ++g) {
+        for (int g = 0; g < n_tiles; ++g) {
             if (row_at != b) {
                 t = row_tiles(a, b);
                 while (j >= t.n) {                              // rows without a tile
@@ -401,12 +447,12 @@ __global__ void __launch_bounds__(kPThreads, 1) mla_paged_kernel(const __grid_co
                 }
             }
             const int st = g & 1;
-            if (!(ok = mbar_wait_warp(kfree(st), ((g >> 1) & 1) ^ 1u, abort_flag, 82))) break;
-            const int qb = q_bufs == 2 ? (seg & 1) : 0;
-            if (first && !(ok = mbar_wait_warp(qfree(qb), ((q_bufs == 2 ? seg >> 1 : seg) & 1) ^ 1u, abort_flag, 83))) break;
+            if (!mbar_wait_warp(kfree(st), ((g >> 1) & 1) ^ 1u, abort_flag, 82)) break;
+            const int qb = kQBufs == 2 ? (seg & 1) : 0;
+            if (first && !mbar_wait_warp(qfree(qb), ((kQBufs == 2 ? seg >> 1 : seg) & 1) ^ 1u, abort_flag, 83)) break;
             if (elect_one()) {
                 if (first) {
-                    const uint32_t dst = base + kPQOff + qb * (16 * kPQRow);
+                    const uint32_t dst = base + qb * (G * kPQRow);
                     mbar_arrive_expect_tx(qfull(qb), G * kPQRow);
                     tma_load_4d(dst, &tm_qa, 0, hg * G, 0, b, qfull(qb));
                     tma_load_3d(dst + G * 1024, &tm_qp, 0, hg * G, b, qfull(qb));
@@ -432,22 +478,28 @@ __global__ void __launch_bounds__(kPThreads, 1) mla_paged_kernel(const __grid_co
             }
         }
     } else if (warp >= 4) {
-        const int quad = warp & 3;
+        const int quad = warp & 3, half = (warp - 4) >> 2, wi = warp - 4;
+        const int tid = threadIdx.x - 128;
         const uint32_t lane_base = static_cast<uint32_t>(quad * 32) << 16;
+        const uint32_t h0 = half * kHT;                        // this thread's first head of the group
+        const int key = 16 * quad + (lane & 15);               // its position within the tile (lanes 0-15)
         const float ninf = __int_as_float(0xff800000);
-        float* alpha_s = reinterpret_cast<float*>(base_ptr + kPAlphaOff);
-        volatile int* grow_s = reinterpret_cast<volatile int*>(alpha_s + 64);
-        float* l_s = reinterpret_cast<float*>(base_ptr + kPMlOff);
-        const int head = hg * G + lane;
-        const bool live = lane < G && head < a.heads;
+        volatile int* vote_s = reinterpret_cast<volatile int*>(base_ptr + kPVoteOff);
         // rows without a visible tile are nobody's: zeros, shared out over the CTAs
         if (hg == 0)
             for (int b = range; b < a.batch; b += a.n_ranges)
                 if (row_tiles(a, b).n == 0)
-                    for (int c = threadIdx.x - 128; c < a.heads * 64; c += 128)
+                    for (int c = tid; c < a.heads * 64; c += 128 * kHalves)
                         reinterpret_cast<uint4*>(a.out + static_cast<int64_t>(b) * a.heads * 512)[c] = make_uint4(0u, 0u, 0u, 0u);
-        float m_ref = ninf, l = 0.f;
+        uint32_t votes = 0;                                    // phases of `vote` taken
+        auto meet = [&](int code) {                            // all softmax warps have come this far
+            __syncwarp();
+            if (lane == 0) mbar_arrive(vote);
+            return mbar_wait_warp(vote, votes++ & 1, abort_flag, code);
+        };
+        float l[kHT];
         int flags4 = 0;
+        bool open = false;                                     // every head has a maximum
         for (int g = 0; g < n_tiles; ++g) {
             const int st = g & 1;
             if (!mbar_wait_warp(kfull(st), (g >> 1) & 1, abort_flag, 84)) break;
@@ -455,157 +507,165 @@ __global__ void __launch_bounds__(kPThreads, 1) mla_paged_kernel(const __grid_co
             const int flags = info_s[st].flags, b = info_s[st].row;
             const bool first = flags & 1, last = flags & 2;
             flags4 = (first ? 0 : flags4) | (flags & 12);
+            const bool seen = lane < 16 && (mask >> key & 1);
+            if (first) {
+                open = false;
+#pragma unroll
+                for (int i = 0; i < kHT; ++i) l[i] = 0.f;
+            }
             if (!mbar_wait_warp(sfull(st), (g >> 1) & 1, abort_flag, 85)) break;
             tc_fence_after();
-            uint32_t pk[32];
-            if (quad == 0) {
-                if (first) {
-                    m_ref = ninf;
-                    l = 0.f;
-                }
-                uint32_t r0[32], r1[32];
-                const uint32_t ts = tmem_base + kPTmemS + static_cast<uint32_t>(st) * kPTile;
-                tmem_ld_32x32(ts, r0);
-                tmem_ld_32x32(ts + 32, r1);
-                tmem_ld_wait(r0);
-                tmem_ld_wait(r1);
-                const uint64_t seen = live ? mask : 0ull;
+            uint32_t r[kHT];
+            tmem_ld_cols(tmem_base + lane_base + kTmemS + static_cast<uint32_t>(st) * G + h0, r);
+            // against the maxima so far: does any score exceed its own by more than 2^8?
+            bool over = !open;
+            if (open) {
+                float top = ninf;
 #pragma unroll
-                for (int i = 0; i < 32; ++i) {
-                    r0[i] = __float_as_uint(__uint_as_float(r0[i]) * a.scale_log2);
-                    r1[i] = __float_as_uint(__uint_as_float(r1[i]) * a.scale_log2);
+                for (int i = 0; i < kHT; i += 4) {
+                    const float4 mu = *reinterpret_cast<const float4*>(mu_s + h0 + i);
+                    top = fmaxf(top, fmaxf(fmaf(__uint_as_float(r[i]), a.scale_log2, -mu.x), fmaf(__uint_as_float(r[i + 1]), a.scale_log2, -mu.y)));
+                    top = fmaxf(top, fmaxf(fmaf(__uint_as_float(r[i + 2]), a.scale_log2, -mu.z), fmaf(__uint_as_float(r[i + 3]), a.scale_log2, -mu.w)));
                 }
-                if (seen != ~0ull) {
-                    const uint32_t lo = static_cast<uint32_t>(seen), hi = static_cast<uint32_t>(seen >> 32);
+                over = seen && top > 8.f;
+            }
+            over = __any_sync(0xffffffffu, over);
+            if (lane == 0) vote_s[st * 8 + wi] = over ? 1 : 0;
+            if (!meet(86)) break;
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) {
-                        if (!(lo >> i & 1)) r0[i] = 0xff800000u;
-                        if (!(hi >> i & 1)) r1[i] = 0xff800000u;
+            for (int w = 0; w < kWarps; ++w) over |= vote_s[st * 8 + w] != 0;
+            if (over) {
+#pragma unroll
+                for (int c = 0; c < kHT; c += 16) {
+                    float x[16];
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) x[i] = seen ? __uint_as_float(r[c + i]) * a.scale_log2 : ninf;
+                    const float top = reduce16(x, [](float u, float w) { return fmaxf(u, w); });
+                    if (lane < 16) w_s[quad * 64 + h0 + c + lane] = top;
+                }
+                if (!meet(89)) break;
+                if (tid < G) {
+                    const float mt = fmaxf(fmaxf(w_s[tid], w_s[64 + tid]), fmaxf(w_s[128 + tid], w_s[192 + tid]));
+                    const float old = first ? ninf : m_s[tid];
+                    const bool grow = mt > old + 8.f;          // false while mt is -infinity
+                    const float now = grow ? mt : old;
+                    m_s[tid] = now;
+                    mu_s[tid] = now == ninf ? 0.f : now;
+                    w_s[tid] = grow ? exp2_fast(old - now) : 1.f;
+                }
+                if (!meet(90)) break;
+                open = true;
+#pragma unroll
+                for (int i = 0; i < kHT; ++i) l[i] *= w_s[h0 + i];
+#pragma unroll
+                for (int i = 0; i < G; i += 32) open &= m_s[G < 32 ? lane & (G - 1) : i + lane] != ninf;
+                open = __all_sync(0xffffffffu, open);
+            }
+            uint32_t pk[kHT / 2];
+#pragma unroll
+            for (int i = 0; i < kHT; i += 4) {
+                const float4 mu = *reinterpret_cast<const float4*>(mu_s + h0 + i);
+                float p0 = exp2_fast(fmaf(__uint_as_float(r[i]), a.scale_log2, -mu.x));
+                float p1 = exp2_fast(fmaf(__uint_as_float(r[i + 1]), a.scale_log2, -mu.y));
+                float p2 = exp2_fast(fmaf(__uint_as_float(r[i + 2]), a.scale_log2, -mu.z));
+                float p3 = exp2_fast(fmaf(__uint_as_float(r[i + 3]), a.scale_log2, -mu.w));
+                if (!seen) p0 = p1 = p2 = p3 = 0.f;
+                l[i] += p0;
+                l[i + 1] += p1;
+                l[i + 2] += p2;
+                l[i + 3] += p3;
+                pk[i / 2] = pack_bf16x2(p0, p1);
+                pk[i / 2 + 1] = pack_bf16x2(p2, p3);
+            }
+            if (half == 0) {
+                // rows of a step that is multiplied, but not visible: zeros
+                const uint32_t step = static_cast<uint32_t>(mask >> (16 * quad)) & 0xffffu;
+                if (step != 0 && step != 0xffffu) {
+                    uint8_t* kt = base_ptr + kPKOff + st * kPTileBytes + quad * 16384;
+                    for (uint32_t z = ~step & 0xffffu; z; z &= z - 1) {
+                        const int row = __ffs(static_cast<int>(z)) - 1;
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            const int piece = lane + 32 * i;
+                            *reinterpret_cast<uint4*>(kt + (row >> 3) * 8192 + (piece >> 3) * 1024 + (row & 7) * 128 +
+                                                      (piece & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
+                        }
                     }
                 }
-                float mx[4] = {ninf, ninf, ninf, ninf};
-#pragma unroll
-                for (int i = 0; i < 32; ++i) {
-                    mx[i & 1] = fmaxf(mx[i & 1], __uint_as_float(r0[i]));
-                    mx[2 + (i & 1)] = fmaxf(mx[2 + (i & 1)], __uint_as_float(r1[i]));
-                }
-                const float mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-                const bool grow = mt > m_ref + 8.f;          // false while mt is -inf
-                const float m_new = grow ? mt : m_ref;
-                const float alpha = grow ? exp2_fast(m_ref - m_new) : 1.f;
-                const float m_use = m_new == ninf ? 0.f : m_new;
-                float sum[2] = {0.f, 0.f};
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const float p0 = exp2_fast(__uint_as_float(r0[2 * i]) - m_use), p1 = exp2_fast(__uint_as_float(r0[2 * i + 1]) - m_use);
-                    const float p2 = exp2_fast(__uint_as_float(r1[2 * i]) - m_use), p3 = exp2_fast(__uint_as_float(r1[2 * i + 1]) - m_use);
-                    sum[0] += p0 + p1;
-                    sum[1] += p2 + p3;
-                    pk[i] = pack_bf16x2(p0, p1);
-                    pk[16 + i] = pack_bf16x2(p2, p3);
-                }
-                l = l * alpha + (sum[0] + sum[1]);
-                m_ref = m_new;
-                alpha_s[st * 32 + lane] = alpha;
-                const bool any = __any_sync(0xffffffffu, grow);
-                if (lane == 0) grow_s[st] = any ? 1 : 0;
-                if (last) l_s[st * 32 + lane] = l;
-                __syncwarp();
-                if (lane == 0) mbar_arrive(afull(st));
-            } else if (mask != ~0ull) {
-                // rows of the steps that are multiplied, but not visible
-                uint64_t z = 0;
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const uint64_t step = 0xffffull << (16 * k);
-                    if (mask & step) z |= step & ~mask;
-                }
-                uint8_t* kt = base_ptr + kPKOff + st * kPTileBytes;
-                const int t = threadIdx.x - 160;                 // 96 threads, 64 pieces of a row
-                while (z) {
-                    const int r = __ffsll(static_cast<long long>(z)) - 1;
-                    z &= z - 1;
-                    if (t < 64)
-                        *reinterpret_cast<uint4*>(kt + (r >> 3) * 8192 + (t >> 3) * 1024 + (r & 7) * 128 + (t & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
-                }
-                fence_proxy_async();
             }
-            if (!mbar_wait_warp(afull(st), (g >> 1) & 1, abort_flag, 86)) break;
-            // read before this warp's arrival on pfull, behind which the slot may be written again
-            const float den = last ? l_s[st * 32 + lane] : 0.f;
             if (g > 0) {
-                // P V of the tile before has retired: P may be overwritten, O is at rest
+                // O += P V of the tile before has retired: P may be overwritten, O is at rest
                 if (!mbar_wait_warp(pfree, (g - 1) & 1, abort_flag, 87)) break;
                 tc_fence_after();
-                if (!first && grow_s[st]) {
-                    const float al = alpha_s[st * 32 + lane];
+                if (over && !first) {
 #pragma unroll 1
-                    for (int c = 0; c < 4; ++c) {
-                        uint32_t o[32];
-                        tmem_ld_32x32(tmem_base + lane_base + c * 32, o);
-                        tmem_ld_wait(o);
+                    for (int f = 0; f < 4; ++f) {
+                        uint32_t o[kHT];
+                        const uint32_t at = tmem_base + lane_base + f * G + h0;
+                        tmem_ld_cols(at, o);
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * al);
-                        tmem_st_32x32(tmem_base + lane_base + c * 32, o);
+                        for (int i = 0; i < kHT; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * w_s[h0 + i]);
+                        tmem_st_cols(at, o);
                     }
                     tmem_st_wait();
                 }
             }
-            if (quad == 0) {
-                // P row: 64 bf16 = 8 pieces of 16 bytes in a 128-byte swizzled row
-                uint8_t* prow = base_ptr + kPPOff + (96 + lane) * 128;
+            if (lane < 16) {
+                uint8_t* line = base_ptr + kPPOff + key * 128;
 #pragma unroll
-                for (int c = 0; c < 8; ++c)
-                    *reinterpret_cast<uint4*>(prow + ((c ^ (lane & 7)) << 4)) =
+                for (int c = 0; c < kHT / 8; ++c)
+                    *reinterpret_cast<uint4*>(line + ((((h0 >> 3) + c) ^ (key & 7)) << 4)) =
                         make_uint4(pk[4 * c], pk[4 * c + 1], pk[4 * c + 2], pk[4 * c + 3]);
-                fence_proxy_async();
             }
+            fence_proxy_async();
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(pfull);
             if (last) {
+                // the sums of a head over the positions: lanes, then quarters (in order)
+                if (!meet(91)) break;                          // w_s has been read
+#pragma unroll
+                for (int c = 0; c < kHT; c += 16) {
+                    float x[16];
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) x[i] = l[c + i];
+                    const float sum = reduce16(x, [](float u, float w) { return u + w; });
+                    if (lane < 16) w_s[quad * 64 + h0 + c + lane] = sum;
+                }
+                if (!meet(92)) break;
                 if (!mbar_wait_warp(pfree, g & 1, abort_flag, 88)) break;
                 tc_fence_after();
                 const int part = part_slot(flags4, range);
-                if (part < 0) {
-                    // the row's only part: a row of no weight at all (every page out of the pool, every score
-                    // -infinity) is zero
-                    const float inv = 1.f / den;
-                    __nv_bfloat16* orow = a.out + (static_cast<int64_t>(b) * a.heads + head) * 512 + quad * 128;
+                const int head0 = hg * G + static_cast<int>(h0), d0 = quad * 32 + lane;
+                if (part >= 0 && tid < G && hg * G + tid < a.heads) {
+                    const float den = (w_s[tid] + w_s[64 + tid]) + (w_s[128 + tid] + w_s[192 + tid]);
+                    *reinterpret_cast<float2*>(a.part_ml + (static_cast<int64_t>(part) * a.heads + hg * G + tid) * 2) =
+                        make_float2(den == 0.f ? ninf : m_s[tid], den);
+                }
+#pragma unroll
+                for (int i = 0; i < kHT; ++i) {
+                    const float* w = w_s + h0 + i;
+                    const float den = (w[0] + w[64]) + (w[128] + w[192]);
+                    l[i] = den == 0.f ? 0.f : part < 0 ? 1.f / den : 1.f;
+                }
+                // a head of no weight at all (every page out of the pool, every score -infinity) is zero
+                auto scaled = [](uint32_t o, float f) { return f == 0.f ? 0.f : __uint_as_float(o) * f; };
 #pragma unroll 1
-                    for (int c = 0; c < 4; ++c) {
-                        uint32_t o[32];
-                        tmem_ld_32x32(tmem_base + lane_base + c * 32, o);
-                        tmem_ld_wait(o);
-                        if (live) {
+                for (int f = 0; f < 4; ++f) {
+                    uint32_t o[kHT];
+                    tmem_ld_cols(tmem_base + lane_base + f * G + h0, o);
+                    if (part < 0) {
+                        __nv_bfloat16* to = a.out + (static_cast<int64_t>(b) * a.heads + head0) * 512 + f * 128 + d0;
 #pragma unroll
-                            for (int i = 0; i < 4; ++i) {
-                                uint32_t w[4];
+                        for (int i = 0; i < kHT; ++i)
+                            if (head0 + i < a.heads)
+                                to[i * 512] = __float2bfloat16_rn(scaled(o[i], l[i]));
+                    } else {
+                        float* to = a.part_o + (static_cast<int64_t>(part) * a.heads + head0) * 512 + f * 128 + d0;
 #pragma unroll
-                                for (int k = 0; k < 4; ++k)
-                                    w[k] = den == 0.f ? 0u
-                                                      : pack_bf16x2(__uint_as_float(o[8 * i + 2 * k]) * inv,
-                                                                    __uint_as_float(o[8 * i + 2 * k + 1]) * inv);
-                                *reinterpret_cast<uint4*>(orow + c * 32 + 8 * i) = make_uint4(w[0], w[1], w[2], w[3]);
-                            }
-                        }
+                        for (int i = 0; i < kHT; ++i)
+                            if (head0 + i < a.heads) to[i * 512] = scaled(o[i], l[i]);
                     }
-                } else {
-                    const int64_t prt = static_cast<int64_t>(part) * a.heads + head;
-                    float* po = a.part_o + prt * 512 + quad * 128;
-#pragma unroll 1
-                    for (int c = 0; c < 4; ++c) {
-                        uint32_t o[32];
-                        tmem_ld_32x32(tmem_base + lane_base + c * 32, o);
-                        tmem_ld_wait(o);
-                        if (live) {
-#pragma unroll
-                            for (int i = 0; i < 32; i += 4)
-                                *reinterpret_cast<uint4*>(po + c * 32 + i) =
-                                    den == 0.f ? make_uint4(0u, 0u, 0u, 0u) : make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
-                        }
-                    }
-                    if (live && quad == 0) *reinterpret_cast<float2*>(a.part_ml + prt * 2) = make_float2(m_ref, l);
                 }
                 tc_fence_before();
                 __syncwarp();
@@ -617,7 +677,7 @@ __global__ void __launch_bounds__(kPThreads, 1) mla_paged_kernel(const __grid_co
     __syncthreads();
     if (warp == 0) {
         tc_fence_after();
-        tmem_dealloc(tmem_base, 256);
+        tmem_dealloc(tmem_base, kTmemCols);
     }
 }
 
@@ -707,16 +767,29 @@ int paged_attn_error_take() {
     return v;
 }
 
-// Heads of a CTA, and the ranges that the tiles are cut into.
+// Heads of a CTA (the fewest groups, then the narrowest that holds its share), and the ranges that the tiles
+// are cut into.
 static int paged_group(int64_t heads) {
-    return static_cast<int>(heads >= kPMaxG ? kPMaxG : (heads + 7) / 8 * 8);
+    const int64_t groups = (heads + kPMaxG - 1) / kPMaxG, share = (heads + groups - 1) / groups;
+    return share <= 16 ? 16 : share <= 32 ? 32 : 64;
 }
 static int paged_ranges(int64_t heads) {
     const int64_t groups = (heads + paged_group(heads) - 1) / paged_group(heads);
-    const int64_t sms = sm_count();
-    int64_t r = sms / groups;
-    if (r < 1) r = 1;
-    return static_cast<int>(r < kJoinMaxParts ? r : kJoinMaxParts);
+    const int64_t r = sm_count() / groups;
+    return static_cast<int>(r < 1 ? 1 : r < kJoinMaxParts ? r : kJoinMaxParts);
+}
+
+template <int G>
+static int launch_paged(const CUtensorMap& tm_qa, const CUtensorMap& tm_qp, const CUtensorMap& tm_kv,
+                        const CUtensorMap& tm_pe, const PagedArgs& a, cudaStream_t s) {
+    if (int rc = ensure_dynamic_smem(reinterpret_cast<const void*>(&mla_paged_kernel<G>), static_cast<int>(kPSmemBytes),
+                                     "rt_mla_paged_decode"))
+        return rc;
+    const int groups = (a.heads + G - 1) / G;
+    mla_paged_kernel<G><<<static_cast<unsigned>(a.n_ranges * groups), kPThreads<G>, kPSmemBytes, s>>>(tm_qa, tm_qp, tm_kv,
+                                                                                                    tm_pe, a);
+    count_launch();
+    return check_launch("mla_paged_kernel");
 }
 
 }  // namespace tc
@@ -768,7 +841,7 @@ extern "C" int rt_mla_paged_decode(const void* q_abs, const void* q_pe, const vo
     a.window = static_cast<int>(window > longest ? 0 : window);
     a.sinks = static_cast<int>(sinks > longest ? longest : sinks);
     a.scale_log2 = softmax_scale * 1.4426950408889634f;
-    a.group = tc::paged_group(heads);
+    const int group = tc::paged_group(heads);
     a.n_ranges = tc::paged_ranges(heads);
     a.ranges = static_cast<int4*>(workspace);
     a.part_ml = reinterpret_cast<float*>(a.ranges + a.n_ranges);
@@ -782,13 +855,13 @@ extern "C" int rt_mla_paged_decode(const void* q_abs, const void* q_pe, const vo
     {
         const uint64_t dims[] = {64, static_cast<uint64_t>(heads), 8, static_cast<uint64_t>(batch)};
         const uint64_t st[] = {static_cast<uint64_t>(u * qa_head_stride), 128, static_cast<uint64_t>(u * qa_batch_stride)};
-        const uint32_t box[] = {64, static_cast<uint32_t>(a.group), 8, 1};
+        const uint32_t box[] = {64, static_cast<uint32_t>(group), 8, 1};
         if (int rc = tc::make_tmap_bf16(&tm_qa, q_abs, 4, dims, st, box)) return rc;
     }
     {
         const uint64_t dims[] = {64, static_cast<uint64_t>(heads), static_cast<uint64_t>(batch)};
         const uint64_t st[] = {static_cast<uint64_t>(u * qp_head_stride), static_cast<uint64_t>(u * qp_batch_stride)};
-        const uint32_t box[] = {64, static_cast<uint32_t>(a.group), 1};
+        const uint32_t box[] = {64, static_cast<uint32_t>(group), 1};
         if (int rc = tc::make_tmap_bf16(&tm_qp, q_pe, 3, dims, st, box)) return rc;
     }
     {
@@ -803,15 +876,11 @@ extern "C" int rt_mla_paged_decode(const void* q_abs, const void* q_pe, const vo
         const uint32_t box[] = {64, box_rows, 1};
         if (int rc = tc::make_tmap_bf16(&tm_pe, pe, 3, dims, st, box)) return rc;
     }
-    if (int rc = ensure_dynamic_smem(reinterpret_cast<const void*>(&tc::mla_paged_kernel),
-                                     static_cast<int>(tc::kPSmemBytes), "rt_mla_paged_decode"))
-        return rc;
-    const int groups = (a.heads + a.group - 1) / a.group;
     cudaStream_t s = as_stream(stream);
-    tc::mla_paged_kernel<<<static_cast<unsigned>(a.n_ranges * groups), tc::kPThreads, tc::kPSmemBytes, s>>>(
-        tm_qa, tm_qp, tm_kv, tm_pe, a);
-    count_launch();
-    if (int rc = check_launch("mla_paged_kernel")) return rc;
+    if (int rc = group == 16   ? tc::launch_paged<16>(tm_qa, tm_qp, tm_kv, tm_pe, a, s)
+                 : group == 32 ? tc::launch_paged<32>(tm_qa, tm_qp, tm_kv, tm_pe, a, s)
+                               : tc::launch_paged<64>(tm_qa, tm_qp, tm_kv, tm_pe, a, s))
+        return rc;
     if (a.n_ranges == 1) return RT_OK;
     dim3 grid(static_cast<unsigned>(heads), static_cast<unsigned>(a.n_ranges - 1));
     tc::mla_paged_join_kernel<<<grid, tc::kJoinThreads, 0, s>>>(a);
