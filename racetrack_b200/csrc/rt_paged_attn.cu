@@ -49,8 +49,7 @@ __device__ __forceinline__ int row_slot(const PagedArgs& a, int b) {
     return s >= 0 && s < a.slots ? s : -1;
 }
 
-__device__ __forceinline__ RowTiles row_tiles(const PagedArgs& a, int b) {
-    const int s = row_slot(a, b);
+__device__ __forceinline__ RowTiles slot_tiles(const PagedArgs& a, int s) {
     const int most = a.width << a.page_log;
     RowTiles t;
     t.len = s < 0 ? 0 : min(max(__ldg(a.lens + s), 0), most);
@@ -66,6 +65,7 @@ __device__ __forceinline__ RowTiles row_tiles(const PagedArgs& a, int b) {
     }
     return t;
 }
+__device__ __forceinline__ RowTiles row_tiles(const PagedArgs& a, int b) { return slot_tiles(a, row_slot(a, b)); }
 
 __device__ __forceinline__ int tile_of(const RowTiles& t, int j) { return j < t.na ? j : t.b0 + (j - t.na); }
 
@@ -82,9 +82,9 @@ __device__ __forceinline__ uint64_t tile_mask(const PagedArgs& a, const RowTiles
 }
 
 // The range of this CTA: its first row and tile, and how many tiles it walks. All threads call it; every
-// thread sums the rows of one slice of the batch. `scratch`: THREADS / 32 + 3 ints of shared memory.
+// thread sums the rows of one slice of the batch. `scratch`: THREADS / 32 + 4 ints of shared memory.
 struct RangeStart {
-    int row, tile, count;
+    int row, tile, count, slot;      // (the row's slot: a load less in front of the first tile)
 };
 template <int THREADS>
 __device__ RangeStart find_range(const PagedArgs& a, int range, volatile int* scratch) {
@@ -103,7 +103,7 @@ __device__ RangeStart find_range(const PagedArgs& a, int range, volatile int* sc
     if (lane == 31) scratch[warp] = x;
     if (threadIdx.x == 0) {
         found[0] = -1;
-        found[1] = found[2] = 0;
+        found[1] = found[2] = found[3] = 0;
     }
     __syncthreads();
     int before = x - mine, total = 0;
@@ -125,9 +125,10 @@ __device__ RangeStart find_range(const PagedArgs& a, int range, volatile int* sc
         found[0] = b;
         found[1] = first - at;
         found[2] = t.n;
+        found[3] = row_slot(a, b);
     }
     __syncthreads();
-    RangeStart r{found[0], found[1], 0};
+    RangeStart r{found[0], found[1], 0, found[3]};
     if (r.row >= 0) r.count = min(per_range, total - first);
     if (threadIdx.x == 0) a.ranges[range] = make_int4(r.row, r.tile, found[2], per_range);
     return r;
@@ -319,6 +320,7 @@ __global__ void __launch_bounds__(kPThreads<G>, 1) mla_paged_kernel(const __grid
     tc_fence_after();
     const uint32_t tmem_base = *slot_ptr;
     const int n_tiles = start.count;
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");     // the join kernel may be set up
 
     if (warp == 0) {
         if (n_tiles > 0 && elect_one()) {
@@ -404,22 +406,17 @@ __global__ void __launch_bounds__(kPThreads<G>, 1) mla_paged_kernel(const __grid
     } else if (warp == 1) {
         // the whole warp walks the range (lanes fetch page numbers), one thread issues the loads
         int b = start.row, j = start.tile, seg = 0;
-        RowTiles t{};
-        int row_at = -1;
-        int slot_row = -1;
+        int slot_row = start.slot, row_at = b;
+        RowTiles t = n_tiles > 0 ? slot_tiles(a, slot_row) : RowTiles{};
         const int page = 1 << a.page_log;
         const int boxes = page < kPTile ? kPTile / page : 1;   // pages of a tile
         int32_t fetched = -1;                                   // lane: page number of entry fetched0 + lane
         int fetched0 = -1, fetched_row = -1;
         for (int g = 0; g < n_tiles; ++g) {
             if (row_at != b) {
-                t = row_tiles(a, b);
-                while (j >= t.n) {                              // rows without a tile
-                    t = row_tiles(a, ++b);
-                    j = 0;
-                }
+                t = slot_tiles(a, slot_row = row_slot(a, b));
+                while (t.n == 0) t = slot_tiles(a, slot_row = row_slot(a, ++b));     // rows without a tile
                 row_at = b;
-                slot_row = row_slot(a, b);
             }
             const bool first = g == 0 || j == 0;
             const bool last = g == n_tiles - 1 || j == t.n - 1;
@@ -515,33 +512,55 @@ __global__ void __launch_bounds__(kPThreads<G>, 1) mla_paged_kernel(const __grid
             }
             if (!mbar_wait_warp(sfull(st), (g >> 1) & 1, abort_flag, 85)) break;
             tc_fence_after();
-            uint32_t r[kHT];
-            tmem_ld_cols(tmem_base + lane_base + kTmemS + static_cast<uint32_t>(st) * G + h0, r);
-            // against the maxima so far: does any score exceed its own by more than 2^8?
-            bool over = !open;
-            if (open) {
-                float top = ninf;
+            float x[kHT];
+            // P against the maxima so far, and whether a score exceeds one of them by more than 2^8; what the
+            // other warps found comes in while the exponentials are evaluated
+            auto scores = [&] {
+                uint32_t r[kHT];
+                tmem_ld_cols(tmem_base + lane_base + kTmemS + static_cast<uint32_t>(st) * G + h0, r);
+#pragma unroll
+                for (int i = 0; i < kHT; ++i) x[i] = __uint_as_float(r[i]);
+            };
+            float top = ninf;
+            auto against = [&] {
 #pragma unroll
                 for (int i = 0; i < kHT; i += 4) {
                     const float4 mu = *reinterpret_cast<const float4*>(mu_s + h0 + i);
-                    top = fmaxf(top, fmaxf(fmaf(__uint_as_float(r[i]), a.scale_log2, -mu.x), fmaf(__uint_as_float(r[i + 1]), a.scale_log2, -mu.y)));
-                    top = fmaxf(top, fmaxf(fmaf(__uint_as_float(r[i + 2]), a.scale_log2, -mu.z), fmaf(__uint_as_float(r[i + 3]), a.scale_log2, -mu.w)));
+                    x[i] = fmaf(x[i], a.scale_log2, -mu.x);
+                    x[i + 1] = fmaf(x[i + 1], a.scale_log2, -mu.y);
+                    x[i + 2] = fmaf(x[i + 2], a.scale_log2, -mu.z);
+                    x[i + 3] = fmaf(x[i + 3], a.scale_log2, -mu.w);
+                    top = fmaxf(top, fmaxf(fmaxf(x[i], x[i + 1]), fmaxf(x[i + 2], x[i + 3])));
                 }
+            };
+            auto exponentials = [&] {
+#pragma unroll
+                for (int i = 0; i < kHT; ++i) x[i] = seen ? exp2_fast(x[i]) : 0.f;
+            };
+            scores();
+            bool over = !open;
+            if (open) {
+                against();
                 over = seen && top > 8.f;
             }
             over = __any_sync(0xffffffffu, over);
-            if (lane == 0) vote_s[st * 8 + wi] = over ? 1 : 0;
-            if (!meet(86)) break;
+            if (lane == 0) {
+                vote_s[st * 8 + wi] = over ? 1 : 0;
+                mbar_arrive(vote);
+            }
+            if (open) exponentials();
+            if (!mbar_wait_warp(vote, votes++ & 1, abort_flag, 86)) break;
 #pragma unroll
             for (int w = 0; w < kWarps; ++w) over |= vote_s[st * 8 + w] != 0;
             if (over) {
+                if (open) scores();
 #pragma unroll
                 for (int c = 0; c < kHT; c += 16) {
-                    float x[16];
+                    float y[16];
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) x[i] = seen ? __uint_as_float(r[c + i]) * a.scale_log2 : ninf;
-                    const float top = reduce16(x, [](float u, float w) { return fmaxf(u, w); });
-                    if (lane < 16) w_s[quad * 64 + h0 + c + lane] = top;
+                    for (int i = 0; i < 16; ++i) y[i] = seen ? x[c + i] * a.scale_log2 : ninf;
+                    const float most = reduce16(y, [](float u, float w) { return fmaxf(u, w); });
+                    if (lane < 16) w_s[quad * 64 + h0 + c + lane] = most;
                 }
                 if (!meet(89)) break;
                 if (tid < G) {
@@ -554,28 +573,21 @@ __global__ void __launch_bounds__(kPThreads<G>, 1) mla_paged_kernel(const __grid
                     w_s[tid] = grow ? exp2_fast(old - now) : 1.f;
                 }
                 if (!meet(90)) break;
-                open = true;
 #pragma unroll
                 for (int i = 0; i < kHT; ++i) l[i] *= w_s[h0 + i];
+                open = true;
 #pragma unroll
                 for (int i = 0; i < G; i += 32) open &= m_s[G < 32 ? lane & (G - 1) : i + lane] != ninf;
                 open = __all_sync(0xffffffffu, open);
+                against();
+                exponentials();
             }
             uint32_t pk[kHT / 2];
 #pragma unroll
-            for (int i = 0; i < kHT; i += 4) {
-                const float4 mu = *reinterpret_cast<const float4*>(mu_s + h0 + i);
-                float p0 = exp2_fast(fmaf(__uint_as_float(r[i]), a.scale_log2, -mu.x));
-                float p1 = exp2_fast(fmaf(__uint_as_float(r[i + 1]), a.scale_log2, -mu.y));
-                float p2 = exp2_fast(fmaf(__uint_as_float(r[i + 2]), a.scale_log2, -mu.z));
-                float p3 = exp2_fast(fmaf(__uint_as_float(r[i + 3]), a.scale_log2, -mu.w));
-                if (!seen) p0 = p1 = p2 = p3 = 0.f;
-                l[i] += p0;
-                l[i + 1] += p1;
-                l[i + 2] += p2;
-                l[i + 3] += p3;
-                pk[i / 2] = pack_bf16x2(p0, p1);
-                pk[i / 2 + 1] = pack_bf16x2(p2, p3);
+            for (int i = 0; i < kHT; i += 2) {
+                l[i] += x[i];
+                l[i + 1] += x[i + 1];
+                pk[i / 2] = pack_bf16x2(x[i], x[i + 1]);
             }
             if (half == 0) {
                 // rows of a step that is multiplied, but not visible: zeros
@@ -626,30 +638,36 @@ __global__ void __launch_bounds__(kPThreads<G>, 1) mla_paged_kernel(const __grid
                 if (!meet(91)) break;                          // w_s has been read
 #pragma unroll
                 for (int c = 0; c < kHT; c += 16) {
-                    float x[16];
+                    float y[16];
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) x[i] = l[c + i];
-                    const float sum = reduce16(x, [](float u, float w) { return u + w; });
+                    for (int i = 0; i < 16; ++i) y[i] = l[c + i];
+                    const float sum = reduce16(y, [](float u, float w) { return u + w; });
                     if (lane < 16) w_s[quad * 64 + h0 + c + lane] = sum;
                 }
                 if (!meet(92)) break;
-                if (!mbar_wait_warp(pfree, g & 1, abort_flag, 88)) break;
-                tc_fence_after();
                 const int part = part_slot(flags4, range);
                 const int head0 = hg * G + static_cast<int>(h0), d0 = quad * 32 + lane;
-                if (part >= 0 && tid < G && hg * G + tid < a.heads) {
+                // one thread a head: the denominator, and what O is multiplied with (0 for a head of no weight at
+                // all, every page out of the pool or every score -infinity: it is zero)
+                if (tid < G) {
                     const float den = (w_s[tid] + w_s[64 + tid]) + (w_s[128 + tid] + w_s[192 + tid]);
-                    *reinterpret_cast<float2*>(a.part_ml + (static_cast<int64_t>(part) * a.heads + hg * G + tid) * 2) =
-                        make_float2(den == 0.f ? ninf : m_s[tid], den);
+                    if (part >= 0 && hg * G + tid < a.heads)
+                        *reinterpret_cast<float2*>(a.part_ml + (static_cast<int64_t>(part) * a.heads + hg * G + tid) * 2) =
+                            make_float2(den == 0.f ? ninf : m_s[tid], den);
+                    w_s[tid] = den == 0.f ? 0.f : part < 0 ? 1.f / den : 1.f;
                 }
+                if (!meet(93)) break;
 #pragma unroll
-                for (int i = 0; i < kHT; ++i) {
-                    const float* w = w_s + h0 + i;
-                    const float den = (w[0] + w[64]) + (w[128] + w[192]);
-                    l[i] = den == 0.f ? 0.f : part < 0 ? 1.f / den : 1.f;
+                for (int i = 0; i < kHT; i += 4) {
+                    const float4 w = *reinterpret_cast<const float4*>(w_s + h0 + i);
+                    l[i] = w.x;
+                    l[i + 1] = w.y;
+                    l[i + 2] = w.z;
+                    l[i + 3] = w.w;
                 }
-                // a head of no weight at all (every page out of the pool, every score -infinity) is zero
                 auto scaled = [](uint32_t o, float f) { return f == 0.f ? 0.f : __uint_as_float(o) * f; };
+                if (!mbar_wait_warp(pfree, g & 1, abort_flag, 88)) break;
+                tc_fence_after();
 #pragma unroll 1
                 for (int f = 0; f < 4; ++f) {
                     uint32_t o[kHT];
@@ -681,73 +699,83 @@ __global__ void __launch_bounds__(kPThreads<G>, 1) mla_paged_kernel(const __grid
     }
 }
 
-// Joins the parts of every row that crosses ranges: blockIdx.y + 1 is a range whose first tile lies inside a
-// row, and the block does the row if that is the row's first crossing. out = sum_s o_s 2^(m_s - M) / sum_s l_s
-// 2^(m_s - M), the parts in the order of their positions. Four threads share a group of four dims and take
-// every fourth part; their sums are added in order, so the result does not depend on timing.
-constexpr int kJoinThreads = 512;
+// Joins the parts of every row that crosses ranges: out = sum_s o_s 2^(m_s - M) / sum_s l_s 2^(m_s - M). A row
+// of P parts crosses P - 1 range borders, and blockIdx.y + 1 is a range, so the row has P - 1 blocks a head:
+// the first S of them (a power of two, at most 16) take 512 / S dims each, with S groups of threads that sum
+// every S-th part; the groups' sums are added in order, so the result does not depend on timing. A row
+// that is cut once is one block of 128 threads, one cut 147 times is 16 blocks of 16 x 8.
+constexpr int kJoinThreads = 128;
 constexpr int kJoinMaxParts = 160;
 __global__ void __launch_bounds__(kJoinThreads) mla_paged_join_kernel(const PagedArgs a) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");        // the parts are complete
     const int r = blockIdx.y + 1, head = blockIdx.x;
     const int4 rg = a.ranges[r];
     if (rg.x < 0 || rg.y == 0) return;
-    const int per = rg.w, t0 = r * per - rg.y, r0 = t0 / per;
-    if (r0 != r - 1) return;
-    const int r1 = (t0 + rg.z - 1) / per, parts = r1 - r0 + 1;
-    __shared__ float w_s[kJoinMaxParts], red[kJoinThreads / 32][2];
-    __shared__ float4 acc_s[3][128];
+    const int per = rg.w, t0 = r * per - rg.y, r0 = t0 / per, r1 = (t0 + rg.z - 1) / per, parts = r1 - r0 + 1;
+    const int slices = 1 << min(4, 31 - __clz(parts - 1)), slice = r - r0 - 1;
+    if (slice >= slices) return;
+    __shared__ float w_s[kJoinMaxParts], red[4][2];
+    __shared__ float4 acc_s[kJoinThreads];
     const float ninf = __int_as_float(0xff800000);
-    auto row_of = [&](int s) { return (static_cast<int64_t>(s == 0 ? 2 * r0 + 1 : 2 * (r0 + s)) * a.heads + head); };
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    float ms = ninf, ls = 0.f;
-    if (tid < parts) {
-        const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + row_of(tid) * 2);
-        ms = ml.x;
-        ls = ml.y;
+    auto row_of = [&](int s) { return static_cast<int64_t>(s == 0 ? 2 * r0 + 1 : 2 * (r0 + s)) * a.heads + head; };
+    const int wide = 128 / slices, c = slice * wide + (tid & (wide - 1)), q = tid / wide;
+    // the first parts' sums are under way while the weights are found
+    float4 o[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        o[i] = *(reinterpret_cast<const float4*>(a.part_o + row_of(min(q + i * slices, parts - 1)) * 512) + c);
+    float2 ml[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int s = tid + i * kJoinThreads;
+        ml[i] = s < parts ? *reinterpret_cast<const float2*>(a.part_ml + row_of(s) * 2) : make_float2(ninf, 0.f);
     }
-    float m = warp_max(ms);
+    float m = warp_max(fmaxf(ml[0].x, ml[1].x));
     if (lane == 0) red[warp][0] = m;
     __syncthreads();
-    m = red[0][0];
-#pragma unroll
-    for (int w = 1; w < kJoinMaxParts / 32; ++w) m = fmaxf(m, red[w][0]);
-    const float weight = ms == ninf ? (ls != 0.f ? ls : 0.f) : exp2f(ms - m);
-    if (tid < parts) w_s[tid] = weight;
-    const float d = warp_sum(tid < parts ? ls * weight : 0.f);
-    if (lane == 0) red[warp][1] = d;
-    __syncthreads();
+    m = fmaxf(fmaxf(red[0][0], red[1][0]), fmaxf(red[2][0], red[3][0]));
     float den = 0.f;
 #pragma unroll
-    for (int w = 0; w < kJoinMaxParts / 32; ++w) den += red[w][1];
-    const int q = tid >> 7, c = tid & 127;
+    for (int i = 0; i < 2; ++i) {
+        // a part without a maximum has no weight, or (NaN scores alone) NaN
+        const float w = ml[i].x == ninf ? (ml[i].y != 0.f ? ml[i].y : 0.f) : exp2f(ml[i].x - m);
+        const int s = tid + i * kJoinThreads;
+        if (s < parts) w_s[s] = w;
+        den += ml[i].y * w;
+    }
+    den = warp_sum(den);
+    if (lane == 0) red[warp][1] = den;
+    __syncthreads();
+    den = (red[0][1] + red[1][1]) + (red[2][1] + red[3][1]);
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int s0 = q; s0 < parts; s0 += 16) {
-        float4 o[4];
+    for (int s0 = q; s0 < parts; s0 += 4 * slices) {
+        if (s0 != q) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-            o[i] = __ldg(reinterpret_cast<const float4*>(a.part_o + row_of(min(s0 + 4 * i, parts - 1)) * 512) + c);
+            for (int i = 0; i < 4; ++i)
+                o[i] = *(reinterpret_cast<const float4*>(a.part_o + row_of(min(s0 + i * slices, parts - 1)) * 512) + c);
+        }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const int s = s0 + 4 * i;
-            if (s < parts) {
-                const float w = w_s[s];
+            if (s0 + i * slices < parts) {
+                const float w = w_s[s0 + i * slices];
                 acc.x += o[i].x * w; acc.y += o[i].y * w; acc.z += o[i].z * w; acc.w += o[i].w * w;
             }
         }
     }
-    if (q > 0) acc_s[q - 1][c] = acc;
-    __syncthreads();
-    if (q == 0) {
-#pragma unroll
-        for (int i = 0; i < 3; ++i) {
-            const float4 o = acc_s[i][c];
-            acc.x += o.x; acc.y += o.y; acc.z += o.z; acc.w += o.w;
+    if (slices > 1) {
+        acc_s[tid] = acc;
+        __syncthreads();
+        if (q != 0) return;
+        for (int i = 1; i < slices; ++i) {
+            const float4 v = acc_s[tid + i * wide];
+            acc.x += v.x; acc.y += v.y; acc.z += v.z; acc.w += v.w;
         }
-        const float inv = 1.f / den;
-        uint2 v = make_uint2(pack_bf16x2(acc.x * inv, acc.y * inv), pack_bf16x2(acc.z * inv, acc.w * inv));
-        if (den == 0.f) v = make_uint2(0u, 0u);
-        *reinterpret_cast<uint2*>(a.out + (static_cast<int64_t>(rg.x) * a.heads + head) * 512 + c * 4) = v;
     }
+    const float inv = 1.f / den;
+    uint2 v = make_uint2(pack_bf16x2(acc.x * inv, acc.y * inv), pack_bf16x2(acc.z * inv, acc.w * inv));
+    if (den == 0.f) v = make_uint2(0u, 0u);
+    *reinterpret_cast<uint2*>(a.out + (static_cast<int64_t>(rg.x) * a.heads + head) * 512 + c * 4) = v;
 }
 
 int sm_count();                                      // rt_gemm.cu
@@ -883,7 +911,21 @@ extern "C" int rt_mla_paged_decode(const void* q_abs, const void* q_pe, const vo
         return rc;
     if (a.n_ranges == 1) return RT_OK;
     dim3 grid(static_cast<unsigned>(heads), static_cast<unsigned>(a.n_ranges - 1));
-    tc::mla_paged_join_kernel<<<grid, tc::kJoinThreads, 0, s>>>(a);
+    // launched while the last CTAs of the kernel before still run; it waits for their parts itself
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(tc::kJoinThreads);
+    cfg.stream = s;
+    cudaLaunchAttribute early{};
+    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    early.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &early;
+    cfg.numAttrs = 1;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, tc::mla_paged_join_kernel, a);
     count_launch();
-    return check_launch("mla_paged_join_kernel");
+    if (e != cudaSuccess) {
+        cudaGetLastError();
+        return fail(RT_ERR_CUDA, "mla_paged_join_kernel: %s", cudaGetErrorString(e));
+    }
+    return RT_OK;
 }
