@@ -15,7 +15,7 @@ namespace rt {
 namespace tc {
 
 constexpr int kPTile = 64;                          // positions per tile
-constexpr uint32_t kPLatBytes = kPTile * 1024;      // latent part of a tile
+constexpr uint32_t kPHalfBytes = kPTile * 512;       // half of the latent dims of a tile
 constexpr uint32_t kPTileBytes = kPTile * 1152;
 constexpr int kPMaxBatch = 65535;
 
@@ -166,11 +166,11 @@ constexpr uint32_t kPQBytes = kPMaxG * kPQRow;       // two sets of queries of u
 constexpr uint32_t kPKOff = kPQBytes;
 constexpr uint32_t kPPOff = kPKOff + 2 * kPTileBytes;        // P: [64 positions][64 heads] bf16
 constexpr uint32_t kPBarOff = kPPOff + kPTile * 128;
-constexpr int kPBars = 14;      // qfull[2] qfree[2] kfull[2] kfree[2] sfull[2] vote pfull pfree ofree
+constexpr int kPBars = 20;      // qfull[2] qfree[2] kfull[2][2] kfree[2][2] sfull[2] vote pfull pfree efull odone ofree
 constexpr uint32_t kPInfoOff = kPBarOff + kPBars * 8 + 16;   // (tensor memory slot, abort flag before it)
-constexpr uint32_t kPVoteOff = kPInfoOff + 2 * 16;           // [2][8] ints
-constexpr uint32_t kPMaxOff = kPVoteOff + 2 * 8 * 4;         // m [64], m or 0 [64], per quarter [4][64]
-constexpr uint32_t kPSmemBytes = kPMaxOff + 6 * 64 * 4 + 1024;
+constexpr uint32_t kPVoteOff = kPInfoOff + 2 * 16;           // [2][4] ints, then the finished row, its part and tiles
+constexpr uint32_t kPMaxOff = kPVoteOff + 12 * 4;            // m [64], m or 0 [64], per quarter [4][64], factors [64]
+constexpr uint32_t kPSmemBytes = kPMaxOff + 7 * 64 * 4 + 1024;
 static_assert(kPKOff % 1024 == 0 && kPPOff % 1024 == 0 && kPInfoOff % 16 == 0 && kPMaxOff % 16 == 0, "alignment");
 static_assert(kPSmemBytes <= 232448, "shared memory budget");
 
@@ -228,20 +228,40 @@ __device__ __forceinline__ void tmem_ld_cols(uint32_t taddr, uint32_t (&r)[16]) 
 __device__ __forceinline__ void tmem_st_cols(uint32_t taddr, const uint32_t (&r)[32]) { tmem_st_32x32(taddr, r); }
 __device__ __forceinline__ void tmem_st_cols(uint32_t taddr, const uint32_t (&r)[16]) { tmem_st_32x16(taddr, r); }
 
-// Combines 16 values over lanes 0-15 with 15 shuffles: lane i is left with value i of all of them.
-template <typename F>
-__device__ __forceinline__ float reduce16(float (&v)[16], F f) {
-    const int lane = threadIdx.x & 31;
-#pragma unroll
-    for (int o = 8; o > 0; o >>= 1) {
-        const bool up = lane & o;
-#pragma unroll
-        for (int i = 0; i < o; ++i) {
-            const float give = up ? v[i] : v[i + o], keep = up ? v[i + o] : v[i];
-            v[i] = f(keep, __shfl_xor_sync(0xffffffffu, give, o));
-        }
-    }
-    return v[0];
+// Lanes 0-15 of the warp's quarter, 8 columns a register quadruple: lane t gets rows t / 4 (r[4 u], r[4 u + 1])
+// and t / 4 + 8 (r[4 u + 2], r[4 u + 3]) of columns 8 u + 2 (t % 4) and the next. Complete on return.
+__device__ __forceinline__ void tmem_ld_16x256b(uint32_t taddr, float (&x)[8]) {
+    asm volatile("tcgen05.ld.sync.aligned.16x256b.x2.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];\n\t"
+                 "tcgen05.wait::ld.sync.aligned;"
+                 : "=f"(x[0]), "=f"(x[1]), "=f"(x[2]), "=f"(x[3]), "=f"(x[4]), "=f"(x[5]), "=f"(x[6]), "=f"(x[7])
+                 : "r"(taddr)
+                 : "memory");
+}
+__device__ __forceinline__ void tmem_ld_16x256b(uint32_t taddr, float (&x)[16]) {
+    asm volatile("tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, "
+                 "%14, %15}, [%16];\n\ttcgen05.wait::ld.sync.aligned;"
+                 : "=f"(x[0]), "=f"(x[1]), "=f"(x[2]), "=f"(x[3]), "=f"(x[4]), "=f"(x[5]), "=f"(x[6]), "=f"(x[7]),
+                   "=f"(x[8]), "=f"(x[9]), "=f"(x[10]), "=f"(x[11]), "=f"(x[12]), "=f"(x[13]), "=f"(x[14]), "=f"(x[15])
+                 : "r"(taddr)
+                 : "memory");
+}
+__device__ __forceinline__ void tmem_ld_16x256b(uint32_t taddr, float (&x)[32]) {
+    asm volatile("tcgen05.ld.sync.aligned.16x256b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, "
+                 "%14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];\n\t"
+                 "tcgen05.wait::ld.sync.aligned;"
+                 : "=f"(x[0]), "=f"(x[1]), "=f"(x[2]), "=f"(x[3]), "=f"(x[4]), "=f"(x[5]), "=f"(x[6]), "=f"(x[7]),
+                   "=f"(x[8]), "=f"(x[9]), "=f"(x[10]), "=f"(x[11]), "=f"(x[12]), "=f"(x[13]), "=f"(x[14]), "=f"(x[15]),
+                   "=f"(x[16]), "=f"(x[17]), "=f"(x[18]), "=f"(x[19]), "=f"(x[20]), "=f"(x[21]), "=f"(x[22]), "=f"(x[23]),
+                   "=f"(x[24]), "=f"(x[25]), "=f"(x[26]), "=f"(x[27]), "=f"(x[28]), "=f"(x[29]), "=f"(x[30]), "=f"(x[31])
+                 : "r"(taddr)
+                 : "memory");
+}
+// Four 8 x 8 blocks of bf16 pairs held like the rows above into shared memory; lane t gives the address of row
+// t % 8 of block t / 8.
+__device__ __forceinline__ void stmatrix_x4(uint32_t addr, uint32_t r0, uint32_t r1, uint32_t r2, uint32_t r3) {
+    asm volatile("stmatrix.sync.aligned.m8n8.x4.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(r0), "r"(r1), "r"(r2),
+                 "r"(r3)
+                 : "memory");
 }
 
 // Where the result of a row's tiles in a range goes: the row's own output if they are all of its tiles, else
@@ -250,19 +270,14 @@ __device__ __forceinline__ int part_slot(int flags, int range) {
     return (flags & 12) == 12 ? -1 : 2 * range + ((flags & 4) ? 1 : 0);
 }
 
-// Softmax warps: one a quarter of tensor memory, two (each half of the heads) for 64 heads.
-template <int G>
-constexpr int kPHalves = G > 32 ? 2 : 1;
-template <int G>
-constexpr int kPThreads = 128 + 128 * kPHalves<G>;   // 0 MMA, 1 producer, 4.. softmax
+constexpr int kPThreads = 384;      // warps: 0 MMA, 1 producer, 4-7 softmax, 8-11 finished rows
 
 template <int G>
-__global__ void __launch_bounds__(kPThreads<G>, 1) mla_paged_kernel(const __grid_constant__ CUtensorMap tm_qa,
-                                                                    const __grid_constant__ CUtensorMap tm_qp,
-                                                                    const __grid_constant__ CUtensorMap tm_kv,
-                                                                    const __grid_constant__ CUtensorMap tm_pe,
-                                                                    const PagedArgs a) {
-    constexpr int kHalves = kPHalves<G>, kHT = G / kHalves, kWarps = 4 * kHalves;
+__global__ void __launch_bounds__(kPThreads, 1) mla_paged_kernel(const __grid_constant__ CUtensorMap tm_qa,
+                                                                 const __grid_constant__ CUtensorMap tm_qp,
+                                                                 const __grid_constant__ CUtensorMap tm_kv,
+                                                                 const __grid_constant__ CUtensorMap tm_pe,
+                                                                 const PagedArgs a) {
     constexpr int kQBufs = G > 32 ? 1 : 2;
     constexpr uint32_t kTmemS = 4 * G, kTmemCols = G == 16 ? 128 : G == 32 ? 256 : 512;
     // fp32 accumulate, bf16 x bf16; S: both K-major, M = 64; O: both MN-major, M = 128
@@ -275,17 +290,21 @@ __global__ void __launch_bounds__(kPThreads<G>, 1) mla_paged_kernel(const __grid
     const uint32_t bars = base + kPBarOff;
     auto qfull = [&](int s) { return bars + 8u * s; };
     auto qfree = [&](int s) { return bars + 8u * (2 + s); };
-    auto kfull = [&](int s) { return bars + 8u * (4 + s); };
-    auto kfree = [&](int s) { return bars + 8u * (6 + s); };
-    auto sfull = [&](int s) { return bars + 8u * (8 + s); };
-    const uint32_t vote = bars + 8u * 10, pfull = bars + 8u * 11, pfree = bars + 8u * 12, ofree = bars + 8u * 13;
+    auto kfull = [&](int s, int half) { return bars + 8u * (4 + 2 * s + half); };
+    auto kfree = [&](int s, int half) { return bars + 8u * (8 + 2 * s + half); };
+    auto sfull = [&](int s) { return bars + 8u * (12 + s); };
+    const uint32_t vote = bars + 8u * 14, pfull = bars + 8u * 15, pfree = bars + 8u * 16, efull = bars + 8u * 17,
+                   odone = bars + 8u * 18, ofree = bars + 8u * 19;
     const uint32_t slot = bars + 8u * kPBars;
     volatile uint32_t* slot_ptr = reinterpret_cast<volatile uint32_t*>(base_ptr + kPBarOff + 8 * kPBars);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(slot_ptr + 1);
     volatile TileInfo* info_s = reinterpret_cast<volatile TileInfo*>(base_ptr + kPInfoOff);
+    volatile int* vote_s = reinterpret_cast<volatile int*>(base_ptr + kPVoteOff);
+    volatile int* done_s = vote_s + 8;                                       // finished row, its part, its tiles
     float* const m_s = reinterpret_cast<float*>(base_ptr + kPMaxOff);        // running maxima
     float* const mu_s = m_s + 64;                                            // the same, 0 for -infinity
     float* const w_s = mu_s + 64;                                            // [4][64]
+    float* const f_s = w_s + 256;                                            // what a finished row's O is multiplied with
 
     const int warp = uniform_warp_id(), lane = threadIdx.x & 31;
     const int groups = (a.heads + G - 1) / G;
@@ -296,14 +315,18 @@ __global__ void __launch_bounds__(kPThreads<G>, 1) mla_paged_kernel(const __grid
         for (int s = 0; s < 2; ++s) {
             mbar_init(qfull(s), 1);
             mbar_init(qfree(s), 1);
-            mbar_init(kfull(s), 1);
-            mbar_init(kfree(s), 1);
+            for (int h = 0; h < 2; ++h) {
+                mbar_init(kfull(s, h), 1);
+                mbar_init(kfree(s, h), 1);
+            }
             mbar_init(sfull(s), 1);
         }
-        mbar_init(vote, kWarps);
-        mbar_init(pfull, kWarps);
+        mbar_init(vote, 4);
+        mbar_init(pfull, 4);
         mbar_init(pfree, 1);
-        mbar_init(ofree, kWarps);
+        mbar_init(efull, 4);
+        mbar_init(odone, 1);
+        mbar_init(ofree, 4);
         fence_mbar_init();
         tma_prefetch_desc(&tm_qa);
         tma_prefetch_desc(&tm_qp);
@@ -314,7 +337,7 @@ __global__ void __launch_bounds__(kPThreads<G>, 1) mla_paged_kernel(const __grid
         tmem_alloc(slot, kTmemCols);
         tmem_relinquish();
     }
-    const RangeStart start = find_range<kPThreads<G>>(a, range, reinterpret_cast<volatile int*>(w_s));
+    const RangeStart start = find_range<kPThreads>(a, range, reinterpret_cast<volatile int*>(w_s));
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -326,40 +349,47 @@ __global__ void __launch_bounds__(kPThreads<G>, 1) mla_paged_kernel(const __grid
         if (n_tiles > 0 && elect_one()) {
             bool ok = true;
             int q = 0, v = 0, q_seg = 0, v_seg = 0;            // tiles scored and accumulated, and their rows
+            int q_half = 0;                                    // halves of tile q whose scores are issued
             bool q_open = false, v_open = false;               // the current row's first tile has been taken
-            uint32_t acc = 0;
             long long t0 = 0;
-            uint32_t spins = 0;
-            // scores of the next landed tile or P V of the tile whose probabilities are written, whichever
+            uint32_t spins = 0, acc = 0;
+            // scores of the next landed half tile or P V of the tile whose probabilities are written, whichever
             // is ready first
             while (ok && v < n_tiles) {
                 bool progressed = false;
-                if (q < n_tiles && q - v < 2 && mbar_try_wait(kfull(q & 1), (q >> 1) & 1)) {
+                if (q < n_tiles && q - v < 2 && mbar_try_wait(kfull(q & 1, q_half), (q >> 1) & 1)) {
                     const int flags = info_s[q & 1].flags;
                     const int qb = kQBufs == 2 ? (q_seg & 1) : 0;
                     if (q_open || mbar_try_wait(qfull(qb), (kQBufs == 2 ? q_seg >> 1 : q_seg) & 1)) {
+                        q_open = true;
                         tc_fence_after();
-                        const uint32_t kb = base + kPKOff + (q & 1) * kPTileBytes;
-                        const uint32_t qa = base + qb * (G * kPQRow);
+                        const uint32_t kb = base + kPKOff + (q & 1) * kPTileBytes + q_half * kPHalfBytes;
+                        const uint32_t qa = base + qb * (G * kPQRow) + q_half * (4 * G * 128);
                         const uint32_t d = tmem_base + kTmemS + static_cast<uint32_t>(q & 1) * G;
 #pragma unroll
-                        for (int c = 0; c < 9; ++c) {
-                            const uint64_t adesc = c < 8 ? smem_desc_groups(kb + c * 1024, 16, 8192)
-                                                         : smem_desc_sw128(kb + kPLatBytes);
+                        for (int c = 0; c < 4; ++c) {
+                            const uint64_t adesc = smem_desc_groups(kb + c * 1024, 16, 4096);
                             const uint64_t bdesc = smem_desc_sw128(qa + c * G * 128);
 #pragma unroll
                             for (int j = 0; j < 4; ++j)
-                                mma_f16(d, adesc + 2u * j, bdesc + 2u * j, kSIdesc, (c | j) != 0 ? 1u : 0u);
+                                mma_f16(d, adesc + 2u * j, bdesc + 2u * j, kSIdesc, (q_half | c | j) != 0 ? 1u : 0u);
                         }
-                        mma_commit(sfull(q & 1));
-                        q_open = true;
-                        if (flags & 2) {
-                            mma_commit(qfree(qb));
-                            ++q_seg;
-                            q_open = false;
-                        }
-                        ++q;
                         progressed = true;
+                        if (q_half == 0) {
+                            q_half = 1;
+                        } else {
+                            const uint64_t adesc = smem_desc_sw128(kb + kPHalfBytes), bdesc = smem_desc_sw128(qa + 4 * G * 128);
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) mma_f16(d, adesc + 2u * j, bdesc + 2u * j, kSIdesc, 1u);
+                            mma_commit(sfull(q & 1));
+                            if (flags & 2) {
+                                mma_commit(qfree(qb));
+                                ++q_seg;
+                                q_open = false;
+                            }
+                            q_half = 0;
+                            ++q;
+                        }
                     }
                 }
                 if (v < q && mbar_try_wait(pfull, v & 1) &&
@@ -369,20 +399,26 @@ __global__ void __launch_bounds__(kPThreads<G>, 1) mla_paged_kernel(const __grid
                     const int flags = info_s[v & 1].flags;
                     if (!v_open) acc = 0;
                     const uint32_t kb = base + kPKOff + (v & 1) * kPTileBytes;
+                    uint32_t acc_f = acc;
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        if ((mask >> (16 * j) & 0xffffu) == 0) continue;
-                        const uint64_t bdesc = smem_desc_groups(base + kPPOff + j * 2048, 16, 1024);
+                    for (int f = 0; f < 4; ++f) {
+                        acc_f = acc;
 #pragma unroll
-                        for (int f = 0; f < 4; ++f)
-                            mma_f16(tmem_base + f * G, smem_desc_groups(kb + j * 16384 + f * 2048, 1024, 8192), bdesc,
-                                    kOIdesc, acc);
-                        acc = 1;
+                        for (int j = 0; j < 4; ++j) {
+                            if ((mask >> (16 * j) & 0xffffu) == 0) continue;
+                            const uint64_t adesc =
+                                smem_desc_groups(kb + (f >> 1) * kPHalfBytes + j * 8192 + (f & 1) * 2048, 1024, 4096);
+                            mma_f16(tmem_base + f * G, adesc, smem_desc_groups(base + kPPOff + j * 2048, 16, 1024), kOIdesc,
+                                    acc_f);
+                            acc_f = 1;
+                        }
+                        if (f & 1) mma_commit(kfree(v & 1, f >> 1));       // its dims are done with
                     }
-                    mma_commit(kfree(v & 1));
+                    acc = acc_f;
                     mma_commit(pfree);
                     v_open = true;
                     if (flags & 2) {
+                        mma_commit(odone);
                         ++v_seg;
                         v_open = false;
                     }
@@ -444,28 +480,37 @@ __global__ void __launch_bounds__(kPThreads<G>, 1) mla_paged_kernel(const __grid
                 }
             }
             const int st = g & 1;
-            if (!mbar_wait_warp(kfree(st), ((g >> 1) & 1) ^ 1u, abort_flag, 82)) break;
+            const uint32_t free_par = ((g >> 1) & 1) ^ 1u;
+            if (!mbar_wait_warp(kfree(st, 0), free_par, abort_flag, 82)) break;
             const int qb = kQBufs == 2 ? (seg & 1) : 0;
             if (first && !mbar_wait_warp(qfree(qb), ((kQBufs == 2 ? seg >> 1 : seg) & 1) ^ 1u, abort_flag, 83)) break;
+            const int row0 = (tile * kPTile) & (page - 1);
+            const uint32_t dst = base + kPKOff + st * kPTileBytes;
             if (elect_one()) {
                 if (first) {
-                    const uint32_t dst = base + qb * (G * kPQRow);
+                    const uint32_t qd = base + qb * (G * kPQRow);
                     mbar_arrive_expect_tx(qfull(qb), G * kPQRow);
-                    tma_load_4d(dst, &tm_qa, 0, hg * G, 0, b, qfull(qb));
-                    tma_load_3d(dst + G * 1024, &tm_qp, 0, hg * G, b, qfull(qb));
+                    tma_load_4d(qd, &tm_qa, 0, hg * G, 0, b, qfull(qb));
+                    tma_load_3d(qd + G * 1024, &tm_qp, 0, hg * G, b, qfull(qb));
                 }
                 info_s[st].mask = mask;
                 info_s[st].row = b;
                 info_s[st].flags = (first ? 1 : 0) | (last ? 2 : 0) | (j == 0 ? 4 : 0) | (j == t.n - 1 ? 8 : 0);
-                mbar_arrive_expect_tx(kfull(st), kPTileBytes);
-                const uint32_t dst = base + kPKOff + st * kPTileBytes;
-                const int row0 = (tile * kPTile) & (page - 1);
+                mbar_arrive_expect_tx(kfull(st, 0), kPHalfBytes);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    if (i >= boxes) break;
-                    tma_load_5d(dst + i * page * 1024, &tm_kv, 0, 0, 0, row0 >> 3, id[i], kfull(st));
-                    tma_load_3d(dst + kPLatBytes + i * page * 128, &tm_pe, 0, row0, id[i], kfull(st));
-                }
+                for (int i = 0; i < 4; ++i)
+                    if (i < boxes) tma_load_5d(dst + i * page * 512, &tm_kv, 0, 0, 0, row0 >> 3, id[i], kfull(st, 0));
+            }
+            __syncwarp();
+            if (!mbar_wait_warp(kfree(st, 1), free_par, abort_flag, 82)) break;
+            if (elect_one()) {
+                mbar_arrive_expect_tx(kfull(st, 1), kPTileBytes - kPHalfBytes);
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (i < boxes) {
+                        tma_load_5d(dst + kPHalfBytes + i * page * 512, &tm_kv, 0, 0, 4, row0 >> 3, id[i], kfull(st, 1));
+                        tma_load_3d(dst + 2 * kPHalfBytes + i * page * 128, &tm_pe, 0, row0, id[i], kfull(st, 1));
+                    }
             }
             __syncwarp();
             if (last) ++seg;
@@ -474,93 +519,92 @@ __global__ void __launch_bounds__(kPThreads<G>, 1) mla_paged_kernel(const __grid
                 j = 0;
             }
         }
-    } else if (warp >= 4) {
-        const int quad = warp & 3, half = (warp - 4) >> 2, wi = warp - 4;
-        const int tid = threadIdx.x - 128;
+    } else if (warp >= 4 && warp < 8) {
+        const int quad = warp & 3, tid = threadIdx.x - 128;
         const uint32_t lane_base = static_cast<uint32_t>(quad * 32) << 16;
-        const uint32_t h0 = half * kHT;                        // this thread's first head of the group
-        const int key = 16 * quad + (lane & 15);               // its position within the tile (lanes 0-15)
+        const int h0 = 2 * (lane & 3);                         // this thread's heads: 8 u + h0 and the next
+        const int key = 16 * quad + (lane >> 2);               // its positions within the tile: key and key + 8
         const float ninf = __int_as_float(0xff800000);
-        volatile int* vote_s = reinterpret_cast<volatile int*>(base_ptr + kPVoteOff);
-        // rows without a visible tile are nobody's: zeros, shared out over the CTAs
-        if (hg == 0)
-            for (int b = range; b < a.batch; b += a.n_ranges)
-                if (row_tiles(a, b).n == 0)
-                    for (int c = tid; c < a.heads * 64; c += 128 * kHalves)
-                        reinterpret_cast<uint4*>(a.out + static_cast<int64_t>(b) * a.heads * 512)[c] = make_uint4(0u, 0u, 0u, 0u);
         uint32_t votes = 0;                                    // phases of `vote` taken
         auto meet = [&](int code) {                            // all softmax warps have come this far
             __syncwarp();
             if (lane == 0) mbar_arrive(vote);
             return mbar_wait_warp(vote, votes++ & 1, abort_flag, code);
         };
-        float l[kHT];
-        int flags4 = 0;
+        // combines v of the thread's two positions' lanes 8 u + h0 .. over the warp's positions
+        auto over_lanes = [&](float v, auto f) {
+            v = f(v, __shfl_xor_sync(0xffffffffu, v, 4));
+            v = f(v, __shfl_xor_sync(0xffffffffu, v, 8));
+            return f(v, __shfl_xor_sync(0xffffffffu, v, 16));
+        };
+        auto larger = [](float u, float w) { return fmaxf(u, w); };
+        auto plus = [](float u, float w) { return u + w; };
+        // lane t: row t % 8 of block t / 8; blocks: positions 0-7 and 8-15 of eight heads, then of the next eight
+        const int st_key = 16 * quad + (lane & 15);
+        const uint32_t st_line = base + kPPOff + st_key * 128;
+        float l[G / 4];
+        int flags4 = 0, seg = 0, seg_first = 0;
         bool open = false;                                     // every head has a maximum
         for (int g = 0; g < n_tiles; ++g) {
             const int st = g & 1;
-            if (!mbar_wait_warp(kfull(st), (g >> 1) & 1, abort_flag, 84)) break;
+            if (!mbar_wait_warp(kfull(st, 0), (g >> 1) & 1, abort_flag, 84)) break;
             const uint64_t mask = info_s[st].mask;
             const int flags = info_s[st].flags, b = info_s[st].row;
             const bool first = flags & 1, last = flags & 2;
             flags4 = (first ? 0 : flags4) | (flags & 12);
-            const bool seen = lane < 16 && (mask >> key & 1);
+            const bool seen0 = mask >> key & 1, seen1 = mask >> (key + 8) & 1;
             if (first) {
                 open = false;
+                seg_first = g;
 #pragma unroll
-                for (int i = 0; i < kHT; ++i) l[i] = 0.f;
+                for (int i = 0; i < G / 4; ++i) l[i] = 0.f;
             }
             if (!mbar_wait_warp(sfull(st), (g >> 1) & 1, abort_flag, 85)) break;
             tc_fence_after();
-            float x[kHT];
+            float x[G / 2];                                    // [8 heads][position, position + 8][2 heads]
             // P against the maxima so far, and whether a score exceeds one of them by more than 2^8; what the
             // other warps found comes in while the exponentials are evaluated
-            auto scores = [&] {
-                uint32_t r[kHT];
-                tmem_ld_cols(tmem_base + lane_base + kTmemS + static_cast<uint32_t>(st) * G + h0, r);
-#pragma unroll
-                for (int i = 0; i < kHT; ++i) x[i] = __uint_as_float(r[i]);
-            };
-            float top = ninf;
+            auto scores = [&] { tmem_ld_16x256b(tmem_base + lane_base + kTmemS + static_cast<uint32_t>(st) * G, x); };
+            float top0 = ninf, top1 = ninf;
             auto against = [&] {
 #pragma unroll
-                for (int i = 0; i < kHT; i += 4) {
-                    const float4 mu = *reinterpret_cast<const float4*>(mu_s + h0 + i);
-                    x[i] = fmaf(x[i], a.scale_log2, -mu.x);
-                    x[i + 1] = fmaf(x[i + 1], a.scale_log2, -mu.y);
-                    x[i + 2] = fmaf(x[i + 2], a.scale_log2, -mu.z);
-                    x[i + 3] = fmaf(x[i + 3], a.scale_log2, -mu.w);
-                    top = fmaxf(top, fmaxf(fmaxf(x[i], x[i + 1]), fmaxf(x[i + 2], x[i + 3])));
+                for (int u = 0; u < G / 8; ++u) {
+                    const float2 mu = *reinterpret_cast<const float2*>(mu_s + 8 * u + h0);
+                    x[4 * u] = fmaf(x[4 * u], a.scale_log2, -mu.x);
+                    x[4 * u + 1] = fmaf(x[4 * u + 1], a.scale_log2, -mu.y);
+                    x[4 * u + 2] = fmaf(x[4 * u + 2], a.scale_log2, -mu.x);
+                    x[4 * u + 3] = fmaf(x[4 * u + 3], a.scale_log2, -mu.y);
+                    top0 = fmaxf(top0, fmaxf(x[4 * u], x[4 * u + 1]));
+                    top1 = fmaxf(top1, fmaxf(x[4 * u + 2], x[4 * u + 3]));
                 }
             };
             auto exponentials = [&] {
 #pragma unroll
-                for (int i = 0; i < kHT; ++i) x[i] = seen ? exp2_fast(x[i]) : 0.f;
+                for (int i = 0; i < G / 2; ++i) x[i] = ((i & 2) ? seen1 : seen0) ? exp2_fast(x[i]) : 0.f;
             };
             scores();
             bool over = !open;
             if (open) {
                 against();
-                over = seen && top > 8.f;
+                over = (seen0 && top0 > 8.f) || (seen1 && top1 > 8.f);
             }
             over = __any_sync(0xffffffffu, over);
             if (lane == 0) {
-                vote_s[st * 8 + wi] = over ? 1 : 0;
+                vote_s[st * 4 + quad] = over ? 1 : 0;
                 mbar_arrive(vote);
             }
             if (open) exponentials();
             if (!mbar_wait_warp(vote, votes++ & 1, abort_flag, 86)) break;
 #pragma unroll
-            for (int w = 0; w < kWarps; ++w) over |= vote_s[st * 8 + w] != 0;
+            for (int w = 0; w < 4; ++w) over |= vote_s[st * 4 + w] != 0;
             if (over) {
                 if (open) scores();
 #pragma unroll
-                for (int c = 0; c < kHT; c += 16) {
-                    float y[16];
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) y[i] = seen ? x[c + i] * a.scale_log2 : ninf;
-                    const float most = reduce16(y, [](float u, float w) { return fmaxf(u, w); });
-                    if (lane < 16) w_s[quad * 64 + h0 + c + lane] = most;
+                for (int i = 0; i < G / 4; ++i) {
+                    const float y0 = seen0 ? x[(i >> 1) * 4 + (i & 1)] * a.scale_log2 : ninf;
+                    const float y1 = seen1 ? x[(i >> 1) * 4 + 2 + (i & 1)] * a.scale_log2 : ninf;
+                    const float most = over_lanes(fmaxf(y0, y1), larger);
+                    if (lane < 4) w_s[quad * 64 + 8 * (i >> 1) + h0 + (i & 1)] = most;
                 }
                 if (!meet(89)) break;
                 if (tid < G) {
@@ -574,7 +618,7 @@ __global__ void __launch_bounds__(kPThreads<G>, 1) mla_paged_kernel(const __grid
                 }
                 if (!meet(90)) break;
 #pragma unroll
-                for (int i = 0; i < kHT; ++i) l[i] *= w_s[h0 + i];
+                for (int i = 0; i < G / 4; ++i) l[i] *= w_s[8 * (i >> 1) + h0 + (i & 1)];
                 open = true;
 #pragma unroll
                 for (int i = 0; i < G; i += 32) open &= m_s[G < 32 ? lane & (G - 1) : i + lane] != ninf;
@@ -582,27 +626,18 @@ __global__ void __launch_bounds__(kPThreads<G>, 1) mla_paged_kernel(const __grid
                 against();
                 exponentials();
             }
-            uint32_t pk[kHT / 2];
 #pragma unroll
-            for (int i = 0; i < kHT; i += 2) {
-                l[i] += x[i];
-                l[i + 1] += x[i + 1];
-                pk[i / 2] = pack_bf16x2(x[i], x[i + 1]);
-            }
-            if (half == 0) {
-                // rows of a step that is multiplied, but not visible: zeros
-                const uint32_t step = static_cast<uint32_t>(mask >> (16 * quad)) & 0xffffu;
-                if (step != 0 && step != 0xffffu) {
-                    uint8_t* kt = base_ptr + kPKOff + st * kPTileBytes + quad * 16384;
-                    for (uint32_t z = ~step & 0xffffu; z; z &= z - 1) {
-                        const int row = __ffs(static_cast<int>(z)) - 1;
+            for (int i = 0; i < G / 4; ++i) l[i] += x[(i >> 1) * 4 + (i & 1)] + x[(i >> 1) * 4 + 2 + (i & 1)];
+            // rows of a step that is multiplied, but not visible: zeros
+            const uint32_t step = static_cast<uint32_t>(mask >> (16 * quad)) & 0xffffu;
+            if (step != 0 && step != 0xffffu) {
+                uint8_t* kt = base_ptr + kPKOff + st * kPTileBytes + quad * 8192;
+                for (uint32_t z = ~step & 0xffffu; z; z &= z - 1) {
+                    const int row = __ffs(static_cast<int>(z)) - 1;
 #pragma unroll
-                        for (int i = 0; i < 2; ++i) {
-                            const int piece = lane + 32 * i;
-                            *reinterpret_cast<uint4*>(kt + (row >> 3) * 8192 + (piece >> 3) * 1024 + (row & 7) * 128 +
-                                                      (piece & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
-                        }
-                    }
+                    for (int i = 0; i < 2; ++i)
+                        *reinterpret_cast<uint4*>(kt + i * kPHalfBytes + (row >> 3) * 4096 + (lane >> 3) * 1024 +
+                                                  (row & 7) * 128 + (lane & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
                 }
             }
             if (g > 0) {
@@ -610,25 +645,25 @@ __global__ void __launch_bounds__(kPThreads<G>, 1) mla_paged_kernel(const __grid
                 if (!mbar_wait_warp(pfree, (g - 1) & 1, abort_flag, 87)) break;
                 tc_fence_after();
                 if (over && !first) {
+                    constexpr int kCols = G < 32 ? G : 32;
 #pragma unroll 1
-                    for (int f = 0; f < 4; ++f) {
-                        uint32_t o[kHT];
-                        const uint32_t at = tmem_base + lane_base + f * G + h0;
+                    for (int c = 0; c < 4 * G; c += kCols) {
+                        uint32_t o[kCols];
+                        const uint32_t at = tmem_base + lane_base + c;
                         tmem_ld_cols(at, o);
+                        const float* w = w_s + (c & (G - 1));
 #pragma unroll
-                        for (int i = 0; i < kHT; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * w_s[h0 + i]);
+                        for (int i = 0; i < kCols; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * w[i]);
                         tmem_st_cols(at, o);
                     }
                     tmem_st_wait();
                 }
             }
-            if (lane < 16) {
-                uint8_t* line = base_ptr + kPPOff + key * 128;
 #pragma unroll
-                for (int c = 0; c < kHT / 8; ++c)
-                    *reinterpret_cast<uint4*>(line + ((((h0 >> 3) + c) ^ (key & 7)) << 4)) =
-                        make_uint4(pk[4 * c], pk[4 * c + 1], pk[4 * c + 2], pk[4 * c + 3]);
-            }
+            for (int u = 0; u < G / 8; u += 2)
+                stmatrix_x4(st_line + (((u + (lane >> 4)) ^ (st_key & 7)) << 4), pack_bf16x2(x[4 * u], x[4 * u + 1]),
+                            pack_bf16x2(x[4 * u + 2], x[4 * u + 3]), pack_bf16x2(x[4 * u + 4], x[4 * u + 5]),
+                            pack_bf16x2(x[4 * u + 6], x[4 * u + 7]));
             fence_proxy_async();
             tc_fence_before();
             __syncwarp();
@@ -637,16 +672,14 @@ __global__ void __launch_bounds__(kPThreads<G>, 1) mla_paged_kernel(const __grid
                 // the sums of a head over the positions: lanes, then quarters (in order)
                 if (!meet(91)) break;                          // w_s has been read
 #pragma unroll
-                for (int c = 0; c < kHT; c += 16) {
-                    float y[16];
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) y[i] = l[c + i];
-                    const float sum = reduce16(y, [](float u, float w) { return u + w; });
-                    if (lane < 16) w_s[quad * 64 + h0 + c + lane] = sum;
+                for (int i = 0; i < G / 4; ++i) {
+                    const float sum = over_lanes(l[i], plus);
+                    if (lane < 4) w_s[quad * 64 + 8 * (i >> 1) + h0 + (i & 1)] = sum;
                 }
                 if (!meet(92)) break;
+                // the row before has been written, so its factors may go
+                if (seg > 0 && !mbar_wait_warp(ofree, (seg - 1) & 1, abort_flag, 93)) break;
                 const int part = part_slot(flags4, range);
-                const int head0 = hg * G + static_cast<int>(h0), d0 = quad * 32 + lane;
                 // one thread a head: the denominator, and what O is multiplied with (0 for a head of no weight at
                 // all, every page out of the pool or every score -infinity: it is zero)
                 if (tid < G) {
@@ -654,41 +687,56 @@ __global__ void __launch_bounds__(kPThreads<G>, 1) mla_paged_kernel(const __grid
                     if (part >= 0 && hg * G + tid < a.heads)
                         *reinterpret_cast<float2*>(a.part_ml + (static_cast<int64_t>(part) * a.heads + hg * G + tid) * 2) =
                             make_float2(den == 0.f ? ninf : m_s[tid], den);
-                    w_s[tid] = den == 0.f ? 0.f : part < 0 ? 1.f / den : 1.f;
+                    f_s[tid] = den == 0.f ? 0.f : part < 0 ? 1.f / den : 1.f;
                 }
-                if (!meet(93)) break;
-#pragma unroll
-                for (int i = 0; i < kHT; i += 4) {
-                    const float4 w = *reinterpret_cast<const float4*>(w_s + h0 + i);
-                    l[i] = w.x;
-                    l[i + 1] = w.y;
-                    l[i + 2] = w.z;
-                    l[i + 3] = w.w;
+                if (tid == 0) {
+                    done_s[0] = b;
+                    done_s[1] = part;
+                    done_s[2] = g - seg_first + 1;
                 }
-                auto scaled = [](uint32_t o, float f) { return f == 0.f ? 0.f : __uint_as_float(o) * f; };
-                if (!mbar_wait_warp(pfree, g & 1, abort_flag, 88)) break;
-                tc_fence_after();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(efull);
+                ++seg;
+            }
+        }
+    } else if (warp >= 8) {
+        // finished rows out of tensor memory, while the next row's first tile is on its way
+        const int quad = warp & 3;
+        const uint32_t lane_base = static_cast<uint32_t>(quad * 32) << 16;
+        const int d0 = quad * 32 + lane, head0 = hg * G;
+        // rows without a visible tile are nobody's: zeros, shared out over the CTAs
+        if (hg == 0)
+            for (int b = range; b < a.batch; b += a.n_ranges)
+                if (row_tiles(a, b).n == 0)
+                    for (int c = threadIdx.x - 256; c < a.heads * 64; c += 128)
+                        reinterpret_cast<uint4*>(a.out + static_cast<int64_t>(b) * a.heads * 512)[c] = make_uint4(0u, 0u, 0u, 0u);
+        constexpr int kCols = G < 32 ? G : 32;
+        for (int seg = 0, left = n_tiles; left > 0; ++seg) {
+            if (!mbar_wait_warp(efull, seg & 1, abort_flag, 94)) break;
+            const int b = done_s[0], part = done_s[1], tiles = done_s[2];
+            if (!mbar_wait_warp(odone, seg & 1, abort_flag, 88)) break;
+            tc_fence_after();
+            left -= tiles;
 #pragma unroll 1
-                for (int f = 0; f < 4; ++f) {
-                    uint32_t o[kHT];
-                    tmem_ld_cols(tmem_base + lane_base + f * G + h0, o);
-                    if (part < 0) {
-                        __nv_bfloat16* to = a.out + (static_cast<int64_t>(b) * a.heads + head0) * 512 + f * 128 + d0;
+            for (int c = 0; c < 4 * G; c += kCols) {
+                uint32_t o[kCols];
+                tmem_ld_cols(tmem_base + lane_base + c, o);
+                const int h = c & (G - 1), d = (c / G) * 128 + d0;
+                const int64_t at = (static_cast<int64_t>(part < 0 ? b : part) * a.heads + head0 + h) * 512 + d;
+                const int live = a.heads - head0 - h;
 #pragma unroll
-                        for (int i = 0; i < kHT; ++i)
-                            if (head0 + i < a.heads)
-                                to[i * 512] = __float2bfloat16_rn(scaled(o[i], l[i]));
-                    } else {
-                        float* to = a.part_o + (static_cast<int64_t>(part) * a.heads + head0) * 512 + f * 128 + d0;
-#pragma unroll
-                        for (int i = 0; i < kHT; ++i)
-                            if (head0 + i < a.heads) to[i * 512] = scaled(o[i], l[i]);
+                for (int i = 0; i < kCols; ++i) {
+                    const float f = f_s[h + i];
+                    const float v = f == 0.f ? 0.f : __uint_as_float(o[i]) * f;
+                    if (i < live) {
+                        if (part < 0) a.out[at + i * 512] = __float2bfloat16_rn(v);
+                        else a.part_o[at + i * 512] = v;
                     }
                 }
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(ofree);
             }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(ofree);
         }
     }
     tc_fence_before();
@@ -814,7 +862,7 @@ static int launch_paged(const CUtensorMap& tm_qa, const CUtensorMap& tm_qp, cons
                                      "rt_mla_paged_decode"))
         return rc;
     const int groups = (a.heads + G - 1) / G;
-    mla_paged_kernel<G><<<static_cast<unsigned>(a.n_ranges * groups), kPThreads<G>, kPSmemBytes, s>>>(tm_qa, tm_qp, tm_kv,
+    mla_paged_kernel<G><<<static_cast<unsigned>(a.n_ranges * groups), kPThreads, kPSmemBytes, s>>>(tm_qa, tm_qp, tm_kv,
                                                                                                     tm_pe, a);
     count_launch();
     return check_launch("mla_paged_kernel");
@@ -895,7 +943,7 @@ extern "C" int rt_mla_paged_decode(const void* q_abs, const void* q_pe, const vo
     {
         const uint64_t dims[] = {64, 8, 8, static_cast<uint64_t>(page_size / 8), static_cast<uint64_t>(pages)};
         const uint64_t st[] = {static_cast<uint64_t>(u * kv_row_stride), 128, static_cast<uint64_t>(8 * u * kv_row_stride), static_cast<uint64_t>(u * kv_page_stride)};
-        const uint32_t box[] = {64, 8, 8, box_rows / 8, 1};
+        const uint32_t box[] = {64, 8, 4, box_rows / 8, 1};
         if (int rc = tc::make_tmap_bf16(&tm_kv, kv, 5, dims, st, box)) return rc;
     }
     {
