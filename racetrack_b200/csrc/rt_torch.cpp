@@ -9,6 +9,7 @@
 #include <c10/cuda/CUDAStream.h>
 #include <torch/extension.h>
 
+#include <cmath>
 #include <optional>
 #include <string>
 
@@ -29,7 +30,8 @@ using OptTensor = std::optional<Tensor>;
     X(rt_index_topk) X(rt_mla_sparse_decode_splits) X(rt_mla_sparse_decode)                       \
     X(rt_page_extend_workspace_ints) X(rt_page_extend) X(rt_page_write) X(rt_page_free)           \
     X(rt_page_fork_workspace_ints) X(rt_page_fork) X(rt_page_compact_workspace_ints)              \
-    X(rt_page_compact) X(rt_page_copy) X(rt_mla_paged_decode_workspace_bytes) X(rt_mla_paged_decode)
+    X(rt_page_compact) X(rt_page_copy) X(rt_mla_paged_decode_workspace_bytes) X(rt_mla_paged_decode) \
+    X(rt_attn_causal_prefill_share) X(rt_attn_window_prefill)
 
 #define RT_POINTER(name) decltype(&::name) p_##name = nullptr;
 RT_TABLE(RT_POINTER)
@@ -800,6 +802,111 @@ Tensor mla_sparse_decode(const Tensor& q_abs, const Tensor& q_pe, const Tensor& 
     return out;
 }
 
+// ---- causal attention of a prompt ---------------------------------------------------------------
+
+// The operands of attention_prefill as the kernels take them: views whose rows are 16-byte aligned, else copies.
+struct Prefill {
+    Tensor q, k_nope, k_pe, v;
+    int64_t tokens, heads, nope, rope, v_dim, kp_ts = 0, kp_hs = 0;
+};
+
+Prefill prefill_operands(const Tensor& q, const Tensor& k_nope, const OptTensor& k_pe, const Tensor& v,
+                         std::optional<int64_t> window, int64_t sinks) {
+    const std::string who = "attention_prefill";
+    require_cuda({&q, &k_nope, &v});
+    if (window && *window < 1) fail(who + ": window must be positive");
+    if (sinks < 0 || (sinks > 0 && !window)) fail(who + ": sinks go with a window and must not be negative");
+    if (k_nope.device() != q.device() || v.device() != q.device() || (k_pe && k_pe->device() != q.device()))
+        fail(who + ": operands must be on one device");
+    Prefill p;
+    bool ok = q.dim() == 3 && k_nope.dim() == 3 && v.dim() == 3;
+    if (ok) {
+        p.tokens = q.size(0);
+        p.heads = q.size(1);
+        p.nope = k_nope.size(2);
+        p.rope = q.size(2) - p.nope;
+        p.v_dim = v.size(2);
+        ok = same_shape(k_nope, {p.tokens, p.heads, p.nope}) && same_shape(v, {p.tokens, p.heads, p.v_dim}) && p.rope >= 0;
+        if (p.rope > 0)
+            ok = ok && k_pe && (same_shape(*k_pe, {p.tokens, p.rope}) || same_shape(*k_pe, {p.tokens, p.heads, p.rope}));
+    }
+    if (!ok)
+        fail(who + ": expected q [T,H,nope+rope], k_nope [T,H,nope], k_pe [T,rope] or [T,H,rope], v [T,H,v]");
+    auto view = [&](const Tensor& t, const char* name) {
+        if (t.scalar_type() != at::kBFloat16) fail(who + ": " + name + " must be bfloat16");
+        bool fits = t.stride(-1) == 1 && aligned16(t);
+        for (int64_t d = 0; d + 1 < t.dim(); ++d) fits = fits && t.stride(d) % 8 == 0;
+        return fits ? t : t.clone(at::MemoryFormat::Contiguous);
+    };
+    p.q = view(q, "q");
+    p.k_nope = view(k_nope, "k_nope");
+    p.v = view(v, "v");
+    if (p.rope > 0) {
+        p.k_pe = view(*k_pe, "k_pe");
+        p.kp_ts = p.k_pe.stride(0);
+        p.kp_hs = p.k_pe.dim() == 3 ? p.k_pe.stride(1) : 0;     // 0: one key a token (an expanded view too)
+    }
+    return p;
+}
+
+void attend(const Prefill& p, void* out, int64_t out_ts, int64_t out_hs, void* codes, float* scales, double scale,
+            int64_t layer_heads, std::optional<int64_t> window, int64_t sinks, const char* what) {
+    const void* k_pe = p.rope > 0 ? p.k_pe.data_ptr() : nullptr;
+    const int64_t kn_ts = p.k_nope.stride(0), kn_hs = p.k_nope.stride(1), v_ts = p.v.stride(0), v_hs = p.v.stride(1);
+    if (window)
+        check(p_rt_attn_window_prefill(p.q.data_ptr(), p.k_nope.data_ptr(), k_pe, p.v.data_ptr(), out, codes, scales,
+                                       p.tokens, p.heads, layer_heads, p.nope, p.rope, p.v_dim, p.q.stride(0), p.q.stride(1),
+                                       kn_ts, kn_hs, p.kp_ts, p.kp_hs, v_ts, v_hs, out_ts, out_hs, *window, sinks,
+                                       static_cast<float>(scale), stream()),
+              what);
+    else
+        check(p_rt_attn_causal_prefill_share(p.q.data_ptr(), p.k_nope.data_ptr(), k_pe, p.v.data_ptr(), out, codes, scales,
+                                             p.tokens, p.heads, layer_heads, p.nope, p.rope, p.v_dim, p.q.stride(0),
+                                             p.q.stride(1), kn_ts, kn_hs, p.kp_ts, p.kp_hs, v_ts, v_hs, out_ts, out_hs,
+                                             static_cast<float>(scale), stream()),
+              what);
+}
+
+Tensor attention_prefill(const Tensor& q, const Tensor& k_nope, const OptTensor& k_pe, const Tensor& v,
+                         std::optional<double> scale, int64_t layer_heads, std::optional<int64_t> window, int64_t sinks) {
+    require_cuda({&q});
+    const c10::cuda::CUDAGuard guard(q.device());
+    const Prefill p = prefill_operands(q, k_nope, k_pe, v, window, sinks);
+    Tensor out = empty({p.tokens, p.heads, p.v_dim}, at::kBFloat16, p.q);
+    attend(p, out.data_ptr(), out.stride(0), out.stride(1), nullptr, nullptr,
+           scale.value_or(1.0 / std::sqrt(static_cast<double>(p.nope + p.rope))), layer_heads ? layer_heads : p.heads, window,
+           sinks, "rt_attn_causal_prefill");
+    return out;
+}
+
+std::tuple<Tensor, Tensor> attention_prefill_fp8(const Tensor& q, const Tensor& k_nope, const OptTensor& k_pe,
+                                                 const Tensor& v, std::optional<double> scale, int64_t layer_heads,
+                                                 std::optional<int64_t> window, int64_t sinks, const OptTensor& out_codes,
+                                                 const OptTensor& out_scales) {
+    require_cuda({&q});
+    require_pair("attention_prefill", out_codes, out_scales);
+    const c10::cuda::CUDAGuard guard(q.device());
+    const Prefill p = prefill_operands(q, k_nope, k_pe, v, window, sinks);
+    const int64_t cols = p.heads * p.v_dim;
+    if (out_codes && (out_codes->element_size() != 1 || out_scales->scalar_type() != at::kFloat ||
+                      !out_codes->is_contiguous() || !out_scales->is_contiguous() ||
+                      !same_shape(*out_codes, {p.tokens, cols}) || !same_shape(*out_scales, {p.tokens, cols / 128}) ||
+                      out_codes->device() != q.device() || out_scales->device() != q.device()))
+        fail("attention_prefill: out must be contiguous (1-byte codes [T, H*v], fp32 scales [T, H*v/128])");
+    // no fused epilogue for other head shapes: the quantiser runs behind the attention kernel
+    if (p.nope != 128 || p.rope != 64 || p.v_dim != 128)
+        return act_quant(attention_prefill(p.q, p.k_nope, p.rope > 0 ? OptTensor(p.k_pe) : std::nullopt, p.v, scale,
+                                           layer_heads, window, sinks)
+                             .view({p.tokens, cols}),
+                         out_codes, out_scales);
+    Tensor codes = out_codes ? *out_codes : empty({p.tokens, cols}, at::kFloat8_e4m3fn, p.q);
+    Tensor scales = out_scales ? *out_scales : empty({p.tokens, p.heads}, at::kFloat, p.q);
+    attend(p, nullptr, 8, 8, codes.data_ptr(), data<float>(scales),
+           scale.value_or(1.0 / std::sqrt(static_cast<double>(p.nope + p.rope))), layer_heads ? layer_heads : p.heads, window,
+           sinks, "rt_attn_causal_prefill_fp8");
+    return {codes, scales};
+}
+
 // ---- paged caches -----------------------------------------------------------------------------
 // These calls run on the device of their tensors, whichever is current, and on its current stream.
 
@@ -1106,6 +1213,8 @@ PYBIND11_MODULE(_rt_torch, m) {
     RT_DEF(fp8_index);
     RT_DEF(index_topk);
     RT_DEF(mla_sparse_decode);
+    RT_DEF(attention_prefill);
+    RT_DEF(attention_prefill_fp8);
     RT_DEF(mla_paged_decode);
     RT_DEF(page_extend);
     RT_DEF(page_write);

@@ -578,8 +578,10 @@ def mla_paged_decode(q_abs: torch.Tensor, q_pe: torch.Tensor, kv_pages: torch.Te
     them (append first), or with `window` to the last `window` of them and the first `sinks`. A row whose
     sequence is out of range (padding: -1) or empty is zero. Lengths stay on the device, so one captured
     graph serves a growing cache. page: a power of two, 16 or more."""
+    if window is not None:
+        window = min(int(window), 1 << 62)
     return _native().mla_paged_decode(q_abs, q_pe, kv_pages, pe_pages, block_table, seq_lens, softmax_scale, seqs,
-                                      window, sinks)
+                                      window, min(int(sinks), 1 << 62))
 
 
 def attention_prefill(q: torch.Tensor, k_nope: torch.Tensor, k_pe: Optional[torch.Tensor],
@@ -604,77 +606,13 @@ def attention_prefill(q: torch.Tensor, k_nope: torch.Tensor, k_pe: Optional[torc
     window: query i sees only the last `window` keys up to its own and the first `sinks` of all; key tiles
     without such a key are neither loaded nor multiplied. A window of T or more is the causal call. Hidden
     keys weigh nothing, NaN included; their values must be finite."""
-    _require_cuda(q, k_nope, v)
-    if window is not None and int(window) < 1:
-        raise RuntimeError("attention_prefill: window must be positive")
-    if sinks < 0 or (sinks and window is None):
-        raise RuntimeError("attention_prefill: sinks go with a window and must not be negative")
-    if any(t is not None and t.device != q.device for t in (k_nope, k_pe, v)):
-        raise RuntimeError("attention_prefill: operands must be on one device")
-    if q.device.index != torch.cuda.current_device():
-        with torch.cuda.device(q.device):
-            return attention_prefill(q, k_nope, k_pe, v, softmax_scale, quantized=quantized, out=out,
-                                     layer_heads=layer_heads, window=window, sinks=sinks)
-    tokens, heads, qk = q.shape
-    nope = k_nope.shape[-1]
-    rope = qk - nope
-    v_dim = v.shape[-1]
-    ok = k_nope.shape == (tokens, heads, nope) and v.shape == (tokens, heads, v_dim) and rope >= 0
-    if rope:
-        ok = ok and k_pe is not None and k_pe.shape in ((tokens, rope), (tokens, heads, rope))
-    if not ok:
-        raise RuntimeError("attention_prefill: expected q [T,H,nope+rope], k_nope [T,H,nope], "
-                           "k_pe [T,rope] or [T,H,rope], v [T,H,v]")
-
-    def view(t, name):
-        if t.dtype != torch.bfloat16:
-            raise RuntimeError(f"attention_prefill: {name} must be bfloat16")
-        if t.stride(-1) != 1 or any(st % 8 for st in t.stride()[:-1]) or t.data_ptr() % 16:
-            t = t.contiguous()
-        return t
-    q, k_nope, v = view(q, "q"), view(k_nope, "k_nope"), view(v, "v")
-    kp_ts = kp_hs = 0
-    if rope:
-        k_pe = view(k_pe, "k_pe")
-        kp_ts = k_pe.stride(0)
-        kp_hs = k_pe.stride(1) if k_pe.dim() == 3 else 0
-        if k_pe.dim() == 3 and kp_hs == 0:         # an expanded view: the shared form
-            k_pe = k_pe[:, 0]
-    if softmax_scale is None:
-        softmax_scale = qk ** -0.5
-    lib = _lib.load()
-    if window is None:
-        attend, masked = lib.rt_attn_causal_prefill_share, ()
-    else:
-        attend, masked = lib.rt_attn_window_prefill, (min(int(window), max(tokens, 1)), min(int(sinks), tokens))
+    if window is not None:
+        window = min(int(window), 1 << 62)
+    sinks = min(int(sinks), 1 << 62)
     if quantized:
-        if out is not None:
-            codes, scales = out
-            if (codes.element_size() != 1 or scales.dtype != torch.float32 or not codes.is_contiguous()
-                    or not scales.is_contiguous() or tuple(codes.shape) != (tokens, heads * v_dim)
-                    or tuple(scales.shape) != (tokens, heads * v_dim // 128)):
-                raise RuntimeError("attention_prefill: out must be contiguous (1-byte codes [T, H*v], fp32 scales [T, H*v/128])")
-        if (nope, rope, v_dim) != (128, 64, 128):
-            # no fused epilogue for this head shape: the quantiser runs behind the attention kernel
-            return fused_act_quant(attention_prefill(q, k_nope, k_pe, v, softmax_scale, layer_heads=layer_heads,
-                                                     window=window, sinks=sinks)
-                                   .view(tokens, heads * v_dim), out=out)
-        if out is None:
-            codes = torch.empty(tokens, heads * v_dim, dtype=torch.float8_e4m3fn, device=q.device)
-            scales = torch.empty(tokens, heads, dtype=torch.float32, device=q.device)
-        _lib.check(attend(
-            q.data_ptr(), k_nope.data_ptr(), k_pe.data_ptr(), v.data_ptr(), None, codes.data_ptr(),
-            scales.data_ptr(), tokens, heads, layer_heads or heads, nope, rope, v_dim, q.stride(0), q.stride(1),
-            k_nope.stride(0), k_nope.stride(1), kp_ts, kp_hs, v.stride(0), v.stride(1), 8, 8,
-            *masked, float(softmax_scale), _stream()), "rt_attn_causal_prefill_fp8")
-        return codes, scales
-    out = torch.empty(tokens, heads, v_dim, dtype=torch.bfloat16, device=q.device)
-    _lib.check(attend(
-        q.data_ptr(), k_nope.data_ptr(), k_pe.data_ptr() if rope else None, v.data_ptr(),
-        out.data_ptr(), None, None, tokens, heads, layer_heads or heads, nope, rope, v_dim, q.stride(0), q.stride(1),
-        k_nope.stride(0), k_nope.stride(1), kp_ts, kp_hs, v.stride(0), v.stride(1),
-        out.stride(0), out.stride(1), *masked, float(softmax_scale), _stream()), "rt_attn_causal_prefill")
-    return out
+        codes, scales = out if out is not None else (None, None)
+        return _native().attention_prefill_fp8(q, k_nope, k_pe, v, softmax_scale, layer_heads or 0, window, sinks, codes, scales)
+    return _native().attention_prefill(q, k_nope, k_pe, v, softmax_scale, layer_heads or 0, window, sinks)
 
 
 def causal_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor) -> torch.Tensor:
