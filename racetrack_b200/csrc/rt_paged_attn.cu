@@ -15,7 +15,8 @@ namespace rt {
 namespace tc {
 
 constexpr int kPTile = 64;                          // positions per tile
-constexpr uint32_t kPHalfBytes = kPTile * 512;       // half of the latent dims of a tile
+constexpr int kPHalf = kPTile / 2;                  // positions that are loaded and given back together
+constexpr uint32_t kPLatBytes = kPTile * 1024;      // latent part of a tile
 constexpr uint32_t kPTileBytes = kPTile * 1152;
 constexpr int kPMaxBatch = 65535;
 
@@ -166,11 +167,11 @@ constexpr uint32_t kPQBytes = kPMaxG * kPQRow;       // two sets of queries of u
 constexpr uint32_t kPKOff = kPQBytes;
 constexpr uint32_t kPPOff = kPKOff + 2 * kPTileBytes;        // P: [64 positions][64 heads] bf16
 constexpr uint32_t kPBarOff = kPPOff + kPTile * 128;
-constexpr int kPBars = 20;      // qfull[2] qfree[2] kfull[2][2] kfree[2][2] sfull[2] vote pfull pfree efull odone ofree
+constexpr int kPBars = 18;      // qfull[2] qfree[2] kfull[2] kfree[2][2] sfull[2] vote pfull pfree efull odone ofree
 constexpr uint32_t kPInfoOff = kPBarOff + kPBars * 8 + 16;   // (tensor memory slot, abort flag before it)
 constexpr uint32_t kPVoteOff = kPInfoOff + 2 * 16;           // [2][4] ints, then the finished row, its part and tiles
-constexpr uint32_t kPMaxOff = kPVoteOff + 12 * 4;            // m [64], m or 0 [64], per quarter [4][64], factors [64]
-constexpr uint32_t kPSmemBytes = kPMaxOff + 7 * 64 * 4 + 1024;
+constexpr uint32_t kPMaxOff = kPVoteOff + 12 * 4;            // m or 0 [64], per quarter [4][64], factors [64]
+constexpr uint32_t kPSmemBytes = kPMaxOff + 6 * 64 * 4 + 1024;
 static_assert(kPKOff % 1024 == 0 && kPPOff % 1024 == 0 && kPInfoOff % 16 == 0 && kPMaxOff % 16 == 0, "alignment");
 static_assert(kPSmemBytes <= 232448, "shared memory budget");
 
@@ -290,19 +291,18 @@ __global__ void __launch_bounds__(kPThreads, 1) mla_paged_kernel(const __grid_co
     const uint32_t bars = base + kPBarOff;
     auto qfull = [&](int s) { return bars + 8u * s; };
     auto qfree = [&](int s) { return bars + 8u * (2 + s); };
-    auto kfull = [&](int s, int half) { return bars + 8u * (4 + 2 * s + half); };
-    auto kfree = [&](int s, int half) { return bars + 8u * (8 + 2 * s + half); };
-    auto sfull = [&](int s) { return bars + 8u * (12 + s); };
-    const uint32_t vote = bars + 8u * 14, pfull = bars + 8u * 15, pfree = bars + 8u * 16, efull = bars + 8u * 17,
-                   odone = bars + 8u * 18, ofree = bars + 8u * 19;
+    auto sfull = [&](int s) { return bars + 8u * (4 + s); };
+    const uint32_t vote = bars + 8u * 6, pfull = bars + 8u * 7, pfree = bars + 8u * 8, efull = bars + 8u * 9,
+                   odone = bars + 8u * 10, ofree = bars + 8u * 11;
+    auto kfull = [&](int s) { return bars + 8u * (12 + s); };
+    auto kfree = [&](int s, int half) { return bars + 8u * (14 + 2 * s + half); };
     const uint32_t slot = bars + 8u * kPBars;
     volatile uint32_t* slot_ptr = reinterpret_cast<volatile uint32_t*>(base_ptr + kPBarOff + 8 * kPBars);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(slot_ptr + 1);
     volatile TileInfo* info_s = reinterpret_cast<volatile TileInfo*>(base_ptr + kPInfoOff);
     volatile int* vote_s = reinterpret_cast<volatile int*>(base_ptr + kPVoteOff);
     volatile int* done_s = vote_s + 8;                                       // finished row, its part, its tiles
-    float* const m_s = reinterpret_cast<float*>(base_ptr + kPMaxOff);        // running maxima
-    float* const mu_s = m_s + 64;                                            // the same, 0 for -infinity
+    float* const mu_s = reinterpret_cast<float*>(base_ptr + kPMaxOff);       // running maxima, 0 for -infinity
     float* const w_s = mu_s + 64;                                            // [4][64]
     float* const f_s = w_s + 256;                                            // what a finished row's O is multiplied with
 
@@ -315,10 +315,9 @@ __global__ void __launch_bounds__(kPThreads, 1) mla_paged_kernel(const __grid_co
         for (int s = 0; s < 2; ++s) {
             mbar_init(qfull(s), 1);
             mbar_init(qfree(s), 1);
-            for (int h = 0; h < 2; ++h) {
-                mbar_init(kfull(s, h), 1);
-                mbar_init(kfree(s, h), 1);
-            }
+            mbar_init(kfull(s), 1);
+            mbar_init(kfree(s, 0), 1);
+            mbar_init(kfree(s, 1), 1);
             mbar_init(sfull(s), 1);
         }
         mbar_init(vote, 4);
@@ -349,47 +348,39 @@ __global__ void __launch_bounds__(kPThreads, 1) mla_paged_kernel(const __grid_co
         if (n_tiles > 0 && elect_one()) {
             bool ok = true;
             int q = 0, v = 0, q_seg = 0, v_seg = 0;            // tiles scored and accumulated, and their rows
-            int q_half = 0;                                    // halves of tile q whose scores are issued
             bool q_open = false, v_open = false;               // the current row's first tile has been taken
             long long t0 = 0;
             uint32_t spins = 0, acc = 0;
-            // scores of the next landed half tile or P V of the tile whose probabilities are written, whichever
+            // scores of the next landed tile or P V of the tile whose probabilities are written, whichever
             // is ready first
             while (ok && v < n_tiles) {
                 bool progressed = false;
-                if (q < n_tiles && q - v < 2 && mbar_try_wait(kfull(q & 1, q_half), (q >> 1) & 1)) {
+                if (q < n_tiles && q - v < 2 && mbar_try_wait(kfull(q & 1), (q >> 1) & 1)) {
                     const int flags = info_s[q & 1].flags;
                     const int qb = kQBufs == 2 ? (q_seg & 1) : 0;
                     if (q_open || mbar_try_wait(qfull(qb), (kQBufs == 2 ? q_seg >> 1 : q_seg) & 1)) {
-                        q_open = true;
                         tc_fence_after();
-                        const uint32_t kb = base + kPKOff + (q & 1) * kPTileBytes + q_half * kPHalfBytes;
-                        const uint32_t qa = base + qb * (G * kPQRow) + q_half * (4 * G * 128);
+                        const uint32_t kb = base + kPKOff + (q & 1) * kPTileBytes;
+                        const uint32_t qa = base + qb * (G * kPQRow);
                         const uint32_t d = tmem_base + kTmemS + static_cast<uint32_t>(q & 1) * G;
 #pragma unroll
-                        for (int c = 0; c < 4; ++c) {
-                            const uint64_t adesc = smem_desc_groups(kb + c * 1024, 16, 4096);
+                        for (int c = 0; c < 9; ++c) {
+                            const uint64_t adesc = c < 8 ? smem_desc_groups(kb + c * 1024, 16, 8192)
+                                                         : smem_desc_sw128(kb + kPLatBytes);
                             const uint64_t bdesc = smem_desc_sw128(qa + c * G * 128);
 #pragma unroll
                             for (int j = 0; j < 4; ++j)
-                                mma_f16(d, adesc + 2u * j, bdesc + 2u * j, kSIdesc, (q_half | c | j) != 0 ? 1u : 0u);
+                                mma_f16(d, adesc + 2u * j, bdesc + 2u * j, kSIdesc, (c | j) != 0 ? 1u : 0u);
                         }
+                        mma_commit(sfull(q & 1));
+                        q_open = true;
+                        if (flags & 2) {
+                            mma_commit(qfree(qb));
+                            ++q_seg;
+                            q_open = false;
+                        }
+                        ++q;
                         progressed = true;
-                        if (q_half == 0) {
-                            q_half = 1;
-                        } else {
-                            const uint64_t adesc = smem_desc_sw128(kb + kPHalfBytes), bdesc = smem_desc_sw128(qa + 4 * G * 128);
-#pragma unroll
-                            for (int j = 0; j < 4; ++j) mma_f16(d, adesc + 2u * j, bdesc + 2u * j, kSIdesc, 1u);
-                            mma_commit(sfull(q & 1));
-                            if (flags & 2) {
-                                mma_commit(qfree(qb));
-                                ++q_seg;
-                                q_open = false;
-                            }
-                            q_half = 0;
-                            ++q;
-                        }
                     }
                 }
                 if (v < q && mbar_try_wait(pfull, v & 1) &&
@@ -399,22 +390,18 @@ __global__ void __launch_bounds__(kPThreads, 1) mla_paged_kernel(const __grid_co
                     const int flags = info_s[v & 1].flags;
                     if (!v_open) acc = 0;
                     const uint32_t kb = base + kPKOff + (v & 1) * kPTileBytes;
-                    uint32_t acc_f = acc;
 #pragma unroll
-                    for (int f = 0; f < 4; ++f) {
-                        acc_f = acc;
+                    for (int j = 0; j < 4; ++j) {
+                        if ((mask >> (16 * j) & 0xffffu) != 0) {
+                            const uint64_t bdesc = smem_desc_groups(base + kPPOff + j * 2048, 16, 1024);
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            if ((mask >> (16 * j) & 0xffffu) == 0) continue;
-                            const uint64_t adesc =
-                                smem_desc_groups(kb + (f >> 1) * kPHalfBytes + j * 8192 + (f & 1) * 2048, 1024, 4096);
-                            mma_f16(tmem_base + f * G, adesc, smem_desc_groups(base + kPPOff + j * 2048, 16, 1024), kOIdesc,
-                                    acc_f);
-                            acc_f = 1;
+                            for (int f = 0; f < 4; ++f)
+                                mma_f16(tmem_base + f * G, smem_desc_groups(kb + j * 16384 + f * 2048, 1024, 8192), bdesc,
+                                        kOIdesc, acc);
+                            acc = 1;
                         }
-                        if (f & 1) mma_commit(kfree(v & 1, f >> 1));       // its dims are done with
+                        if (j & 1) mma_commit(kfree(v & 1, j >> 1));       // its positions are done with
                     }
-                    acc = acc_f;
                     mma_commit(pfree);
                     v_open = true;
                     if (flags & 2) {
@@ -445,7 +432,7 @@ __global__ void __launch_bounds__(kPThreads, 1) mla_paged_kernel(const __grid_co
         int slot_row = start.slot, row_at = b;
         RowTiles t = n_tiles > 0 ? slot_tiles(a, slot_row) : RowTiles{};
         const int page = 1 << a.page_log;
-        const int boxes = page < kPTile ? kPTile / page : 1;   // pages of a tile
+        const int rows = min(page, kPHalf), boxes = kPTile / rows;    // rows of a box, boxes of a tile
         int32_t fetched = -1;                                   // lane: page number of entry fetched0 + lane
         int fetched0 = -1, fetched_row = -1;
         for (int g = 0; g < n_tiles; ++g) {
@@ -458,7 +445,7 @@ __global__ void __launch_bounds__(kPThreads, 1) mla_paged_kernel(const __grid_co
             const bool last = g == n_tiles - 1 || j == t.n - 1;
             const int tile = tile_of(t, j);
             const int m0 = (tile * kPTile) >> a.page_log;       // first entry of the row's table
-            if (fetched_row != b || m0 < fetched0 || m0 + boxes > fetched0 + 32) {
+            if (fetched_row != b || m0 < fetched0 || ((tile * kPTile + kPTile - rows) >> a.page_log) >= fetched0 + 32) {
                 fetched0 = m0;
                 fetched_row = b;
                 const int m = m0 + lane;
@@ -466,53 +453,55 @@ __global__ void __launch_bounds__(kPThreads, 1) mla_paged_kernel(const __grid_co
             }
             uint64_t mask = tile_mask(a, t, tile);
             const int used = (t.len + page - 1) >> a.page_log;  // entries behind the sequence's end are not read
-            const uint64_t page_bits = page < 64 ? (1ull << page) - 1 : ~0ull;
-            int id[4];
+            const uint64_t row_bits = (1ull << rows) - 1;
+            int id[4];                                          // the page of each box
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 id[i] = -1;
                 if (i < boxes) {
-                    id[i] = __shfl_sync(0xffffffffu, fetched, m0 - fetched0 + i);
-                    if (m0 + i >= used || id[i] < 0 || id[i] >= a.pages) {
+                    const int m = (tile * kPTile + i * rows) >> a.page_log;
+                    id[i] = __shfl_sync(0xffffffffu, fetched, m - fetched0);
+                    if (m >= used || id[i] < 0 || id[i] >= a.pages) {
                         id[i] = -1;
-                        mask &= ~(page_bits << (i * page & 63));
+                        mask &= ~(row_bits << (i * rows));
                     }
                 }
             }
             const int st = g & 1;
             const uint32_t free_par = ((g >> 1) & 1) ^ 1u;
-            if (!mbar_wait_warp(kfree(st, 0), free_par, abort_flag, 82)) break;
             const int qb = kQBufs == 2 ? (seg & 1) : 0;
-            if (first && !mbar_wait_warp(qfree(qb), ((kQBufs == 2 ? seg >> 1 : seg) & 1) ^ 1u, abort_flag, 83)) break;
-            const int row0 = (tile * kPTile) & (page - 1);
             const uint32_t dst = base + kPKOff + st * kPTileBytes;
-            if (elect_one()) {
-                if (first) {
-                    const uint32_t qd = base + qb * (G * kPQRow);
-                    mbar_arrive_expect_tx(qfull(qb), G * kPQRow);
-                    tma_load_4d(qd, &tm_qa, 0, hg * G, 0, b, qfull(qb));
-                    tma_load_3d(qd + G * 1024, &tm_qp, 0, hg * G, b, qfull(qb));
-                }
-                info_s[st].mask = mask;
-                info_s[st].row = b;
-                info_s[st].flags = (first ? 1 : 0) | (last ? 2 : 0) | (j == 0 ? 4 : 0) | (j == t.n - 1 ? 8 : 0);
-                mbar_arrive_expect_tx(kfull(st, 0), kPHalfBytes);
+            bool ok = true;
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (i < boxes) tma_load_5d(dst + i * page * 512, &tm_kv, 0, 0, 0, row0 >> 3, id[i], kfull(st, 0));
-            }
-            __syncwarp();
-            if (!mbar_wait_warp(kfree(st, 1), free_par, abort_flag, 82)) break;
-            if (elect_one()) {
-                mbar_arrive_expect_tx(kfull(st, 1), kPTileBytes - kPHalfBytes);
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (i < boxes) {
-                        tma_load_5d(dst + kPHalfBytes + i * page * 512, &tm_kv, 0, 0, 4, row0 >> 3, id[i], kfull(st, 1));
-                        tma_load_3d(dst + 2 * kPHalfBytes + i * page * 128, &tm_pe, 0, row0, id[i], kfull(st, 1));
+            for (int half = 0; half < 2; ++half) {
+                if (!(ok = mbar_wait_warp(kfree(st, half), free_par, abort_flag, 82))) break;
+                if (half == 0 && first &&
+                    !(ok = mbar_wait_warp(qfree(qb), ((kQBufs == 2 ? seg >> 1 : seg) & 1) ^ 1u, abort_flag, 83)))
+                    break;
+                if (elect_one()) {
+                    if (half == 0) {
+                        if (first) {
+                            const uint32_t qd = base + qb * (G * kPQRow);
+                            mbar_arrive_expect_tx(qfull(qb), G * kPQRow);
+                            tma_load_4d(qd, &tm_qa, 0, hg * G, 0, b, qfull(qb));
+                            tma_load_3d(qd + G * 1024, &tm_qp, 0, hg * G, b, qfull(qb));
+                        }
+                        info_s[st].mask = mask;
+                        info_s[st].row = b;
+                        info_s[st].flags = (first ? 1 : 0) | (last ? 2 : 0) | (j == 0 ? 4 : 0) | (j == t.n - 1 ? 8 : 0);
+                        mbar_arrive_expect_tx(kfull(st), kPTileBytes);     // both halves
                     }
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (i < boxes && i * rows / kPHalf == half) {
+                            const int row = (tile * kPTile + i * rows) & (page - 1);
+                            tma_load_5d(dst + i * rows * 1024, &tm_kv, 0, 0, 0, row >> 3, id[i], kfull(st));
+                            tma_load_3d(dst + kPLatBytes + i * rows * 128, &tm_pe, 0, row, id[i], kfull(st));
+                        }
+                }
+                __syncwarp();
             }
-            __syncwarp();
+            if (!ok) break;
             if (last) ++seg;
             if (++j == t.n) {
                 ++b;
@@ -545,9 +534,10 @@ __global__ void __launch_bounds__(kPThreads, 1) mla_paged_kernel(const __grid_co
         float l[G / 4];
         int flags4 = 0, seg = 0, seg_first = 0;
         bool open = false;                                     // every head has a maximum
+        float m_own = ninf;                                    // that of head tid
         for (int g = 0; g < n_tiles; ++g) {
             const int st = g & 1;
-            if (!mbar_wait_warp(kfull(st, 0), (g >> 1) & 1, abort_flag, 84)) break;
+            if (!mbar_wait_warp(kfull(st), (g >> 1) & 1, abort_flag, 84)) break;
             const uint64_t mask = info_s[st].mask;
             const int flags = info_s[st].flags, b = info_s[st].row;
             const bool first = flags & 1, last = flags & 2;
@@ -607,22 +597,22 @@ __global__ void __launch_bounds__(kPThreads, 1) mla_paged_kernel(const __grid_co
                     if (lane < 4) w_s[quad * 64 + 8 * (i >> 1) + h0 + (i & 1)] = most;
                 }
                 if (!meet(89)) break;
+                bool blank = false;
                 if (tid < G) {
                     const float mt = fmaxf(fmaxf(w_s[tid], w_s[64 + tid]), fmaxf(w_s[128 + tid], w_s[192 + tid]));
-                    const float old = first ? ninf : m_s[tid];
+                    const float old = first ? ninf : m_own;
                     const bool grow = mt > old + 8.f;          // false while mt is -infinity
-                    const float now = grow ? mt : old;
-                    m_s[tid] = now;
-                    mu_s[tid] = now == ninf ? 0.f : now;
-                    w_s[tid] = grow ? exp2_fast(old - now) : 1.f;
+                    m_own = grow ? mt : old;
+                    blank = m_own == ninf;
+                    mu_s[tid] = blank ? 0.f : m_own;
+                    w_s[tid] = grow ? exp2_fast(old - m_own) : 1.f;
                 }
+                blank = __any_sync(0xffffffffu, blank);
+                if (lane == 0) vote_s[st * 4 + quad] = blank ? 1 : 0;      // (the votes have been read)
                 if (!meet(90)) break;
 #pragma unroll
                 for (int i = 0; i < G / 4; ++i) l[i] *= w_s[8 * (i >> 1) + h0 + (i & 1)];
-                open = true;
-#pragma unroll
-                for (int i = 0; i < G; i += 32) open &= m_s[G < 32 ? lane & (G - 1) : i + lane] != ninf;
-                open = __all_sync(0xffffffffu, open);
+                open = (vote_s[st * 4] | vote_s[st * 4 + 1] | vote_s[st * 4 + 2] | vote_s[st * 4 + 3]) == 0;
                 against();
                 exponentials();
             }
@@ -631,13 +621,13 @@ __global__ void __launch_bounds__(kPThreads, 1) mla_paged_kernel(const __grid_co
             // rows of a step that is multiplied, but not visible: zeros
             const uint32_t step = static_cast<uint32_t>(mask >> (16 * quad)) & 0xffffu;
             if (step != 0 && step != 0xffffu) {
-                uint8_t* kt = base_ptr + kPKOff + st * kPTileBytes + quad * 8192;
+                uint8_t* kt = base_ptr + kPKOff + st * kPTileBytes + quad * 16384;
                 for (uint32_t z = ~step & 0xffffu; z; z &= z - 1) {
                     const int row = __ffs(static_cast<int>(z)) - 1;
 #pragma unroll
                     for (int i = 0; i < 2; ++i)
-                        *reinterpret_cast<uint4*>(kt + i * kPHalfBytes + (row >> 3) * 4096 + (lane >> 3) * 1024 +
-                                                  (row & 7) * 128 + (lane & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
+                        *reinterpret_cast<uint4*>(kt + (row >> 3) * 8192 + ((lane >> 3) + 4 * i) * 1024 + (row & 7) * 128 +
+                                                  (lane & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
                 }
             }
             if (g > 0) {
@@ -686,7 +676,7 @@ __global__ void __launch_bounds__(kPThreads, 1) mla_paged_kernel(const __grid_co
                     const float den = (w_s[tid] + w_s[64 + tid]) + (w_s[128 + tid] + w_s[192 + tid]);
                     if (part >= 0 && hg * G + tid < a.heads)
                         *reinterpret_cast<float2*>(a.part_ml + (static_cast<int64_t>(part) * a.heads + hg * G + tid) * 2) =
-                            make_float2(den == 0.f ? ninf : m_s[tid], den);
+                            make_float2(den == 0.f ? ninf : m_own, den);
                     f_s[tid] = den == 0.f ? 0.f : part < 0 ? 1.f / den : 1.f;
                 }
                 if (tid == 0) {
@@ -926,7 +916,7 @@ extern "C" int rt_mla_paged_decode(const void* q_abs, const void* q_pe, const vo
     // one row of dims as eight blocks of 64: {dims, heads, blocks, rows} and {dims, 8 rows, blocks, groups of
     // rows, pages}
     CUtensorMap tm_qa, tm_qp, tm_kv, tm_pe;
-    const uint32_t box_rows = static_cast<uint32_t>(page_size < tc::kPTile ? page_size : tc::kPTile);
+    const uint32_t box_rows = static_cast<uint32_t>(page_size < tc::kPHalf ? page_size : tc::kPHalf);
     const int64_t u = 2;
     {
         const uint64_t dims[] = {64, static_cast<uint64_t>(heads), 8, static_cast<uint64_t>(batch)};
@@ -943,7 +933,7 @@ extern "C" int rt_mla_paged_decode(const void* q_abs, const void* q_pe, const vo
     {
         const uint64_t dims[] = {64, 8, 8, static_cast<uint64_t>(page_size / 8), static_cast<uint64_t>(pages)};
         const uint64_t st[] = {static_cast<uint64_t>(u * kv_row_stride), 128, static_cast<uint64_t>(8 * u * kv_row_stride), static_cast<uint64_t>(u * kv_page_stride)};
-        const uint32_t box[] = {64, 8, 4, box_rows / 8, 1};
+        const uint32_t box[] = {64, 8, 8, box_rows / 8, 1};
         if (int rc = tc::make_tmap_bf16(&tm_kv, kv, 5, dims, st, box)) return rc;
     }
     {
