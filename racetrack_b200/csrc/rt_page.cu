@@ -387,47 +387,45 @@ __global__ void __launch_bounds__(kCopyThreads) page_fork_commit_kernel(const Fo
 
 // ---- compact and copy ---------------------------------------------------------------------------
 // The live pages come to lie in [0, live): the k-th lowest live page outside that range moves into the
-// k-th lowest free one inside it. moves[k] = {from, to}, remap[p] = where page p is now; head = {live,
-// number of moves}.
+// k-th lowest free one inside it. moves[k] = {from, to}; rank[p] = k for page p >= live (-1: not in
+// use); head = {live, number of moves}.
 __global__ void __launch_bounds__(kPlanThreads) page_compact_plan_kernel(const int32_t* refs, int pages, int32_t* head,
-                                                                         int2* moves, int32_t* remap) {
+                                                                         int2* moves, int32_t* rank) {
     __shared__ int warp_sums[32];
-    int live = 0;
-    for (int p0 = 0; p0 < pages; p0 += 4 * kPlanThreads) {
-        int mine = 0, sum;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int p = p0 + i * kPlanThreads + static_cast<int>(threadIdx.x);
-            if (p < pages && refs[p] > 0) ++mine;
-        }
-        block_exclusive(mine, warp_sums, sum);
-        live += sum;
+    // a warp takes consecutive pages, a lane one of 32, so ranks come from ballots and neighbours write to
+    // neighbouring places
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int share = ((pages + kPlanThreads - 1) / kPlanThreads) * 32;
+    const int p0 = min(warp * share, pages), p1 = min(p0 + share, pages);
+    auto used32 = [&](int p) { return __ballot_sync(0xffffffffu, p + lane < p1 && refs[p + lane] > 0); };
+    int mine = 0, live;
+#pragma unroll 8
+    for (int p = p0; p < p1; p += 32) mine += __popc(used32(p));
+    block_exclusive(lane == 0 ? mine : 0, warp_sums, live);
+    // live pages outside the range, free pages inside it
+    auto below = [&](int p) { return p >= live ? 0u : live - p >= 32 ? ~0u : (1u << (live - p)) - 1; };
+    auto there = [&](int p) { return p1 - p >= 32 ? ~0u : (1u << (p1 - p)) - 1; };
+    int outs = 0, ins = 0;
+#pragma unroll 8
+    for (int p = p0; p < p1; p += 32) {
+        const uint32_t used = used32(p);
+        outs += __popc(used & ~below(p));
+        ins += __popc(~used & below(p) & there(p));
     }
-    int out = 0, in = 0;             // live pages outside the range, free pages inside it
-    for (int p0 = 0; p0 < pages; p0 += 4 * kPlanThreads) {
-        const int p = p0 + 4 * static_cast<int>(threadIdx.x);
-        int outs = 0, ins = 0, sum;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            if (p + i >= pages) continue;
-            const bool used = refs[p + i] > 0;
-            remap[p + i] = p + i;
-            if (used && p + i >= live) outs |= 1 << i;
-            if (!used && p + i < live) ins |= 1 << i;
-        }
-        // a block's pages on either side of `live`: both counts in one sum (16 bits each hold 4096)
-        const int before = block_exclusive(__popc(outs) | (__popc(ins) << 16), warp_sums, sum);
-        int ko = out + (before & 0xffff), ki = in + (before >> 16);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            if (outs >> i & 1) moves[ko++].x = p + i;
-            if (ins >> i & 1) moves[ki++].y = p + i;
-        }
-        out += sum & 0xffff;
-        in += sum >> 16;
+    int out, in;
+    int ko = block_exclusive(lane == 0 ? outs : 0, warp_sums, out), ki = block_exclusive(lane == 0 ? ins : 0, warp_sums, in);
+    ko = __shfl_sync(0xffffffffu, ko, 0);
+    ki = __shfl_sync(0xffffffffu, ki, 0);
+    const uint32_t before = (1u << lane) - 1;
+#pragma unroll 4
+    for (int p = p0; p < p1; p += 32) {
+        const uint32_t used = used32(p), o = used & ~below(p), h = ~used & below(p) & there(p);
+        if (o >> lane & 1) moves[ko + __popc(o & before)].x = p + lane;
+        if (h >> lane & 1) moves[ki + __popc(h & before)].y = p + lane;
+        if (p + lane >= live && p + lane < p1) rank[p + lane] = (o >> lane & 1) ? ko + __popc(o & before) : -1;
+        ko += __popc(o);
+        ki += __popc(h);
     }
-    __syncthreads();
-    for (int k = threadIdx.x; k < out; k += kPlanThreads) remap[moves[k].x] = moves[k].y;
     if (threadIdx.x == 0) {
         head[0] = live;
         head[1] = out;
@@ -448,7 +446,7 @@ struct MoveArgs {
     int32_t* table;              // compaction only
     int64_t table_stride;
     int32_t* refs;
-    const int32_t* remap;
+    const int32_t* rank;
     int n_seqs, width, pages;
     int64_t pieces;              // of one page over all buffers
 };
@@ -459,13 +457,14 @@ __global__ void __launch_bounds__(kCopyThreads) page_move_kernel(const MoveArgs 
     if (a.moves) {
         const int64_t step = static_cast<int64_t>(gridDim.x) * kCopyThreads;
         const int64_t t0 = blockIdx.x * static_cast<int64_t>(kCopyThreads) + threadIdx.x;
+        const int live = a.head[0];
         if (n > 0)
             for (int64_t j = t0; j < static_cast<int64_t>(a.n_seqs) * a.width; j += step) {
                 int32_t* const e = a.table + (j / a.width) * a.table_stride + j % a.width;
                 const int p = *e;
-                if (p >= 0 && p < a.pages) {
-                    const int q = a.remap[p];
-                    if (q != p) *e = q;
+                if (p >= live && p < a.pages) {
+                    const int k = a.rank[p];
+                    if (k >= 0) *e = a.moves[k].y;
                 }
             }
         for (int64_t k = t0; k < n; k += step) {
@@ -696,7 +695,7 @@ extern "C" int rt_page_compact(void* const* bases, const int64_t* page_strides, 
     a.moves = reinterpret_cast<const int2*>(workspace + 4);
     a.head = workspace;
     a.table = table; a.table_stride = table_stride; a.refs = refs;
-    a.remap = workspace + 4 + 2 * pages;
+    a.rank = workspace + 4 + 2 * pages;
     a.n_seqs = static_cast<int>(n_seqs); a.width = static_cast<int>(width); a.pages = static_cast<int>(pages);
     return page_move("page_move_kernel", a, bufs, pages, stream);
 }
