@@ -1,5 +1,6 @@
 """Decode step of the synthetic DeepSeek-V3.2 layer on the B200 kernels: B sequences, one new
-token each, per-sequence caches of `cache_len` positions, DSA sparse attention.
+token each, over per-sequence caches of `cache_len` positions with DSA sparse attention (DecodeLayer), or
+over paged caches of sequences of any lengths with dense or windowed attention (PagedDecodeLayer).
 
 Counterpart of the reference's "MQA decode" branch (racetrack/models/deepseek.py:766-778,793-811):
 the latent and rope caches are appended, the query is absorbed through the key half of wkv_b,
@@ -28,6 +29,7 @@ import torch
 
 from . import indexer, ops
 from .layer import LayerShape, RealisticLayer, _draw
+from .paging import PagedCaches
 
 INDEX_HEADS = 64
 INDEX_DIM = 128
@@ -80,7 +82,64 @@ class DecodeCaches:
             self.index_scale[:, :fill] = scales.view(batch, fill)
 
 
-class DecodeLayer(RealisticLayer):
+class _AbsorbedLayer(RealisticLayer):
+    """What both decode layers share: the two absorbed projections, and the stack around an attention half."""
+
+    def _absorb(self, weights: dict) -> None:
+        s, h = self.shape, self.local_heads
+        wkv = weights["w_kv_b"].view(h, s.nope + s.v_dim, s.kv_lora)
+        # per-head operands of the two absorbed projections, K-major for the batched GEMM
+        self.w_uk_t = wkv[:, :s.nope].transpose(1, 2).contiguous()    # [h, kv_lora, nope]: q_nope -> latent
+        self.w_uv = wkv[:, s.nope:].contiguous()                       # [h, v, kv_lora]: latent -> v
+        self.softmax_scale = s.qk_dim ** -0.5
+
+    def _project_out(self, latent: torch.Tensor, out: torch.Tensor | None) -> torch.Tensor:
+        """Latent attention output [B, h, kv_lora] -> this rank's partial sum in `out` (an exchange buffer the
+        other ranks read), or the all-reduced [B, H]."""
+        s = self.shape
+        heads_out = ops.linear_bf16_batched(latent, self.w_uv).reshape(latent.shape[0], -1)     # [B, h * v]
+        if out is not None:
+            return self.w_o(heads_out, out=out)
+        return self._all_reduce(self.w_o(heads_out))
+
+    def _decode_exchange(self, batch: int):
+        """The two [B, H] partial-sum buffers of this batch size, mapped across the ranks once."""
+        from . import peer
+        key = ("decode", batch)
+        px = self._peer.get(key)
+        if px is None:
+            shape = (batch, self.shape.hidden)
+            px = peer.PeerExchange(self.comm, self.ones_h.device,
+                                   {"attn": (shape, torch.bfloat16), "ffn": (shape, torch.bfloat16)})
+            self._peer[key] = px
+        return px
+
+    def _stack(self, hidden: torch.Tensor, layers: int, attend) -> torch.Tensor:
+        """`layers` applications of the layer to hidden [B, H]; attend(normed, out) is the attention half."""
+        s = self.shape
+        normed = ops.fused_rms_norm(hidden, self.ones_h, eps=s.eps)
+        px = None
+        if self.world > 1 and self.reduce and self.peer_reduce and hidden.is_cuda:
+            # the two all-reduces of a layer (racetrack/realistic_bench.py:315-316,351) for the few
+            # rows of a decode step: every rank leaves its partial sums in a buffer its peers have
+            # mapped, and after one device barrier every rank sums all of them, adds the residual
+            # and normalises in ONE kernel (a one-shot all-reduce fused with its consumer)
+            px = self._decode_exchange(hidden.shape[0])
+        for _ in range(layers):
+            if px is not None:
+                attend(normed, px.local["attn"])
+                normed, hidden = px.reduce_residual_norm("attn", hidden, self.ones_h, eps=s.eps, all_rows=True)
+                self.ffn_partial(normed, out=px.local["ffn"])
+                normed, hidden = px.reduce_residual_norm("ffn", hidden, self.ones_h, eps=s.eps, all_rows=True)
+                continue
+            attn = attend(normed, None)
+            normed, hidden = ops.fused_residual_norm(attn, hidden, self.ones_h, eps=s.eps)
+            ffn = self.ffn_forward(normed)
+            normed, hidden = ops.fused_residual_norm(ffn, hidden, self.ones_h, eps=s.eps)
+        return hidden
+
+
+class DecodeLayer(_AbsorbedLayer):
     """One rank's shard of the layer in decode mode; `decode_stack` applies it `layers` times to
     the B new tokens at position `start_pos` (the reference reuses one layer for the whole stack,
     racetrack/realistic_bench.py:420-423, so the caches are this one layer's)."""
@@ -91,14 +150,10 @@ class DecodeLayer(RealisticLayer):
                  process_group=None):
         super().__init__(shape, weights, rank, world, ffn="moe", route=route, proj=proj,
                          process_group=process_group)
-        s, h = shape, self.local_heads
-        wkv = weights["w_kv_b"].view(h, s.nope + s.v_dim, s.kv_lora)
-        # per-head operands of the two absorbed projections, K-major for the batched GEMM
-        self.w_uk_t = wkv[:, :s.nope].transpose(1, 2).contiguous()    # [h, kv_lora, nope]: q_nope -> latent
-        self.w_uv = wkv[:, s.nope:].contiguous()                       # [h, v, kv_lora]: latent -> v
+        s = shape
+        self._absorb(weights)
         self.w_kv_b = None          # the prefill form of this projection is never used by a decode step
         self.index_weights, self.caches, self.index_topk = index_weights, caches, index_topk
-        self.softmax_scale = s.qk_dim ** -0.5
         self.freqs = rope_table(s.rope, caches.kv.shape[1], s.rope_base, weights["w_qkv_a"].device)
 
     def decode_attention(self, normed: torch.Tensor, start_pos: int,
@@ -124,44 +179,70 @@ class DecodeLayer(RealisticLayer):
                                         positions=positions)
         latent = ops.mla_sparse_decode(q_abs, q[..., s.nope:], c.kv[:, :end], c.pe[:, :end], picked,
                                        self.softmax_scale)                                 # [B, h, kv_lora]
-        heads_out = ops.linear_bf16_batched(latent, self.w_uv)                          # [B, h, v]
-        if out is not None:
-            return self.w_o(heads_out.reshape(batch, h * s.v_dim), out=out)
-        return self._all_reduce(self.w_o(heads_out.reshape(batch, h * s.v_dim)))
-
-    def _decode_exchange(self, batch: int):
-        """The two [B, H] partial-sum buffers of this batch size, mapped across the ranks once."""
-        from . import peer
-        key = ("decode", batch)
-        px = self._peer.get(key)
-        if px is None:
-            shape = (batch, self.shape.hidden)
-            px = peer.PeerExchange(self.comm, self.ones_h.device,
-                                   {"attn": (shape, torch.bfloat16), "ffn": (shape, torch.bfloat16)})
-            self._peer[key] = px
-        return px
+        return self._project_out(latent, out)
 
     def decode_stack(self, hidden: torch.Tensor, start_pos: int, layers: int) -> torch.Tensor:
         """hidden [B, H] bf16 (the new token of every sequence) -> hidden after `layers`
         applications of the layer."""
-        s = self.shape
-        normed = ops.fused_rms_norm(hidden, self.ones_h, eps=s.eps)
-        px = None
-        if self.world > 1 and self.reduce and self.peer_reduce and hidden.is_cuda:
-            # the two all-reduces of a layer (racetrack/realistic_bench.py:315-316,351) for the few
-            # rows of a decode step: every rank leaves its partial sums in a buffer its peers have
-            # mapped, and after one device barrier every rank sums all of them, adds the residual
-            # and normalises in ONE kernel (a one-shot all-reduce fused with its consumer)
-            px = self._decode_exchange(hidden.shape[0])
-        for _ in range(layers):
-            if px is not None:
-                self.decode_attention(normed, start_pos, out=px.local["attn"])
-                normed, hidden = px.reduce_residual_norm("attn", hidden, self.ones_h, eps=s.eps, all_rows=True)
-                self.ffn_partial(normed, out=px.local["ffn"])
-                normed, hidden = px.reduce_residual_norm("ffn", hidden, self.ones_h, eps=s.eps, all_rows=True)
-                continue
-            attn = self.decode_attention(normed, start_pos)
-            normed, hidden = ops.fused_residual_norm(attn, hidden, self.ones_h, eps=s.eps)
-            ffn = self.ffn_forward(normed)
-            normed, hidden = ops.fused_residual_norm(ffn, hidden, self.ones_h, eps=s.eps)
-        return hidden
+        return self._stack(hidden, layers, lambda normed, out: self.decode_attention(normed, start_pos, out))
+
+
+class PagedDecodeLayer(_AbsorbedLayer):
+    """Prefill and decode over paged caches (paging.PagedCaches): sequences of any lengths, each token
+    attending to every position of its sequence or, with window / sinks, to the last `window` and the first
+    `sinks` of them. The decode branch of racetrack/models/deepseek.py:766-778,793-811 without the indexer, one
+    sequence a row; as in the synthetic stack one layer is applied `layers` times, so the caches are this one
+    layer's. Lists of sequences are int32 on the device, -1 is padding; nothing is read back, so a step, growth
+    of the caches included, can be captured in a CUDA graph (`caches.check()` afterwards tells of
+    sequences that found no page)."""
+
+    def __init__(self, shape: LayerShape, weights: dict, rank: int = 0, world: int = 1, *, caches: PagedCaches,
+                 route: str = "topk_softmax", proj: str = "bf16", process_group=None, window: int | None = None,
+                 sinks: int = 0):
+        super().__init__(shape, weights, rank, world, ffn="moe", route=route, proj=proj, process_group=process_group,
+                         window=window, sinks=sinks)
+        self._absorb(weights)
+        self.caches = caches
+        self._slots = None              # where the rows of the prompt under way go
+
+    def cache_rows(self, kv_c: torch.Tensor, k_pe: torch.Tensor) -> None:
+        if self._slots is not None:
+            ops.page_write((self.caches.kv, self.caches.pe), (kv_c, k_pe), self._slots)
+
+    def prefill(self, hidden: torch.Tensor, seq: torch.Tensor, layers: int) -> torch.Tensor:
+        """hidden [T, H] bf16, the prompt of the empty sequence seq (int32 [1]) -> hidden after `layers`
+        applications of the layer; the prompt's rows are left in the caches."""
+        tokens = hidden.shape[0]
+        offsets = torch.arange(2, device=hidden.device, dtype=torch.int32) * tokens
+        self._slots = self.caches.extend(tokens, seq, offsets=offsets)
+        try:
+            return self.forward_stack(hidden, torch.arange(tokens, device=hidden.device, dtype=torch.int64), layers)
+        finally:
+            self._slots = None
+
+    def decode_attention(self, normed: torch.Tensor, seqs: torch.Tensor, slots: torch.Tensor,
+                         positions: torch.Tensor, out: torch.Tensor | None = None) -> torch.Tensor:
+        """The attention half of a step: row b is the newest token of sequence seqs[b], at positions[b] (int64),
+        its cache row slots[b] (caches.extend)."""
+        s, h, c = self.shape, self.local_heads, self.caches
+        batch = normed.shape[0]
+        qkv = self.w_qkv_a(normed)
+        q_c, kv_c, k_pe = ops.fused_norm_rope(
+            qkv[:, :s.q_lora], self.q_norm, qkv[:, s.q_lora:s.q_lora + s.kv_lora], self.kv_norm,
+            qkv[:, s.q_lora + s.kv_lora:], positions, eps=s.eps, rope_base=s.rope_base)
+        ops.page_write((c.kv, c.pe), (kv_c, k_pe), slots)
+        q = self.w_q_b(q_c).view(batch, h, s.qk_dim)
+        ops.fused_rope_half(q[..., s.nope:], positions, rope_base=s.rope_base, inplace=True)
+        q_abs = ops.linear_bf16_batched(q[..., :s.nope], self.w_uk_t)                    # [B, h, kv_lora]
+        latent = ops.mla_paged_decode(q_abs, q[..., s.nope:], c.kv, c.pe, c.block_table, c.seq_lens, self.softmax_scale,
+                                      seqs=seqs, window=self.window, sinks=self.sinks)
+        return self._project_out(latent, out)
+
+    def decode_stack(self, hidden: torch.Tensor, seqs: torch.Tensor, layers: int) -> torch.Tensor:
+        """hidden [B, H] bf16, the new token of every sequence of the list -> hidden after `layers`
+        applications of the layer; the caches grow by one position a sequence."""
+        c = self.caches
+        slots = c.extend(hidden.shape[0], seqs)
+        lengths = c.seq_lens.index_select(0, seqs.clamp(min=0, max=c.seq_lens.shape[0] - 1))
+        positions = (lengths.long() - 1).clamp_(min=0)
+        return self._stack(hidden, layers, lambda normed, out: self.decode_attention(normed, seqs, slots, positions, out))

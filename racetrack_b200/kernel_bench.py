@@ -142,6 +142,19 @@ def cases(tokens: int) -> dict[str, tuple[Callable[[], object], int]]:
         out[f"mla_sparse_decode[{B} seq x {heads} heads]"] = (
             (lambda qa=qa, qp=qp: ops.mla_sparse_decode(qa, qp, kv, pe, sel, 192 ** -0.5)),
             B * 2048 * (KV_LORA + ROPE) * 2 + B * heads * (2 * KV_LORA + ROPE) * 2)
+    # the dense form over pages of 64: the same sequences, every position of 4096; and a prompt's rows
+    # appended to a sequence (rows in, rows out)
+    pages, page_pe = kv.view(-1, 64, KV_LORA), pe.view(-1, 64, ROPE)
+    i32 = dict(device="cuda", dtype=torch.int32)
+    block, lens = torch.randperm(B * 64, device="cuda").int().view(B, 64), torch.full((B,), 4096, **i32)
+    for heads in (16, 128):
+        qa, qp = _randn(B, heads, KV_LORA) * 0.3, _randn(B, heads, ROPE) * 0.3
+        out[f"mla_paged_decode[{B} seq x 4096 x {heads} heads]"] = (
+            (lambda qa=qa, qp=qp: ops.mla_paged_decode(qa, qp, pages, page_pe, block, lens, 192 ** -0.5)),
+            B * 4096 * (KV_LORA + ROPE) * 2 + B * heads * (2 * KV_LORA + ROPE) * 2)
+    new = (_randn(T, KV_LORA), _randn(T, ROPE))
+    slots = torch.randperm(B * 4096, device="cuda")[:T].int() if T <= B * 4096 else torch.zeros(T, **i32)
+    out["page_write"] = (lambda: ops.page_write((pages, page_pe), new, slots), 2 * T * (KV_LORA + ROPE) * 2)
     return out
 
 
@@ -184,6 +197,12 @@ def gemm_cases(tokens: int) -> dict[str, tuple[Callable[[], object], int, int, s
         out[f"attention_prefill[{T} tokens x {heads} heads]"] = (
             (lambda q=q, kv=kv, kpe=kpe: ops.attention_prefill(q, kv[..., :128], kpe, kv[..., 128:])),
             flops, nbytes, "bf16")
+
+        if T > 1024:
+            seen = 1024 * T - 1024 * 1023 // 2
+            out[f"attention_prefill/window 1024[{T} tokens x {heads} heads]"] = (
+                (lambda q=q, kv=kv, kpe=kpe: ops.attention_prefill(q, kv[..., :128], kpe, kv[..., 128:], window=1024)),
+                2 * heads * seen * (192 + 128), nbytes, "bf16")
 
         def single(q=q, kv=kv, kpe=kpe):      # the single-CTA schedule whatever the length
             prev = ops.attention_prefill_schedule(1)

@@ -223,11 +223,16 @@ class Projection:
 
 class RealisticLayer:
     """One rank's shard of the synthetic layer; `forward_stack` applies it `layers` times.
-    proj = "bf16" | "fp8" | "mixed" selects the arithmetic of the dense projections."""
+    proj = "bf16" | "fp8" | "mixed" selects the arithmetic of the dense projections. window: attention to the
+    last `window` tokens up to a query's own and the first `sinks` of all instead of all of them."""
 
     def __init__(self, shape: LayerShape, weights: dict, rank: int = 0, world: int = 1, *,
                  ffn: str = "moe", route: str = "topk_softmax", proj: str = "bf16",
-                 process_group=None, token_sharded: bool = True, peer_reduce: bool = True):
+                 process_group=None, token_sharded: bool = True, peer_reduce: bool = True,
+                 window: Optional[int] = None, sinks: int = 0):
+        if window is not None and ATTENTION_CORE != "rt":
+            raise RuntimeError("RealisticLayer: a window needs this library's attention kernel")
+        self.window, self.sinks = window, sinks
         self.shape, self.rank, self.world, self.ffn, self.route = shape, rank, world, ffn, route
         self.group, self.proj = process_group, proj
         self.token_sharded = token_sharded
@@ -314,20 +319,26 @@ class RealisticLayer:
         q_c, kv_c, k_pe = ops.fused_norm_rope(
             qkv[:, :s.q_lora], self.q_norm, qkv[:, s.q_lora:s.q_lora + s.kv_lora], self.kv_norm,
             qkv[:, s.q_lora + s.kv_lora:], positions, eps=s.eps, rope_base=s.rope_base)
+        self.cache_rows(kv_c, k_pe)
         q = self.w_q_b(q_c).view(tokens, h, s.qk_dim)
         ops.fused_rope_half(q[..., s.nope:], positions, rope_base=s.rope_base, inplace=True)
         if self.attn_core == "rt":
             kv = self.w_kv_b(kv_c).view(tokens, h, s.nope + s.v_dim)
             if quantized:
                 return ops.attention_prefill(q, kv[..., :s.nope], k_pe, kv[..., s.nope:], quantized=True, out=out,
-                                             layer_heads=s.heads)
-            local = ops.attention_prefill(q, kv[..., :s.nope], k_pe, kv[..., s.nope:], layer_heads=s.heads)
+                                             layer_heads=s.heads, window=self.window, sinks=self.sinks)
+            local = ops.attention_prefill(q, kv[..., :s.nope], k_pe, kv[..., s.nope:], layer_heads=s.heads,
+                                          window=self.window, sinks=self.sinks)
         else:
             kv = self.w_kv_b(kv_c).view(tokens, h, s.qk_dim + s.v_dim)
             ops.head_broadcast_(kv[..., s.nope:s.qk_dim], k_pe)       # K = [k_nope | k_pe] in place
             local = attention_core(q, kv[..., :s.qk_dim], kv[..., s.qk_dim:])
         local = local.reshape(tokens, h * s.v_dim)
         return ops.fused_act_quant(local, out=out) if quantized else local
+
+    def cache_rows(self, kv_c: torch.Tensor, k_pe: torch.Tensor) -> None:
+        """The latent rows [T, kv_lora] and rope keys [T, rope] of a prompt as they are computed: kept by layers
+        that decode from them (decode.PagedDecodeLayer)."""
 
     def attention_rows_from_heads(self, px, heads_out: Optional[torch.Tensor], lo: int, hi: int) -> torch.Tensor:
         """The output projection of this rank's token rows [lo, hi) over ALL heads: the heads'
