@@ -197,6 +197,17 @@ __device__ __forceinline__ void tma_load_5d(uint32_t dst, const CUtensorMap* m, 
         : "memory");
 }
 
+// The box of a load into L2.
+__device__ __forceinline__ void tma_prefetch_5d(const CUtensorMap* m, int c0, int c1, int c2, int c3, int c4) {
+    asm volatile("cp.async.bulk.prefetch.tensor.5d.L2.global [%0, {%1, %2, %3, %4, %5}];" ::"l"(m), "r"(c0), "r"(c1), "r"(c2),
+                 "r"(c3), "r"(c4)
+                 : "memory");
+}
+__device__ __forceinline__ void tma_prefetch_3d(const CUtensorMap* m, int c0, int c1, int c2) {
+    asm volatile("cp.async.bulk.prefetch.tensor.3d.L2.global [%0, {%1, %2, %3}];" ::"l"(m), "r"(c0), "r"(c1), "r"(c2)
+                 : "memory");
+}
+
 __device__ __forceinline__ float exp2_fast(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -270,6 +281,61 @@ __device__ __forceinline__ void stmatrix_x4(uint32_t addr, uint32_t r0, uint32_t
 __device__ __forceinline__ int part_slot(int flags, int range) {
     return (flags & 12) == 12 ? -1 : 2 * range + ((flags & 4) ? 1 : 0);
 }
+
+// Where the tile walk of a range stands.
+struct TileWalk {
+    int b, j, slot, row_at;                          // row, tile within it, its slot, the row that `t` is of
+    RowTiles t;
+    int32_t fetched = -1;                            // lane: page number of entry fetched0 + lane of row fetched_row
+    int fetched0 = -1, fetched_row = -1;
+    int tile, flags, id[4];                          // of this step: tile, TileInfo flags, the page of each box
+    uint64_t mask;
+
+    __device__ __forceinline__ TileWalk(const PagedArgs& a, const RangeStart& start)
+        : b(start.row), j(start.tile), slot(start.slot), row_at(start.row),
+          t(start.count > 0 ? slot_tiles(a, start.slot) : RowTiles{}) {}
+
+    // The range's tile g (whole warp: the lanes fetch page numbers). rows: positions of a box.
+    __device__ __forceinline__ void step(const PagedArgs& a, int g, int n_tiles, int rows) {
+        const int lane = threadIdx.x & 31, page = 1 << a.page_log, boxes = kPTile / rows;
+        if (row_at != b) {
+            t = slot_tiles(a, slot = row_slot(a, b));
+            while (t.n == 0) t = slot_tiles(a, slot = row_slot(a, ++b));     // rows without a tile
+            row_at = b;
+        }
+        flags = (g == 0 || j == 0 ? 1 : 0) | (g == n_tiles - 1 || j == t.n - 1 ? 2 : 0) | (j == 0 ? 4 : 0) |
+                (j == t.n - 1 ? 8 : 0);
+        tile = tile_of(t, j);
+        const int m0 = (tile * kPTile) >> a.page_log, m1 = (tile * kPTile + kPTile - rows) >> a.page_log;
+        if (fetched_row != b || m0 < fetched0 || m1 >= fetched0 + 32) {
+            fetched0 = m0;
+            fetched_row = b;
+            const int m = m0 + lane;
+            fetched = m < a.width ? __ldg(a.table + slot * a.table_stride + m) : -1;
+        }
+        mask = tile_mask(a, t, tile);
+        const int used = (t.len + page - 1) >> a.page_log;      // entries behind the sequence's end are not read
+        const uint64_t row_bits = rows < 64 ? (1ull << rows) - 1 : ~0ull;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            id[i] = -1;
+            if (i < boxes) {
+                const int m = (tile * kPTile + i * rows) >> a.page_log;
+                id[i] = __shfl_sync(0xffffffffu, fetched, m - fetched0);
+                if (m >= used || id[i] < 0 || id[i] >= a.pages) {
+                    id[i] = -1;
+                    mask &= ~(row_bits << (i * rows));
+                }
+            }
+        }
+    }
+    __device__ __forceinline__ void advance() {
+        if (++j == t.n) {
+            ++b;
+            j = 0;
+        }
+    }
+};
 
 constexpr int kPThreads = 384;      // warps: 0 MMA, 1 producer, 4-7 softmax, 8-11 finished rows
 
@@ -427,85 +493,61 @@ __global__ void __launch_bounds__(kPThreads, 1) mla_paged_kernel(const __grid_co
         }
         __syncwarp();
     } else if (warp == 1) {
-        // the whole warp walks the range (lanes fetch page numbers), one thread issues the loads
-        int b = start.row, j = start.tile, seg = 0;
-        int slot_row = start.slot, row_at = b;
-        RowTiles t = n_tiles > 0 ? slot_tiles(a, slot_row) : RowTiles{};
-        const int page = 1 << a.page_log;
-        const int rows = min(page, kPHalf), boxes = kPTile / rows;    // rows of a box, boxes of a tile
-        int32_t fetched = -1;                                   // lane: page number of entry fetched0 + lane
-        int fetched0 = -1, fetched_row = -1;
+        // the whole warp walks the range, one thread issues the loads
+        TileWalk w(a, start);
+        const int page = 1 << a.page_log, rows = min(page, kPHalf), boxes = kPTile / rows;    // rows of a box, boxes of a tile
+        int seg = 0;
+        if (n_tiles > 0) w.step(a, 0, n_tiles, rows);
         for (int g = 0; g < n_tiles; ++g) {
-            if (row_at != b) {
-                t = slot_tiles(a, slot_row = row_slot(a, b));
-                while (t.n == 0) t = slot_tiles(a, slot_row = row_slot(a, ++b));     // rows without a tile
-                row_at = b;
-            }
-            const bool first = g == 0 || j == 0;
-            const bool last = g == n_tiles - 1 || j == t.n - 1;
-            const int tile = tile_of(t, j);
-            const int m0 = (tile * kPTile) >> a.page_log;       // first entry of the row's table
-            if (fetched_row != b || m0 < fetched0 || ((tile * kPTile + kPTile - rows) >> a.page_log) >= fetched0 + 32) {
-                fetched0 = m0;
-                fetched_row = b;
-                const int m = m0 + lane;
-                fetched = m < a.width ? __ldg(a.table + slot_row * a.table_stride + m) : -1;
-            }
-            uint64_t mask = tile_mask(a, t, tile);
-            const int used = (t.len + page - 1) >> a.page_log;  // entries behind the sequence's end are not read
-            const uint64_t row_bits = (1ull << rows) - 1;
-            int id[4];                                          // the page of each box
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                id[i] = -1;
-                if (i < boxes) {
-                    const int m = (tile * kPTile + i * rows) >> a.page_log;
-                    id[i] = __shfl_sync(0xffffffffu, fetched, m - fetched0);
-                    if (m >= used || id[i] < 0 || id[i] >= a.pages) {
-                        id[i] = -1;
-                        mask &= ~(row_bits << (i * rows));
-                    }
-                }
-            }
-            const int st = g & 1;
+            const int st = g & 1, qb = kQBufs == 2 ? (seg & 1) : 0;
             const uint32_t free_par = ((g >> 1) & 1) ^ 1u;
-            const int qb = kQBufs == 2 ? (seg & 1) : 0;
             const uint32_t dst = base + kPKOff + st * kPTileBytes;
             bool ok = true;
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
                 if (!(ok = mbar_wait_warp(kfree(st, half), free_par, abort_flag, 82))) break;
-                if (half == 0 && first &&
+                if (half == 0 && (w.flags & 1) &&
                     !(ok = mbar_wait_warp(qfree(qb), ((kQBufs == 2 ? seg >> 1 : seg) & 1) ^ 1u, abort_flag, 83)))
                     break;
                 if (elect_one()) {
                     if (half == 0) {
-                        if (first) {
+                        if (w.flags & 1) {
                             const uint32_t qd = base + qb * (G * kPQRow);
                             mbar_arrive_expect_tx(qfull(qb), G * kPQRow);
-                            tma_load_4d(qd, &tm_qa, 0, hg * G, 0, b, qfull(qb));
-                            tma_load_3d(qd + G * 1024, &tm_qp, 0, hg * G, b, qfull(qb));
+                            tma_load_4d(qd, &tm_qa, 0, hg * G, 0, w.b, qfull(qb));
+                            tma_load_3d(qd + G * 1024, &tm_qp, 0, hg * G, w.b, qfull(qb));
                         }
-                        info_s[st].mask = mask;
-                        info_s[st].row = b;
-                        info_s[st].flags = (first ? 1 : 0) | (last ? 2 : 0) | (j == 0 ? 4 : 0) | (j == t.n - 1 ? 8 : 0);
+                        info_s[st].mask = w.mask;
+                        info_s[st].row = w.b;
+                        info_s[st].flags = w.flags;
                         mbar_arrive_expect_tx(kfull(st), kPTileBytes);     // both halves
                     }
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
                         if (i < boxes && i * rows / kPHalf == half) {
-                            const int row = (tile * kPTile + i * rows) & (page - 1);
-                            tma_load_5d(dst + i * rows * 1024, &tm_kv, 0, 0, 0, row >> 3, id[i], kfull(st));
-                            tma_load_3d(dst + kPLatBytes + i * rows * 128, &tm_pe, 0, row, id[i], kfull(st));
+                            const int row = (w.tile * kPTile + i * rows) & (page - 1);
+                            tma_load_5d(dst + i * rows * 1024, &tm_kv, 0, 0, 0, row >> 3, w.id[i], kfull(st));
+                            tma_load_3d(dst + kPLatBytes + i * rows * 128, &tm_pe, 0, row, w.id[i], kfull(st));
                         }
                 }
                 __syncwarp();
             }
             if (!ok) break;
-            if (last) ++seg;
-            if (++j == t.n) {
-                ++b;
-                j = 0;
+            if (w.flags & 2) ++seg;
+            w.advance();
+            if (g + 1 < n_tiles) {
+                // the next tile, whose place in shared memory is still taken, on its way into L2
+                w.step(a, g + 1, n_tiles, rows);
+                if (elect_one()) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (i < boxes && w.id[i] >= 0) {
+                            const int row = (w.tile * kPTile + i * rows) & (page - 1);
+                            tma_prefetch_5d(&tm_kv, 0, 0, 0, row >> 3, w.id[i]);
+                            tma_prefetch_3d(&tm_pe, 0, row, w.id[i]);
+                        }
+                }
+                __syncwarp();
             }
         }
     } else if (warp >= 4 && warp < 8) {
