@@ -703,6 +703,13 @@ int rt_page_write(void* const* bases, const int64_t* page_strides, const int64_t
                   const void* const* rows, const int64_t* row_strides, int64_t n_buffers,
                   const int32_t* slots, int64_t tokens, int64_t pages, int64_t page_size, void* stream);
 
+/* rt_page_extend and rt_page_write of the new rows, in one launch where the tokens are few. */
+int rt_page_append(void* const* bases, const int64_t* page_strides, const int64_t* row_bytes,
+                   const void* const* rows, const int64_t* row_strides, int64_t n_buffers, int32_t* table,
+                   int64_t table_stride, int32_t* lens, int32_t* refs, int32_t* status, const int32_t* seqs,
+                   const int32_t* offsets, int32_t* slots, int32_t* workspace, int64_t n_seqs, int64_t width,
+                   int64_t pages, int64_t page_size, int64_t n, int64_t tokens, void* stream);
+
 /* The sequences of the list give their pages back and are empty (a second mention does nothing). */
 int rt_page_free(int32_t* table, int64_t table_stride, int32_t* lens, int32_t* refs, const int32_t* seqs,
                  int64_t n_seqs, int64_t width, int64_t pages, int64_t n, void* stream);

@@ -77,6 +77,7 @@ SIGNATURES: dict[str, tuple] = {
     "rt_page_extend_workspace_ints": (_L, [_L, _L]),
     "rt_page_extend": (_I, [_P, _L] + [_P] * 7 + [_L] * 6 + [_P]),
     "rt_page_write": (_I, [_P] * 5 + [_L, _P, _L, _L, _L, _P]),
+    "rt_page_append": (_I, [_P] * 5 + [_L, _P, _L] + [_P] * 7 + [_L] * 6 + [_P]),
     "rt_page_free": (_I, [_P, _L, _P, _P, _P, _L, _L, _L, _L, _P]),
     "rt_page_fork_workspace_ints": (_L, [_L, _L]),
     "rt_page_fork": (_I, [_P] * 3 + [_L, _P, _L] + [_P] * 6 + [_L] * 5 + [_P]),

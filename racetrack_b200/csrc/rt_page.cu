@@ -46,6 +46,14 @@ struct Rows {
 using AllBuffers = Buffers<RT_PAGE_MAX_BUFFERS>;
 using AllRows = Rows<RT_PAGE_MAX_BUFFERS>;
 
+static Rows<kFewBuffers> few(const AllRows& all) {
+    Rows<kFewBuffers> f;
+    for (int i = 0; i < kFewBuffers; ++i) {
+        f.base[i] = all.base[i];
+        f.stride[i] = all.stride[i];
+    }
+    return f;
+}
 static Buffers<kFewBuffers> few(const AllBuffers& all) {
     Buffers<kFewBuffers> f;
     f.n = all.n;
@@ -131,7 +139,24 @@ __device__ __forceinline__ void extend_entry(const ExtendArgs& a, int i, int& s,
     count = (a.offsets ? min(max(a.offsets[i + 1], first), a.tokens) : i + 1) - first;
 }
 
-__global__ void __launch_bounds__(kPlanThreads) page_extend_kernel(const ExtendArgs a) {
+// Row t of buffer k's rows into slot `slot`, by one warp.
+template <int CAP>
+__device__ __forceinline__ void write_row(const Buffers<CAP>& bufs, const Rows<CAP>& rows, int k, int64_t t, int slot,
+                                          int page) {
+    const int lane = threadIdx.x & 31;
+    const Buffer& b = bufs.b[k];
+    const uint8_t* src = rows.base[k] + t * rows.stride[k];
+    uint8_t* dst = b.base + (slot / page) * b.page_stride + (slot % page) * b.row_bytes;
+    if (b.row_bytes % 16 == 0 && rows.stride[k] % 16 == 0 && (reinterpret_cast<uintptr_t>(src) & 15) == 0) {
+        for (int64_t o = lane * 16; o < b.row_bytes; o += 512)
+            *reinterpret_cast<uint4*>(dst + o) = ld_once16(src + o);
+    } else {
+        for (int64_t o = lane * 4; o < b.row_bytes; o += 128)
+            *reinterpret_cast<uint32_t*>(dst + o) = *reinterpret_cast<const uint32_t*>(src + o);
+    }
+}
+
+__device__ void extend(const ExtendArgs& a) {
     extern __shared__ int32_t owner[];       // [n_seqs]: the first entry that names the sequence
     __shared__ int warp_sums[32];
     int32_t* const cum = a.work;
@@ -217,29 +242,35 @@ __global__ void __launch_bounds__(kPlanThreads) page_extend_kernel(const ExtendA
     if (lacking) atomicAdd(a.status + 1, lacking);
 }
 
+__global__ void __launch_bounds__(kPlanThreads) page_extend_kernel(const ExtendArgs a) { extend(a); }
+
+// The same, and the rows of a decode step behind it: for few tokens a launch costs more than the blocks that it
+// brings save (rows of 1152 bytes, calls in a row: 16 tokens 10.5 us in two launches, 7.4 in one; 64 10.9 and 10.2;
+// 128 12.1 and 15.6).
+constexpr int kAppendTokens = 64;
+constexpr int64_t kAppendBytes = 80 << 10;
+__global__ void __launch_bounds__(kPlanThreads) page_append_kernel(const ExtendArgs a,
+                                                                   const __grid_constant__ Buffers<kFewBuffers> bufs,
+                                                                   const __grid_constant__ Rows<kFewBuffers> rows) {
+    extend(a);
+    __syncthreads();
+    for (int w = threadIdx.x >> 5; w < a.tokens * bufs.n; w += kPlanThreads / 32) {
+        const int t = w / bufs.n, slot = a.slots[t];
+        if (slot >= 0) write_row(bufs, rows, w - t * bufs.n, t, slot, a.page);
+    }
+}
+
 // rows[b][t] -> row slots[t] of buffer b: one warp a row and buffer.
 template <int CAP>
 __global__ void __launch_bounds__(kCopyThreads) page_write_kernel(const __grid_constant__ Buffers<CAP> bufs,
                                                                   const __grid_constant__ Rows<CAP> rows,
                                                                   const int32_t* __restrict__ slots, int64_t tokens,
                                                                   int64_t pages, int page) {
-    const int lane = threadIdx.x & 31;
     const int64_t warps = static_cast<int64_t>(gridDim.x) * (kCopyThreads / 32);
     for (int64_t w = blockIdx.x * static_cast<int64_t>(kCopyThreads / 32) + (threadIdx.x >> 5); w < tokens * bufs.n; w += warps) {
         const int64_t t = w / bufs.n;
-        const int k = static_cast<int>(w - t * bufs.n);
         const int slot = __ldg(slots + t);
-        if (slot < 0 || slot >= pages * page) continue;
-        const Buffer& b = bufs.b[k];
-        const uint8_t* src = rows.base[k] + t * rows.stride[k];
-        uint8_t* dst = b.base + (slot / page) * b.page_stride + (slot % page) * b.row_bytes;
-        if (b.row_bytes % 16 == 0 && rows.stride[k] % 16 == 0 && (reinterpret_cast<uintptr_t>(src) & 15) == 0) {
-            for (int64_t o = lane * 16; o < b.row_bytes; o += 512)
-                *reinterpret_cast<uint4*>(dst + o) = ld_once16(src + o);
-        } else {
-            for (int64_t o = lane * 4; o < b.row_bytes; o += 128)
-                *reinterpret_cast<uint32_t*>(dst + o) = *reinterpret_cast<const uint32_t*>(src + o);
-        }
+        if (slot >= 0 && slot < pages * page) write_row(bufs, rows, static_cast<int>(w - t * bufs.n), t, slot, page);
     }
 }
 
@@ -261,7 +292,7 @@ __global__ void __launch_bounds__(kCopyThreads) page_free_kernel(int32_t* table,
 // ---- fork -------------------------------------------------------------------------------------
 // dst[i] becomes a second holder of src[i]'s full pages and gets a copy of the used rows of its
 // partial last page. All entries take effect at once (a sequence may be source of some and
-// destination of one, as when the beams of a search change places), in three launches: the plan,
+// destination of one, as when the beams of a search change places), in three steps: the plan,
 // which hands out the pages of the partial copies; the new rows of the table, staged, with the
 // references they add and the copies; then the old rows' references go and the new rows come. Pages
 // are therefore handed out before the destinations' old ones return, and no page that is still read is
@@ -283,7 +314,7 @@ struct ForkArgs {
     int n_seqs, width, pages, page, n;
 };
 
-__global__ void __launch_bounds__(kPlanThreads) page_fork_plan_kernel(const ForkArgs a) {
+__device__ void fork_plan(const ForkArgs& a) {
     extern __shared__ int32_t owner[];
     __shared__ int warp_sums[32];
     for (int s = threadIdx.x; s < a.n_seqs; s += kPlanThreads) owner[s] = 0x7fffffff;
@@ -339,15 +370,12 @@ __global__ void __launch_bounds__(kPlanThreads) page_fork_plan_kernel(const Fork
     if (lacking) atomicAdd(a.status + 1, lacking);
 }
 
-// blockIdx.x: entry; blockIdx.y: part of its row of the table, and of its copies.
+// Entry i's new row of the table, the references it adds, and its copies: thread t0 of `step`.
 template <int CAP>
-__global__ void __launch_bounds__(kCopyThreads) page_fork_stage_kernel(const ForkArgs a,
-                                                                       const __grid_constant__ Buffers<CAP> bufs) {
-    const int i = blockIdx.x;
+__device__ __forceinline__ void fork_stage(const ForkArgs& a, const Buffers<CAP>& bufs, int i, int t0, int step) {
     const ForkPlan p = a.plan[i];
     if (p.src < 0) return;
     const int full = p.len / a.page, tail = p.len % a.page;
-    const int step = gridDim.y * kCopyThreads, t0 = blockIdx.y * kCopyThreads + threadIdx.x;
     for (int m = t0; m < a.width; m += step) {
         int e = -1;
         if (m < full) {
@@ -371,18 +399,45 @@ __global__ void __launch_bounds__(kCopyThreads) page_fork_stage_kernel(const For
     }
 }
 
-__global__ void __launch_bounds__(kCopyThreads) page_fork_commit_kernel(const ForkArgs a) {
-    const int i = blockIdx.x;
+// The old row's references go, the new one comes.
+__device__ __forceinline__ void fork_commit(const ForkArgs& a, int i, int t0, int step) {
     const ForkPlan p = a.plan[i];
     if (p.src < 0) return;
     const int d = a.dst[i];
-    for (int m = blockIdx.y * kCopyThreads + threadIdx.x; m < a.width; m += gridDim.y * kCopyThreads) {
+    for (int m = t0; m < a.width; m += step) {
         int32_t* const e = a.table + d * a.table_stride + m;
         const int old = *e;
         if (old >= 0 && old < a.pages) atomicSub(a.refs + old, 1);
         *e = a.staged[static_cast<int64_t>(i) * a.width + m];
     }
-    if (blockIdx.y == 0 && threadIdx.x == 0) a.lens[d] = p.len;
+    if (t0 == 0) a.lens[d] = p.len;
+}
+
+__global__ void __launch_bounds__(kPlanThreads) page_fork_plan_kernel(const ForkArgs a) { fork_plan(a); }
+
+// blockIdx.x: entry; blockIdx.y: part of its row of the table, and of its copies.
+template <int CAP>
+__global__ void __launch_bounds__(kCopyThreads) page_fork_stage_kernel(const ForkArgs a,
+                                                                       const __grid_constant__ Buffers<CAP> bufs) {
+    fork_stage(a, bufs, blockIdx.x, blockIdx.y * kCopyThreads + threadIdx.x, gridDim.y * kCopyThreads);
+}
+__global__ void __launch_bounds__(kCopyThreads) page_fork_commit_kernel(const ForkArgs a) {
+    fork_commit(a, blockIdx.x, blockIdx.y * kCopyThreads + threadIdx.x, gridDim.y * kCopyThreads);
+}
+
+// All three in one block, for few entries and small pages (pages of 64 rows of 1152 bytes, calls in a row: 14.4 us in
+// three launches whatever the tail; in one 8.2 for one entry, 10.3 to 13.6 for 4 with tails of 28 and 63 rows, 12.7 to
+// 19.0 for 8).
+constexpr int kForkEntries = 4;
+constexpr int64_t kForkBytes = 320 << 10;
+__global__ void __launch_bounds__(kPlanThreads) page_fork_kernel(const ForkArgs a,
+                                                                 const __grid_constant__ Buffers<kFewBuffers> bufs) {
+    fork_plan(a);
+    __syncthreads();
+    const int share = kPlanThreads / a.n, i = threadIdx.x / share, t0 = threadIdx.x % share;
+    if (i < a.n) fork_stage(a, bufs, i, t0, share);
+    __syncthreads();
+    if (i < a.n) fork_commit(a, i, t0, share);
 }
 
 // ---- compact and copy ---------------------------------------------------------------------------
@@ -538,6 +593,17 @@ static int fill_buffers(const char* who, AllBuffers* out, void* const* bases, co
     return RT_OK;
 }
 
+static int fill_rows(const char* who, AllRows* out, const void* const* rows, const int64_t* row_strides, int64_t n) {
+    RT_REQUIRE(rows && row_strides, RT_ERR_BAD_ARG, "%s: null pointer", who);
+    for (int64_t i = 0; i < n; ++i) {
+        RT_REQUIRE(rows[i] && (reinterpret_cast<uintptr_t>(rows[i]) & 3) == 0 && row_strides[i] % 4 == 0 && row_strides[i] >= 0,
+                   RT_ERR_BAD_ARG, "%s: rows must be 4-byte aligned", who);
+        out->base[i] = static_cast<const uint8_t*>(rows[i]);
+        out->stride[i] = row_strides[i];
+    }
+    return RT_OK;
+}
+
 }  // namespace page
 }  // namespace rt
 
@@ -545,23 +611,34 @@ using namespace rt;
 
 extern "C" int64_t rt_page_extend_workspace_ints(int64_t n, int64_t tokens) { return 2 * n + tokens; }
 
+// The arguments of an extension, checked.
+static int extend_args(const char* who, page::ExtendArgs* a, int32_t* table, int64_t table_stride, int32_t* lens, int32_t* refs, int32_t* status,
+                       const int32_t* seqs, const int32_t* offsets, int32_t* slots, int32_t* workspace, int64_t n_seqs,
+                       int64_t width, int64_t pages, int64_t page_size, int64_t n, int64_t tokens) {
+    if (int rc = page::check_table(who, table, lens, refs, table_stride, n_seqs, width, pages, page_size))
+        return rc;
+    RT_REQUIRE(n >= 0 && tokens >= 0 && n < (1ll << 30) && tokens < (1ll << 30), RT_ERR_BAD_ARG, "%s: bad list", who);
+    RT_REQUIRE(offsets || tokens == n, RT_ERR_BAD_ARG, "%s: without offsets every entry brings one token", who);
+    RT_REQUIRE(seqs || n <= n_seqs, RT_ERR_BAD_ARG, "%s: more entries than sequences", who);
+    RT_REQUIRE((n == 0 && tokens == 0) || (status && workspace && (tokens == 0 || slots)), RT_ERR_BAD_ARG, "%s: null pointer", who);
+    *a = page::ExtendArgs{table, table_stride, lens, refs, status, seqs, offsets, slots, workspace,
+                          static_cast<int>(n_seqs), static_cast<int>(width), static_cast<int>(pages),
+                          static_cast<int>(page_size), static_cast<int>(n), static_cast<int>(tokens)};
+    return RT_OK;
+}
+
 extern "C" int rt_page_extend(int32_t* table, int64_t table_stride, int32_t* lens, int32_t* refs, int32_t* status,
                               const int32_t* seqs, const int32_t* offsets, int32_t* slots, int32_t* workspace,
                               int64_t n_seqs, int64_t width, int64_t pages, int64_t page_size, int64_t n, int64_t tokens,
                               void* stream) {
-    if (int rc = page::check_table("rt_page_extend", table, lens, refs, table_stride, n_seqs, width, pages, page_size))
+    page::ExtendArgs a;
+    if (int rc = extend_args("rt_page_extend", &a, table, table_stride, lens, refs, status, seqs, offsets, slots, workspace,
+                             n_seqs, width, pages, page_size, n, tokens))
         return rc;
-    RT_REQUIRE(n >= 0 && tokens >= 0 && n < (1ll << 30) && tokens < (1ll << 30), RT_ERR_BAD_ARG, "rt_page_extend: bad list");
-    RT_REQUIRE(offsets || tokens == n, RT_ERR_BAD_ARG, "rt_page_extend: without offsets every entry brings one token");
-    RT_REQUIRE(seqs || n <= n_seqs, RT_ERR_BAD_ARG, "rt_page_extend: more entries than sequences");
     if (n == 0 && tokens == 0) return RT_OK;
-    RT_REQUIRE(status && workspace && (tokens == 0 || slots), RT_ERR_BAD_ARG, "rt_page_extend: null pointer");
     const int smem = static_cast<int>(n_seqs * 4);
     if (int rc = ensure_dynamic_smem(reinterpret_cast<const void*>(&page::page_extend_kernel), smem, "rt_page_extend"))
         return rc;
-    page::ExtendArgs a{table, table_stride, lens, refs, status, seqs, offsets, slots, workspace,
-                       static_cast<int>(n_seqs), static_cast<int>(width), static_cast<int>(pages),
-                       static_cast<int>(page_size), static_cast<int>(n), static_cast<int>(tokens)};
     page::page_extend_kernel<<<1, page::kPlanThreads, smem, as_stream(stream)>>>(a);
     count_launch();
     return check_launch("page_extend_kernel");
@@ -576,30 +653,53 @@ extern "C" int rt_page_write(void* const* bases, const int64_t* page_strides, co
     page::AllRows r{};
     if (tokens == 0 || pages == 0 || n_buffers == 0) return RT_OK;
     if (int rc = page::fill_buffers("rt_page_write", &bufs, bases, page_strides, row_bytes, n_buffers, page_size)) return rc;
-    RT_REQUIRE(slots && rows && row_strides, RT_ERR_BAD_ARG, "rt_page_write: null pointer");
-    for (int64_t i = 0; i < n_buffers; ++i) {
-        RT_REQUIRE(rows[i] && (reinterpret_cast<uintptr_t>(rows[i]) & 3) == 0 && row_strides[i] % 4 == 0 && row_strides[i] >= 0,
-                   RT_ERR_BAD_ARG, "rt_page_write: rows must be 4-byte aligned");
-        r.base[i] = static_cast<const uint8_t*>(rows[i]);
-        r.stride[i] = row_strides[i];
-    }
+    RT_REQUIRE(slots, RT_ERR_BAD_ARG, "rt_page_write: null pointer");
+    if (int rc = page::fill_rows("rt_page_write", &r, rows, row_strides, n_buffers)) return rc;
     const int64_t blocks = (tokens * n_buffers + page::kCopyThreads / 32 - 1) / (page::kCopyThreads / 32);
     const int64_t most = 8ll * page::sms();
     const unsigned grid = static_cast<unsigned>(blocks < most ? blocks : most);
     if (n_buffers <= page::kFewBuffers) {
-        page::Rows<page::kFewBuffers> fr;
-        for (int i = 0; i < page::kFewBuffers; ++i) {
-            fr.base[i] = r.base[i];
-            fr.stride[i] = r.stride[i];
-        }
         page::page_write_kernel<<<grid, page::kCopyThreads, 0, as_stream(stream)>>>(
-            page::few(bufs), fr, slots, tokens, pages, static_cast<int>(page_size));
+            page::few(bufs), page::few(r), slots, tokens, pages, static_cast<int>(page_size));
     } else {
         page::page_write_kernel<<<grid, page::kCopyThreads, 0, as_stream(stream)>>>(bufs, r, slots, tokens, pages,
                                                                                     static_cast<int>(page_size));
     }
     count_launch();
     return check_launch("page_write_kernel");
+}
+
+extern "C" int rt_page_append(void* const* bases, const int64_t* page_strides, const int64_t* row_bytes,
+                              const void* const* rows, const int64_t* row_strides, int64_t n_buffers, int32_t* table,
+                              int64_t table_stride, int32_t* lens, int32_t* refs, int32_t* status, const int32_t* seqs,
+                              const int32_t* offsets, int32_t* slots, int32_t* workspace, int64_t n_seqs, int64_t width,
+                              int64_t pages, int64_t page_size, int64_t n, int64_t tokens, void* stream) {
+    page::ExtendArgs a;
+    page::AllBuffers bufs{};
+    page::AllRows r{};
+    if (int rc = extend_args("rt_page_append", &a, table, table_stride, lens, refs, status, seqs, offsets, slots, workspace,
+                             n_seqs, width, pages, page_size, n, tokens))
+        return rc;
+    const bool writes = tokens > 0 && pages > 0 && n_buffers != 0;
+    int64_t row_total = 0;
+    if (writes) {
+        if (int rc = page::fill_buffers("rt_page_append", &bufs, bases, page_strides, row_bytes, n_buffers, page_size)) return rc;
+        if (int rc = page::fill_rows("rt_page_append", &r, rows, row_strides, n_buffers)) return rc;
+        for (int i = 0; i < bufs.n; ++i) row_total += bufs.b[i].row_bytes;
+    }
+    if (!writes || tokens > page::kAppendTokens || tokens * row_total > page::kAppendBytes || bufs.n > page::kFewBuffers) {
+        if (int rc = rt_page_extend(table, table_stride, lens, refs, status, seqs, offsets, slots, workspace, n_seqs, width,
+                                    pages, page_size, n, tokens, stream))
+            return rc;
+        return writes ? rt_page_write(bases, page_strides, row_bytes, rows, row_strides, n_buffers, slots, tokens, pages,
+                                      page_size, stream) : RT_OK;
+    }
+    const int smem = static_cast<int>(n_seqs * 4);
+    if (int rc = ensure_dynamic_smem(reinterpret_cast<const void*>(&page::page_append_kernel), smem, "rt_page_append"))
+        return rc;
+    page::page_append_kernel<<<1, page::kPlanThreads, smem, as_stream(stream)>>>(a, page::few(bufs), page::few(r));
+    count_launch();
+    return check_launch("page_append_kernel");
 }
 
 extern "C" int rt_page_free(int32_t* table, int64_t table_stride, int32_t* lens, int32_t* refs, const int32_t* seqs,
@@ -641,6 +741,16 @@ extern "C" int rt_page_fork(void* const* bases, const int64_t* page_strides, con
     a.n_seqs = static_cast<int>(n_seqs); a.width = static_cast<int>(width); a.pages = static_cast<int>(pages);
     a.page = static_cast<int>(page_size); a.n = static_cast<int>(n);
     cudaStream_t st = as_stream(stream);
+    int64_t page_bytes = 0;
+    for (int i = 0; i < bufs.n; ++i) page_bytes += bufs.b[i].page_bytes;
+    if (n <= page::kForkEntries && bufs.n <= page::kFewBuffers && n * page_bytes <= page::kForkBytes &&
+        n * width <= 4 * page::kPlanThreads) {
+        if (int rc = ensure_dynamic_smem(reinterpret_cast<const void*>(&page::page_fork_kernel), smem, "rt_page_fork"))
+            return rc;
+        page::page_fork_kernel<<<1, page::kPlanThreads, smem, st>>>(a, page::few(bufs));
+        count_launch();
+        return check_launch("page_fork_kernel");
+    }
     page::page_fork_plan_kernel<<<1, page::kPlanThreads, smem, st>>>(a);
     count_launch();
     if (int rc = check_launch("page_fork_plan_kernel")) return rc;

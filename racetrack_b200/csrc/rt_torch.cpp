@@ -28,7 +28,7 @@ using OptTensor = std::optional<Tensor>;
     X(rt_gemm_bf16) X(rt_gemm_bf16_splitk_splits) X(rt_gemm_bf16_splitk) X(rt_gemm_bf16_batched)  \
     X(rt_gemm_fp8) X(rt_gemm_nvfp4_grouped) X(rt_index_prep_into) X(rt_index_head_weights) X(rt_fp8_index_batched)              \
     X(rt_index_topk) X(rt_mla_sparse_decode_splits) X(rt_mla_sparse_decode)                       \
-    X(rt_page_extend_workspace_ints) X(rt_page_extend) X(rt_page_write) X(rt_page_free)           \
+    X(rt_page_extend_workspace_ints) X(rt_page_extend) X(rt_page_append) X(rt_page_write) X(rt_page_free)           \
     X(rt_page_fork_workspace_ints) X(rt_page_fork) X(rt_page_compact_workspace_ints)              \
     X(rt_page_compact) X(rt_page_copy) X(rt_mla_paged_decode_workspace_bytes) X(rt_mla_paged_decode) \
     X(rt_attn_causal_prefill_share) X(rt_attn_window_prefill)
@@ -976,8 +976,9 @@ PageBuffers page_buffers(const std::string& who, const std::vector<Tensor>& buff
     return p;
 }
 
-Tensor extend(const std::string& who, const Tables& t, const Tensor& status, int64_t tokens, int64_t page,
-              const OptTensor& seqs, const OptTensor& offsets) {
+// The entries of a list that grows sequences by `tokens`, checked.
+int64_t extend_entries(const std::string& who, const Tables& t, const Tensor& status, int64_t tokens, int64_t page,
+                       const OptTensor& seqs, const OptTensor& offsets) {
     require_status(who, status, t.table);
     if (tokens < 0 || page < 1) fail(who + ": tokens and page_size must not be negative or zero");
     if (seqs) require_list(who, "seqs", *seqs, t.table);
@@ -989,20 +990,21 @@ Tensor extend(const std::string& who, const Tables& t, const Tensor& status, int
     if (seqs && seqs->numel() != n) fail(who + ": offsets must have one entry more than seqs");
     if (!offsets && tokens != n) fail(who + ": without offsets every sequence of the list gets one token");
     if (!seqs && n > t.seqs()) fail(who + ": more entries than the table has sequences");
-    Tensor slots = empty({tokens}, at::kInt, t.table);
-    Tensor work = empty({std::max<int64_t>(1, p_rt_page_extend_workspace_ints(n, tokens))}, at::kInt, t.table);
-    check(p_rt_page_extend(data<int32_t>(t.table), t.stride(), data<int32_t>(t.lens), data<int32_t>(t.refs),
-                           data<int32_t>(status), data<int32_t>(seqs), data<int32_t>(offsets), data<int32_t>(slots),
-                           data<int32_t>(work), t.seqs(), t.width(), t.pages(), page, n, tokens, stream()),
-          "rt_page_extend");
-    return slots;
+    return n;
 }
 
 Tensor page_extend(const Tensor& table, const Tensor& lens, const Tensor& refs, const Tensor& status, int64_t tokens,
                    int64_t page_size, const OptTensor& seqs, const OptTensor& offsets) {
     const Tables t = page_tables("page_extend", table, lens, refs);
     const c10::cuda::CUDAGuard guard(table.device());
-    return extend("page_extend", t, status, tokens, page_size, seqs, offsets);
+    const int64_t n = extend_entries("page_extend", t, status, tokens, page_size, seqs, offsets);
+    Tensor slots = empty({tokens}, at::kInt, table);
+    Tensor work = empty({std::max<int64_t>(1, p_rt_page_extend_workspace_ints(n, tokens))}, at::kInt, table);
+    check(p_rt_page_extend(data<int32_t>(table), t.stride(), data<int32_t>(lens), data<int32_t>(refs), data<int32_t>(status),
+                           data<int32_t>(seqs), data<int32_t>(offsets), data<int32_t>(slots), data<int32_t>(work), t.seqs(),
+                           t.width(), t.pages(), page_size, n, tokens, stream()),
+          "rt_page_extend");
+    return slots;
 }
 
 // The rows of a call, one tensor [tokens, ...] a buffer, and the copies that keep them alive.
@@ -1043,12 +1045,6 @@ PageRows page_rows(const std::string& who, const std::vector<Tensor>& buffers, c
     return r;
 }
 
-void write(const PageBuffers& p, const PageRows& r, const Tensor& slots) {
-    check(p_rt_page_write(p.bases.data(), p.strides.data(), p.row_bytes.data(), r.bases.data(), r.strides.data(), p.n,
-                          data<int32_t>(slots), r.tokens, p.pages, p.page, stream()),
-          "rt_page_write");
-}
-
 void page_write(const std::vector<Tensor>& buffers, const std::vector<Tensor>& rows, const Tensor& slots) {
     require_cuda({&slots});
     if (buffers.empty()) fail("page_write: at least one page buffer is required");
@@ -1057,7 +1053,9 @@ void page_write(const std::vector<Tensor>& buffers, const std::vector<Tensor>& r
     const c10::cuda::CUDAGuard guard(slots.device());
     const PageRows r = page_rows("page_write", buffers, rows);
     if (slots.numel() != r.tokens) fail("page_write: one slot for each row is required");
-    write(p, r, slots);
+    check(p_rt_page_write(p.bases.data(), p.strides.data(), p.row_bytes.data(), r.bases.data(), r.strides.data(), p.n,
+                          data<int32_t>(slots), r.tokens, p.pages, p.page, stream()),
+          "rt_page_write");
 }
 
 Tensor page_append(const std::vector<Tensor>& buffers, const std::vector<Tensor>& rows, const Tensor& table,
@@ -1067,8 +1065,14 @@ Tensor page_append(const std::vector<Tensor>& buffers, const std::vector<Tensor>
     const PageBuffers p = page_buffers("page_append", buffers, table, t.pages());
     const c10::cuda::CUDAGuard guard(table.device());
     const PageRows r = page_rows("page_append", buffers, rows);
-    const Tensor slots = extend("page_append", t, status, r.tokens, p.page, seqs, offsets);
-    write(p, r, slots);
+    const int64_t n = extend_entries("page_append", t, status, r.tokens, p.page, seqs, offsets);
+    Tensor slots = empty({r.tokens}, at::kInt, table);
+    Tensor work = empty({std::max<int64_t>(1, p_rt_page_extend_workspace_ints(n, r.tokens))}, at::kInt, table);
+    check(p_rt_page_append(p.bases.data(), p.strides.data(), p.row_bytes.data(), r.bases.data(), r.strides.data(), p.n,
+                           data<int32_t>(table), t.stride(), data<int32_t>(lens), data<int32_t>(refs), data<int32_t>(status),
+                           data<int32_t>(seqs), data<int32_t>(offsets), data<int32_t>(slots), data<int32_t>(work), t.seqs(),
+                           t.width(), t.pages(), p.page, n, r.tokens, stream()),
+          "rt_page_append");
     return slots;
 }
 

@@ -237,6 +237,36 @@ def test_long_lists_take_several_passes_of_the_block():
     same(c, m)
 
 
+@pytest.mark.parametrize("tokens, forks", [(1, 1), (63, 3), (64, 4), (65, 5), (129, 9)])
+def test_lists_on_both_sides_of_the_single_launch(tokens, forks):
+    c, m = make(700, 16, tokens + 10, 4)
+    append(c, m, list(range(tokens)), [1 + 7 * i % 31 for i in range(tokens)], 40)
+    for step in range(3):
+        append(c, m, list(range(tokens)), [1] * tokens, 41 + step, offsets=False)
+    append(c, m, [0], [min(tokens, 33)], 44)                    # all of the rows to one sequence
+    pairs = ([i % tokens for i in range(forks)], [tokens + i for i in range(forks)])
+    c.fork(ints(pairs[0]), ints(pairs[1]))
+    m.fork(*pairs)
+    c.fork(ints(pairs[1]), ints(pairs[0][:1] + pairs[1][:-1]))  # each to its neighbour's place
+    m.fork(pairs[1], pairs[0][:1] + pairs[1][:-1])
+    same(c, m)
+    m.assert_consistent()
+
+
+def test_wide_tables_and_long_pages_fork():
+    """One entry whose row of the table, and one whose pages, are more than a single block is given."""
+    c, m = make(30, 16, 4, 5000, extra=None)
+    append(c, m, [0, 1], [70, 33], 45)
+    c.fork(ints([0]), ints([2]))
+    m.fork([0], [2])
+    same(c, m)
+    c, m = make(3, 1024, 3, 2, extra=None)
+    append(c, m, [0], [1023], 46)
+    c.fork(ints([0]), ints([2]))
+    m.fork([0], [2])
+    same(c, m)
+
+
 def test_many_buffers_at_once():
     """All layers' buffers under one table."""
     c, m = make(8, 16, 3, 3, extra={f"layer{i}": ((8,), torch.bfloat16) for i in range(60)})

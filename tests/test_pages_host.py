@@ -58,6 +58,16 @@ def test_c_entry_points_check_shapes_before_any_launch(lib):
     assert extend(page=0) == -1 and extend(n=-1, tokens=-1) == -1
     assert extend(n=0, tokens=0) == 0
 
+    def append(rows=base, row_stride=64, row=64, seqs=4, n=1, tokens=1, n_buffers=1, stride=64 * 16, slots=p):
+        return lib.rt_page_append(base, one(stride), one(row), rows, one(row_stride), n_buffers, p, 4, p, p, p, p, None, slots,
+                                  p, seqs, 4, 8, 16, n, tokens, None)
+    assert append(seqs=40000) == -2 and append(slots=None) == -1 and append(tokens=3) == -1
+    assert append(rows=(ctypes.c_void_p * 1)(p + 2)) == -1 and b"4-byte aligned" in lib.rt_last_error()
+    assert append(rows=None) == -1 and append(row_stride=-64) == -1 and append(row_stride=6) == -1
+    assert append(row=6) == -1 and append(stride=8) == -1 and append(n_buffers=-1) == -2
+    assert append(seqs=4, n=1, tokens=1, rows=(ctypes.c_void_p * 1)(None)) == -1
+    assert append(n=0, tokens=0) == 0
+
     def copy(base_ptr=base, stride=64 * 16, row=64, n_buffers=1, page=16):
         return lib.rt_page_copy(base_ptr, one(stride), one(row), n_buffers, p, p, 1, 8, page, None)
     assert copy(row=6) == -1 and b"multiples of 4" in lib.rt_last_error()
