@@ -9,6 +9,14 @@
 //
 // A row of 1152 bytes serves 2 * 1088 flops for each head, 242 flop/B at 128 heads: with few heads the
 // kernel is bound by reading the cache once, with all of them memory and tensor cores take about the same.
+// Measured on one B200, kernels and join, calls in a row on inputs of three sets (copy rate 6546 GB/s):
+//   16 heads, 48 sequences of up to 32768 (0.56 GB)  97 us, 5740 GB/s; 64 of 4096 (0.30 GB) 60 us
+//   32 heads, 128 under a window of 1024 (0.11 GB)   40 us; 64 of 4096 67 us
+//   128 heads, 64 of 4096                            96 us, 760 TFLOP/s; 64 heads 75 us
+//   one sequence of 17 positions, 16 heads           10 us; of 131072 41 us
+// Two kernels share the walk over the tiles and the join. mla_paged_kernel serves groups of up to 32 heads,
+// mla_paged_wide_kernel of 64; each served all groups once: the first takes 124 us for 64 x 4096 at 128 heads
+// (80 at 64), the second 45 for the window's case and 100 for the ragged one.
 #include "rt_tc.cuh"
 
 namespace rt {
@@ -24,7 +32,7 @@ constexpr int kPMaxBatch = 65535;
 // The visible positions of row b are the tiles {0 .. na - 1} (sinks) and {b0 .. b0 + nb - 1} of 64
 // positions. All rows' tiles in one line are cut into as many equal ranges as there are CTAs, so
 // ragged lengths keep every SM busy alike; a row that crosses from one range into the next is finished by
-// the merge kernel. The host knows no length: each CTA sums them itself.
+// the join kernel. The host knows no length: each CTA sums them itself.
 struct PagedArgs {
     const int32_t* table;         // [slots, width]
     const int32_t* lens;          // [slots]
@@ -135,35 +143,37 @@ __device__ RangeStart find_range(const PagedArgs& a, int range, volatile int* sc
     return r;
 }
 
-// ---- the kernel -------------------------------------------------------------------------------
-// Work of a CTA: its range of tiles for one group of G heads (16, 32 or 64; more heads are several groups,
-// whose CTAs run side by side and share the tiles in L2). Positions and dims are the rows of the products,
-// heads the columns: with few heads what the tensor core reads from shared memory is then little
-// more than the tile itself. (Heads as rows, padded to 128, took 2300 + 1400 cycles a tile for 16 heads:
-// 4 KB of mostly empty query rows for each instruction. This form takes about half.) Per tile of 64
-// positions:
-//   producer  one TMA box a page brings the latent rows as [8-row groups][8 blocks of 64 dims][8 rows][128
-//             B] (128-byte swizzle), one the rope keys: a page of any size lands in the same
-//             layout, of which both products read their operand (the group stride is a field of the
-//             descriptor), so the rows are staged once. Two tiles in flight (144 KB);
+// ---- up to 32 heads a group -------------------------------------------------------------------
+// Work of a CTA: its range of tiles for one group of G heads, 16 or 32 (more heads are several groups, whose CTAs
+// run side by side and share the tiles in L2). Positions and dims are the rows of the products, heads the
+// columns: with few heads what the tensor core reads from shared memory is then little more than the tile
+// itself. (Heads as rows, padded to 128, took 2300 + 1400 cycles a tile for 16 heads: 4 KB of mostly empty
+// query rows for each instruction. This form takes about half.) Per tile of 64 positions:
+//   producer  one TMA box a page (32 positions at most, which are also given back together) brings the latent
+//             rows as [8-row groups][8 blocks of 64 dims][8 rows][128 B] (128-byte swizzle), one the rope keys: a
+//             page of any size lands in the same layout, of which both products read their operand (the group
+//             stride is a field of the descriptor), so the rows are staged once. Two tiles are staged (144 KB);
+//             the one behind them is asked into L2 (without: 64 x 4096 x 128 heads 128 us instead of 123, ragged
+//             104 instead of 99; two or three tiles ahead are no better). Boxes of half or a quarter of the dims
+//             instead of the positions: 134 and 142 us;
 //   S = K Q^T 36 tcgen05.mma (M = 64 positions, N = G heads, K = 16 dims), both K-major;
-//   softmax   a thread holds one position's scores of 16 or 32 heads (an M = 64 product lies in lanes 0-15
-//             of each quarter of tensor memory). The maxima it works against change only when a score
-//             exceeds one by 2^8: all warps vote on that, and only then (and at a row's first tile)
-//             look for new maxima, across lanes and warps. P = 2^(s - m) goes as bf16 into shared memory,
-//             one 128-byte line of heads a position; a thread sums its own probabilities in fp32,
-//             and the sums meet at the row's end;
+//   softmax   warps 4-7. An M = 64 product lies in lanes 0-15 of each quarter of tensor memory; read in 16 x 256
+//             bit blocks a thread holds two positions of G / 4 heads, so all lanes work. The maxima change only
+//             when a score exceeds one by 2^8: all warps vote on that, and only then (and at a row's first tile)
+//             look for new maxima, across lanes and warps. P = 2^(s - m) goes as bf16 into shared memory, one
+//             128-byte line of heads a position; a thread sums its own probabilities in fp32, and the sums meet
+//             at the row's end;
 //   O^T += V^T P^T  tcgen05.mma (M = 128 of the 512 dims, N = G, K = 16 positions): the tile again, as the
-//             MN-major operand, P MN-major too. Only steps that hold a visible position are multiplied.
+//             MN-major operand, P MN-major too. Only steps that hold a visible position are multiplied;
+//   output    warps 8-11 read a finished row from tensor memory while the next one's first tile is under way.
 // O is 4 blocks of G columns in tensor memory, the two score buffers 2 G behind it. All sums, maxima and O
 // are fp32; P is rounded to bf16 because the tensor core multiplies it with bf16 rows (2^-8 of a
 // probability at most, no more than the rounding of the rows). Positions that are not visible weigh
 // exactly nothing whatever memory holds there: their scores are not looked at, their rows are zeroed in
 // shared memory between the two products (0 * NaN). A page number outside the pool reads as zeros (the
 // TMA unit's bounds) and its positions are not visible.
-constexpr int kPMaxG = 64;
 constexpr uint32_t kPQRow = 9 * 128;                 // bytes of a staged head
-constexpr uint32_t kPQBytes = kPMaxG * kPQRow;       // two sets of queries of up to 32 heads, or one of 64
+constexpr uint32_t kPQBytes = 2 * 32 * kPQRow;       // two rows' queries
 constexpr uint32_t kPKOff = kPQBytes;
 constexpr uint32_t kPPOff = kPKOff + 2 * kPTileBytes;        // P: [64 positions][64 heads] bf16
 constexpr uint32_t kPBarOff = kPPOff + kPTile * 128;
@@ -186,6 +196,11 @@ struct TileInfo {
 __device__ __forceinline__ uint64_t smem_desc_groups(uint32_t addr, uint32_t lbo, uint32_t sbo) {
     return static_cast<uint64_t>((addr & 0x3ffffu) >> 4) | (static_cast<uint64_t>(lbo >> 4) << 16) |
            (static_cast<uint64_t>(sbo >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+
+// A descriptor whose halves are known apart: start address and leading offset (in 16 bytes), group stride and mode.
+__device__ __forceinline__ uint64_t smem_desc_at(uint32_t low, uint32_t sbo) {
+    return static_cast<uint64_t>(low) | (static_cast<uint64_t>((sbo >> 4) | (1u << 14) | (2u << 29)) << 32);
 }
 
 __device__ __forceinline__ void tma_load_5d(uint32_t dst, const CUtensorMap* m, int c0, int c1, int c2, int c3,
@@ -282,6 +297,62 @@ __device__ __forceinline__ int part_slot(int flags, int range) {
     return (flags & 12) == 12 ? -1 : 2 * range + ((flags & 4) ? 1 : 0);
 }
 
+// O (the same quarter) times a factor a head.
+template <int G>
+__device__ __forceinline__ void rescale(uint32_t o_at, const float* w) {
+    constexpr int kCols = G < 32 ? G : 32;
+#pragma unroll 1
+    for (int c = 0; c < 4 * G; c += kCols) {
+        uint32_t o[kCols];
+        tmem_ld_cols(o_at + c, o);
+#pragma unroll
+        for (int i = 0; i < kCols; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * w[(c & (G - 1)) + i]);
+        tmem_st_cols(o_at + c, o);
+    }
+    tmem_st_wait();
+}
+
+// A finished row's O (warp: a quarter of each block of 128 dims, all G heads) times f, to its output or its part.
+template <int G>
+__device__ __forceinline__ void write_row(const PagedArgs& a, int part, int row, int head0, uint32_t o_at, const float* f) {
+    constexpr int kCols = G < 32 ? G : 32;
+    const int d0 = threadIdx.x & 127;
+#pragma unroll 1
+    for (int c = 0; c < 4 * G; c += kCols) {
+        uint32_t o[kCols];
+        tmem_ld_cols(o_at + c, o);
+        const int h = c & (G - 1), d = (c / G) * 128 + d0;
+        const int64_t at = (static_cast<int64_t>(part < 0 ? row : part) * a.heads + head0 + h) * 512 + d;
+        const int live = a.heads - head0 - h;
+        // (factors before stores, and no branch a head: with both a head took 37 cycles, now 20)
+        float v[kCols];
+#pragma unroll
+        for (int i = 0; i < kCols; i += 4) *reinterpret_cast<float4*>(v + i) = *reinterpret_cast<const float4*>(f + h + i);
+#pragma unroll
+        for (int i = 0; i < kCols; ++i) v[i] = v[i] == 0.f ? 0.f : __uint_as_float(o[i]) * v[i];
+        auto each = [&](auto put) {
+            if (live >= kCols) {
+#pragma unroll
+                for (int i = 0; i < kCols; ++i) put(i);
+            } else {
+#pragma unroll
+                for (int i = 0; i < kCols; ++i)
+                    if (i < live) put(i);
+            }
+        };
+        if (part < 0) each([&](int i) { a.out[at + i * 512] = __float2bfloat16_rn(v[i]); });
+        else each([&](int i) { a.part_o[at + i * 512] = v[i]; });
+    }
+}
+
+// Rows without a visible tile are nobody's: zeros, shared out over the ranges (128 threads).
+__device__ __forceinline__ void clear_empty_rows(const PagedArgs& a, int range) {
+    for (int b = range; b < a.batch; b += a.n_ranges)
+        if (row_tiles(a, b).n == 0)
+            for (int c = threadIdx.x & 127; c < a.heads * 64; c += 128)
+                reinterpret_cast<uint4*>(a.out + static_cast<int64_t>(b) * a.heads * 512)[c] = make_uint4(0u, 0u, 0u, 0u);
+}
+
 // Where the tile walk of a range stands.
 struct TileWalk {
     int b, j, slot, row_at;                          // row, tile within it, its slot, the row that `t` is of
@@ -322,10 +393,8 @@ struct TileWalk {
             if (i < boxes) {
                 const int m = (tile * kPTile + i * rows) >> a.page_log;
                 id[i] = __shfl_sync(0xffffffffu, fetched, m - fetched0);
-                if (m >= used || id[i] < 0 || id[i] >= a.pages) {
-                    id[i] = -1;
-                    mask &= ~(row_bits << (i * rows));
-                }
+                if (m >= used || id[i] < 0 || id[i] >= a.pages) mask &= ~(row_bits << (i * rows));
+                if ((mask >> (i * rows) & row_bits) == 0) id[i] = -1;     // nothing visible: not read
             }
         }
     }
@@ -345,8 +414,8 @@ __global__ void __launch_bounds__(kPThreads, 1) mla_paged_kernel(const __grid_co
                                                                  const __grid_constant__ CUtensorMap tm_kv,
                                                                  const __grid_constant__ CUtensorMap tm_pe,
                                                                  const PagedArgs a) {
-    constexpr int kQBufs = G > 32 ? 1 : 2;
-    constexpr uint32_t kTmemS = 4 * G, kTmemCols = G == 16 ? 128 : G == 32 ? 256 : 512;
+    static_assert(G <= 32, "heads");
+    constexpr uint32_t kTmemS = 4 * G, kTmemCols = 8 * G;
     // fp32 accumulate, bf16 x bf16; S: both K-major, M = 64; O: both MN-major, M = 128
     constexpr uint32_t kSIdesc = (1u << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(G >> 3) << 17) | (4u << 24);
     constexpr uint32_t kOIdesc = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 15) | (1u << 16) |
@@ -423,8 +492,8 @@ __global__ void __launch_bounds__(kPThreads, 1) mla_paged_kernel(const __grid_co
                 bool progressed = false;
                 if (q < n_tiles && q - v < 2 && mbar_try_wait(kfull(q & 1), (q >> 1) & 1)) {
                     const int flags = info_s[q & 1].flags;
-                    const int qb = kQBufs == 2 ? (q_seg & 1) : 0;
-                    if (q_open || mbar_try_wait(qfull(qb), (kQBufs == 2 ? q_seg >> 1 : q_seg) & 1)) {
+                    const int qb = q_seg & 1;
+                    if (q_open || mbar_try_wait(qfull(qb), (q_seg >> 1) & 1)) {
                         tc_fence_after();
                         const uint32_t kb = base + kPKOff + (q & 1) * kPTileBytes;
                         const uint32_t qa = base + qb * (G * kPQRow);
@@ -499,7 +568,7 @@ __global__ void __launch_bounds__(kPThreads, 1) mla_paged_kernel(const __grid_co
         int seg = 0;
         if (n_tiles > 0) w.step(a, 0, n_tiles, rows);
         for (int g = 0; g < n_tiles; ++g) {
-            const int st = g & 1, qb = kQBufs == 2 ? (seg & 1) : 0;
+            const int st = g & 1, qb = seg & 1;
             const uint32_t free_par = ((g >> 1) & 1) ^ 1u;
             const uint32_t dst = base + kPKOff + st * kPTileBytes;
             bool ok = true;
@@ -507,7 +576,7 @@ __global__ void __launch_bounds__(kPThreads, 1) mla_paged_kernel(const __grid_co
             for (int half = 0; half < 2; ++half) {
                 if (!(ok = mbar_wait_warp(kfree(st, half), free_par, abort_flag, 82))) break;
                 if (half == 0 && (w.flags & 1) &&
-                    !(ok = mbar_wait_warp(qfree(qb), ((kQBufs == 2 ? seg >> 1 : seg) & 1) ^ 1u, abort_flag, 83)))
+                    !(ok = mbar_wait_warp(qfree(qb), ((seg >> 1) & 1) ^ 1u, abort_flag, 83)))
                     break;
                 if (elect_one()) {
                     if (half == 0) {
@@ -676,20 +745,7 @@ __global__ void __launch_bounds__(kPThreads, 1) mla_paged_kernel(const __grid_co
                 // O += P V of the tile before has retired: P may be overwritten, O is at rest
                 if (!mbar_wait_warp(pfree, (g - 1) & 1, abort_flag, 87)) break;
                 tc_fence_after();
-                if (over && !first) {
-                    constexpr int kCols = G < 32 ? G : 32;
-#pragma unroll 1
-                    for (int c = 0; c < 4 * G; c += kCols) {
-                        uint32_t o[kCols];
-                        const uint32_t at = tmem_base + lane_base + c;
-                        tmem_ld_cols(at, o);
-                        const float* w = w_s + (c & (G - 1));
-#pragma unroll
-                        for (int i = 0; i < kCols; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * w[i]);
-                        tmem_st_cols(at, o);
-                    }
-                    tmem_st_wait();
-                }
+                if (over && !first) rescale<G>(tmem_base + lane_base, w_s);
             }
 #pragma unroll
             for (int u = 0; u < G / 8; u += 2)
@@ -735,37 +791,492 @@ __global__ void __launch_bounds__(kPThreads, 1) mla_paged_kernel(const __grid_co
         // finished rows out of tensor memory, while the next row's first tile is on its way
         const int quad = warp & 3;
         const uint32_t lane_base = static_cast<uint32_t>(quad * 32) << 16;
-        const int d0 = quad * 32 + lane, head0 = hg * G;
-        // rows without a visible tile are nobody's: zeros, shared out over the CTAs
-        if (hg == 0)
-            for (int b = range; b < a.batch; b += a.n_ranges)
-                if (row_tiles(a, b).n == 0)
-                    for (int c = threadIdx.x - 256; c < a.heads * 64; c += 128)
-                        reinterpret_cast<uint4*>(a.out + static_cast<int64_t>(b) * a.heads * 512)[c] = make_uint4(0u, 0u, 0u, 0u);
-        constexpr int kCols = G < 32 ? G : 32;
+        if (hg == 0) clear_empty_rows(a, range);
         for (int seg = 0, left = n_tiles; left > 0; ++seg) {
             if (!mbar_wait_warp(efull, seg & 1, abort_flag, 94)) break;
             const int b = done_s[0], part = done_s[1], tiles = done_s[2];
             if (!mbar_wait_warp(odone, seg & 1, abort_flag, 88)) break;
             tc_fence_after();
             left -= tiles;
-#pragma unroll 1
-            for (int c = 0; c < 4 * G; c += kCols) {
-                uint32_t o[kCols];
-                tmem_ld_cols(tmem_base + lane_base + c, o);
-                const int h = c & (G - 1), d = (c / G) * 128 + d0;
-                const int64_t at = (static_cast<int64_t>(part < 0 ? b : part) * a.heads + head0 + h) * 512 + d;
-                const int live = a.heads - head0 - h;
+            write_row<G>(a, part, b, hg * G, tmem_base + lane_base, f_s);
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(ofree);
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 0) {
+        tc_fence_after();
+        tmem_dealloc(tmem_base, kTmemCols);
+    }
+}
+
+// ---- 33 heads and more ------------------------------------------------------------------------
+// Groups of 64 heads, the same mathematics. With 64 query rows in shared memory only two tiles fit beside them,
+// and a tile's way (load 2000 cycles, scores 1400, softmax 1400, P V 1100) took 3100 cycles over two places. Here
+// the queries lie in tensor memory, as the A operand of the scores: 64 heads are its rows, dims 0-287 of the
+// rows 16 i .. 16 i + 15 in lanes 32 i .. of 144 columns, dims 288-575 in lanes 32 i + 16 .. of the same columns,
+// each half with a product of its own (18 tcgen05.mma, M = 64, N = 64 positions), and the softmax adds
+// the two. O^T (256 columns), the scores (64) and the queries (144) fill the 512 columns, and the ring in
+// shared memory has three places. A row's queries travel through one of them (TMA, swizzled) before its
+// first tile; warps 8-11 bring them into tensor memory and give the place back.
+//   scores    warp 0, P V warp 2: issued by one warp in turn, with a question to every barrier between them, the
+//             tensor core stood still for 650 of 2650 cycles a tile;
+//   softmax   warps 4-7, a thread has 16 positions of two heads: a head's maximum and sum are found in four
+//             lanes. All warps still vote whether any head's maximum grew, since a warp that scales O holds all
+//             heads of its dims;
+//   P         K-major [head][position] in shared memory, the B operand of O^T += V^T P^T.
+// 2100 to 2400 cycles a tile at 128 heads (64 x 4096: 96 us); what bounds it is the tensor core's time for 52
+// small instructions a tile, 1080 + 850 cycles, and the loads behind it (without asking the next tile into L2:
+// 101 us). Measured and not kept: the two halves of the scores as buffers of their own (107 against 104 then),
+// queries that the warps read from global memory (1 x 4096: 24 us against 23 then).
+constexpr int kWideG = 64;
+constexpr int kWideStages = 3;
+constexpr uint32_t kWidePOff = kWideStages * kPTileBytes;    // P: [64 heads][64 positions] bf16
+constexpr uint32_t kWideBarOff = kWidePOff + kWideG * 128;
+constexpr int kWideBars = 14 + 3 * kWideStages;
+constexpr uint32_t kWideInfoOff = kWideBarOff + kWideBars * 8 + 8;     // (tensor memory slot and abort flag before it)
+constexpr uint32_t kWideVoteOff = kWideInfoOff + kWideStages * 16;     // [2][4] ints
+constexpr uint32_t kWideMaxOff = kWideVoteOff + 8 * 4;       // factors of O [64], of a finished row [64]
+constexpr uint32_t kWideSmemBytes = kWideMaxOff + 2 * kWideG * 4 + 1024;
+static_assert(kWidePOff % 1024 == 0 && kWideInfoOff % 16 == 0 && kWideMaxOff % 16 == 0, "alignment");
+static_assert(kWideSmemBytes <= 232448, "shared memory budget");
+constexpr uint32_t kWideQCols = 18 * 8;      // columns of half a query row in tensor memory
+
+__global__ void __launch_bounds__(kPThreads, 1) mla_paged_wide_kernel(const __grid_constant__ CUtensorMap tm_qa,
+                                                                      const __grid_constant__ CUtensorMap tm_qp,
+                                                                      const __grid_constant__ CUtensorMap tm_kv,
+                                                                      const __grid_constant__ CUtensorMap tm_pe,
+                                                                      const PagedArgs a) {
+    constexpr int G = kWideG;
+    constexpr uint32_t kTmemS = 4 * G, kTmemQ = kTmemS + kPTile, kTmemCols = 512;
+    static_assert(kTmemQ + kWideQCols <= kTmemCols, "tensor memory");
+    // fp32 accumulate, bf16 x bf16; S: M = 64, N = 64, both K-major; O: V^T MN-major, P K-major, M = 128
+    constexpr uint32_t kSIdesc = (1u << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(kPTile >> 3) << 17) | (4u << 24);
+    constexpr uint32_t kOIdesc = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 15) | (static_cast<uint32_t>(G >> 3) << 17) |
+                                 (8u << 24);
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    uint8_t* base_ptr = smem_raw + (base - smem_u32(smem_raw));
+    const uint32_t bars = base + kWideBarOff;
+    const uint32_t vote = bars, pfull = bars + 8u, pfree = bars + 8u * 2, efull = bars + 8u * 3, odone = bars + 8u * 4,
+                   ofree = bars + 8u * 5, sfull = bars + 8u * 6, sfree = bars + 8u * 7, qfull = bars + 8u * 8, qfree = bars + 8u * 9;
+    auto qland = [&](int s) { return bars + 8u * (10 + s); };      // (two rows' queries may be in the ring)
+    auto qread = [&](int s) { return bars + 8u * (12 + s); };
+    auto kfull = [&](int s) { return bars + 8u * (14 + s); };
+    auto kfree = [&](int s, int half) { return bars + 8u * (14 + kWideStages + 2 * s + half); };
+    // A row of the batch takes one place of the ring for its queries, then one a tile.
+    struct Place {
+        int at = 0;
+        uint32_t parity = 0;
+        __device__ __forceinline__ void next() {
+            if (++at == kWideStages) {
+                at = 0;
+                parity ^= 1u;
+            }
+        }
+    };
+    const uint32_t slot = bars + 8u * kWideBars;
+    volatile uint32_t* slot_ptr = reinterpret_cast<volatile uint32_t*>(base_ptr + kWideBarOff + 8 * kWideBars);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(slot_ptr + 1);
+    volatile TileInfo* info_s = reinterpret_cast<volatile TileInfo*>(base_ptr + kWideInfoOff);
+    volatile int* vote_s = reinterpret_cast<volatile int*>(base_ptr + kWideVoteOff);
+    float* const w_s = reinterpret_cast<float*>(base_ptr + kWideMaxOff);        // what O is multiplied with when maxima grow
+    float* const f_s = w_s + 64;                                             // what a finished row's O is multiplied with
+
+    const int warp = uniform_warp_id(), lane = threadIdx.x & 31;
+    const int groups = (a.heads + G - 1) / G;
+    const int hg = blockIdx.x % groups, range = blockIdx.x / groups;
+
+    if (threadIdx.x == 0) {
+        *abort_flag = 0;
+        for (int s = 0; s < kWideStages; ++s) {
+            mbar_init(kfull(s), 1);
+            mbar_init(kfree(s, 0), 1);
+            mbar_init(kfree(s, 1), 1);
+        }
+        for (int s = 0; s < 2; ++s) {
+            mbar_init(qland(s), 1);
+            mbar_init(qread(s), 4);
+        }
+        mbar_init(qfull, 4);
+        mbar_init(qfree, 1);
+        mbar_init(sfull, 1);
+        mbar_init(sfree, 4);
+        mbar_init(vote, 4);
+        mbar_init(pfull, 4);
+        mbar_init(pfree, 1);
+        mbar_init(efull, 4);
+        mbar_init(odone, 1);
+        mbar_init(ofree, 4);
+        fence_mbar_init();
+        tma_prefetch_desc(&tm_qa);
+        tma_prefetch_desc(&tm_qp);
+        tma_prefetch_desc(&tm_kv);
+        tma_prefetch_desc(&tm_pe);
+    }
+    if (warp == 0) {
+        tmem_alloc(slot, kTmemCols);
+        tmem_relinquish();
+    }
+    const RangeStart start = find_range<kPThreads>(a, range, reinterpret_cast<volatile int*>(w_s));
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem_base = *slot_ptr;
+    const int n_tiles = start.count;
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");     // the join kernel may be set up
+
+    if (warp == 0) {
+        // scores
+        const uint32_t tm = __shfl_sync(0xffffffffu, tmem_base, 0);
+        Place p;
+        p.next();
+        int seg = 0;
+        bool open = false;                                     // the current row's queries have been waited for
+        for (int g = 0; g < n_tiles; ++g) {
+            if (!open && !mbar_wait_warp(qfull, seg & 1, abort_flag, 76)) break;
+            if (!mbar_wait_warp(kfull(p.at), p.parity, abort_flag, 81)) break;
+            const bool last = info_s[p.at].flags & 2;
+            const uint32_t k0 = __shfl_sync(0xffffffffu, ((base + p.at * kPTileBytes) >> 4) | (1u << 16), 0);
+            if (g > 0 && !mbar_wait_warp(sfree, (g - 1) & 1, abort_flag, 80)) break;
+            tc_fence_after();
+            if (elect_one()) {
 #pragma unroll
-                for (int i = 0; i < kCols; ++i) {
-                    const float f = f_s[h + i];
-                    const float v = f == 0.f ? 0.f : __uint_as_float(o[i]) * f;
-                    if (i < live) {
-                        if (part < 0) a.out[at + i * 512] = __float2bfloat16_rn(v);
-                        else a.part_o[at + i * 512] = v;
+                for (int i = 0; i < 36; ++i) {
+                    const uint32_t lanes = i >= 18 ? 16u << 16 : 0u;
+                    const uint64_t k = i < 32 ? smem_desc_at(k0 + 64 * (i >> 2) + 2 * (i & 3), 8192)
+                                              : smem_desc_at(k0 + (kPLatBytes >> 4) + 2 * (i & 3), 1024);
+                    mma_f16_ts(tm + kTmemS + lanes, tm + kTmemQ + lanes + 8u * (i % 18), k, kSIdesc, i % 18 != 0 ? 1u : 0u);
+                }
+                mma_commit(sfull);
+                if (last) mma_commit(qfree);
+            }
+            __syncwarp();
+            open = !last;
+            if (last) {
+                ++seg;
+                p.next();
+            }
+            p.next();
+        }
+    } else if (warp == 2) {
+        // O += P V
+        const uint32_t tm = __shfl_sync(0xffffffffu, tmem_base, 0);
+        const uint32_t p0 = ((base + kWidePOff) >> 4) | (1u << 16);
+        Place p;
+        p.next();
+        int seg = 0;
+        bool open = false;                                     // the row before is out of tensor memory
+        uint32_t acc = 0;
+        for (int g = 0; g < n_tiles; ++g) {
+            if (!mbar_wait_warp(kfull(p.at), p.parity, abort_flag, 79)) break;
+            const uint64_t mask = info_s[p.at].mask;
+            const bool last = info_s[p.at].flags & 2;
+            const uint32_t v0 = __shfl_sync(0xffffffffu, ((base + p.at * kPTileBytes) >> 4) | (64u << 16), 0);
+            if (!open) {
+                if (seg > 0 && !mbar_wait_warp(ofree, (seg - 1) & 1, abort_flag, 78)) break;
+                acc = 0;
+            }
+            if (!mbar_wait_warp(pfull, g & 1, abort_flag, 77)) break;
+            tc_fence_after();
+            if (elect_one()) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    if ((mask >> (16 * j) & 0xffffu) != 0) {
+#pragma unroll
+                        for (int f = 0; f < 4; ++f)
+                            mma_f16(tm + f * G, smem_desc_at(v0 + j * 1024u + f * 128u, 8192),
+                                    smem_desc_at(p0 + 2u * j, 1024), kOIdesc, acc);
+                        acc = 1;
+                    }
+                    if (j & 1) mma_commit(kfree(p.at, j >> 1));            // its positions are done with
+                }
+                mma_commit(pfree);
+                if (last) mma_commit(odone);
+            }
+            __syncwarp();
+            if (mask != 0) acc = 1;
+            open = !last;
+            if (last) {
+                ++seg;
+                p.next();
+            }
+            p.next();
+        }
+    } else if (warp == 1) {
+        // the whole warp walks the range, one thread issues the loads
+        TileWalk w(a, start);
+        const int page = 1 << a.page_log, rows = min(page, kPHalf), boxes = kPTile / rows;    // rows of a box, boxes of a tile
+        if (n_tiles > 0) w.step(a, 0, n_tiles, rows);
+        Place p;
+        p.parity = 1;                                          // (the ring begins free)
+        int segs = 0;
+        for (int g = 0; g < n_tiles; ++g) {
+            bool ok = true;
+            if (w.flags & 1) {
+                const uint32_t dst = base + p.at * kPTileBytes;
+                if (!mbar_wait_warp(kfree(p.at, 0), p.parity, abort_flag, 95)) break;
+                if (!mbar_wait_warp(kfree(p.at, 1), p.parity, abort_flag, 96)) break;
+                if (elect_one()) {
+                    mbar_arrive_expect_tx(qland(segs & 1), G * 1152);
+                    tma_load_4d(dst, &tm_qa, 0, hg * G, 0, w.b, qland(segs & 1));
+                    tma_load_3d(dst + G * 1024, &tm_qp, 0, hg * G, w.b, qland(segs & 1));
+                    mbar_arrive(kfull(p.at));                  // (its phases count all uses of the place)
+                }
+                __syncwarp();
+                ++segs;
+                p.next();
+            }
+            const int st = p.at;
+            const uint32_t dst = base + st * kPTileBytes;
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                if (!(ok = mbar_wait_warp(kfree(st, half), p.parity, abort_flag, 82))) break;
+                if (elect_one()) {
+                    if (half == 0) {
+                        info_s[st].mask = w.mask;
+                        info_s[st].flags = w.flags;
+                        mbar_arrive_expect_tx(kfull(st), kPTileBytes);     // both halves
+                    }
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (i < boxes && i * rows / kPHalf == half) {
+                            const int row = (w.tile * kPTile + i * rows) & (page - 1);
+                            tma_load_5d(dst + i * rows * 1024, &tm_kv, 0, 0, 0, row >> 3, w.id[i], kfull(st));
+                            tma_load_3d(dst + kPLatBytes + i * rows * 128, &tm_pe, 0, row, w.id[i], kfull(st));
+                        }
+                }
+                __syncwarp();
+            }
+            if (!ok) break;
+            p.next();
+            w.advance();
+            if (g + 1 < n_tiles) {
+                // the next tile, whose place in shared memory is still taken, on its way into L2
+                w.step(a, g + 1, n_tiles, rows);
+                if (elect_one()) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (i < boxes && w.id[i] >= 0) {
+                            const int row = (w.tile * kPTile + i * rows) & (page - 1);
+                            tma_prefetch_5d(&tm_kv, 0, 0, 0, row >> 3, w.id[i]);
+                            tma_prefetch_3d(&tm_pe, 0, row, w.id[i]);
+                        }
+                }
+                __syncwarp();
+            }
+        }
+    } else if (warp >= 4 && warp < 8) {
+        const int quad = warp & 3;
+        const uint32_t lane_base = static_cast<uint32_t>(quad * 32) << 16;
+        const int p0 = 2 * (lane & 3);                         // this thread's positions: 8 u + p0 and the next
+        const int h0 = 16 * quad + (lane >> 2);                // its heads within the group: h0 and h0 + 8
+        const float ninf = __int_as_float(0xff800000);
+        uint32_t votes = 0;                                    // phases of `vote` taken
+        // over the four lanes that hold a head's positions
+        auto over_lanes = [&](float v, auto f) {
+            v = f(v, __shfl_xor_sync(0xffffffffu, v, 1));
+            return f(v, __shfl_xor_sync(0xffffffffu, v, 2));
+        };
+        auto larger = [](float u, float w) { return fmaxf(u, w); };
+        auto plus = [](float u, float w) { return u + w; };
+        // lane t: row t % 8 of block t / 8; blocks: heads 0-7 and 8-15 of eight positions, then of the next eight
+        const int st_head = 16 * quad + (lane & 15);
+        const uint32_t st_line = base + kWidePOff + st_head * 128;
+        float l[2], m[2];                                      // denominators (the thread's share), maxima
+        int flags4 = 0, seg = 0;
+        Place p;
+        p.next();
+        for (int g = 0; g < n_tiles; ++g) {
+            const int st = p.at;
+            if (!mbar_wait_warp(kfull(st), p.parity, abort_flag, 84)) break;
+            const uint64_t mask = info_s[st].mask;
+            const int flags = info_s[st].flags;
+            const bool first = flags & 1, last = flags & 2;
+            flags4 = (first ? 0 : flags4) | (flags & 12);
+            if (first) {
+                l[0] = l[1] = 0.f;
+                m[0] = m[1] = ninf;
+            }
+            float x[32], y[32];                                // [8 positions][head, head + 8][2 positions]
+            if (!mbar_wait_warp(sfull, g & 1, abort_flag, 85)) break;
+            tc_fence_after();
+            tmem_ld_16x256b(tmem_base + lane_base + kTmemS, x);
+            tmem_ld_16x256b(tmem_base + lane_base + (16u << 16) + kTmemS, y);
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(sfree);                 // the next tile's may come
+#pragma unroll
+            for (int i = 0; i < 32; ++i) x[i] = (x[i] + y[i]) * a.scale_log2;
+            if (mask != ~0ull) {
+#pragma unroll
+                for (int i = 0; i < 32; ++i)
+                    if (!(mask >> (8 * (i >> 2) + p0 + (i & 1)) & 1)) x[i] = ninf;
+            }
+            float top[2] = {ninf, ninf};
+#pragma unroll
+            for (int i = 0; i < 32; ++i) top[i >> 1 & 1] = fmaxf(top[i >> 1 & 1], x[i]);
+            // (false while a top is -infinity)
+            bool over = top[0] > m[0] + 8.f || top[1] > m[1] + 8.f;
+            over = __any_sync(0xffffffffu, over);
+            if (!first) {
+                // does any head's maximum grow: what the others found comes in while new maxima are found
+                if (lane == 0) {
+                    vote_s[(g & 1) * 4 + quad] = over ? 1 : 0;
+                    mbar_arrive(vote);
+                }
+            }
+            float w[2] = {1.f, 1.f};
+            if (over) {
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                    const float mt = over_lanes(top[r], larger);
+                    if (mt > m[r] + 8.f) {
+                        w[r] = exp2_fast(m[r] - mt);
+                        m[r] = mt;
+                        l[r] *= w[r];
                     }
                 }
             }
+            const float mu0 = m[0] == ninf ? 0.f : m[0], mu1 = m[1] == ninf ? 0.f : m[1];
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+                x[i] = exp2_fast(x[i] - ((i & 2) ? mu1 : mu0));
+                l[i >> 1 & 1] += x[i];
+            }
+            bool grown = false;
+            if (!first) {
+                if (!mbar_wait_warp(vote, votes++ & 1, abort_flag, 86)) break;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) grown |= vote_s[(g & 1) * 4 + i] != 0;
+                // (all warps vote on this tile, so none reads the factors of one before)
+                if (grown && (lane & 3) == 0) {
+                    w_s[h0] = w[0];
+                    w_s[h0 + 8] = w[1];
+                }
+            }
+            // rows of a step that is multiplied, but not visible: zeros
+            const uint32_t step = static_cast<uint32_t>(mask >> (16 * quad)) & 0xffffu;
+            if (step != 0 && step != 0xffffu) {
+                uint8_t* kt = base_ptr + st * kPTileBytes + quad * 16384;
+                for (uint32_t z = ~step & 0xffffu; z; z &= z - 1) {
+                    const int row = __ffs(static_cast<int>(z)) - 1;
+#pragma unroll
+                    for (int i = 0; i < 2; ++i)
+                        *reinterpret_cast<uint4*>(kt + (row >> 3) * 8192 + ((lane >> 3) + 4 * i) * 1024 + (row & 7) * 128 +
+                                                  (lane & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
+                }
+            }
+            if (g > 0) {
+                // O += P V of the tile before has retired: P may be overwritten, O is at rest
+                if (!mbar_wait_warp(pfree, (g - 1) & 1, abort_flag, 87)) break;
+                tc_fence_after();
+            }
+            if (grown) {
+                __syncwarp();
+                if (lane == 0) mbar_arrive(vote);              // the factors are written
+                if (!mbar_wait_warp(vote, votes++ & 1, abort_flag, 90)) break;
+                rescale<G>(tmem_base + lane_base, w_s);
+            }
+#pragma unroll
+            for (int u = 0; u < 8; u += 2)
+                stmatrix_x4(st_line + (((u + (lane >> 4)) ^ (st_head & 7)) << 4), pack_bf16x2(x[4 * u], x[4 * u + 1]),
+                            pack_bf16x2(x[4 * u + 2], x[4 * u + 3]), pack_bf16x2(x[4 * u + 4], x[4 * u + 5]),
+                            pack_bf16x2(x[4 * u + 6], x[4 * u + 7]));
+            fence_proxy_async();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(pfull);
+            if (last) {
+                // the row before has been written, so its factors may go
+                if (seg > 0 && !mbar_wait_warp(ofree, (seg - 1) & 1, abort_flag, 93)) break;
+                const int part = part_slot(flags4, range);
+                // a head's denominator, and what O is multiplied with (0 for a head of no weight at all, every page
+                // out of the pool or every score -infinity: it is zero)
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                    const float den = over_lanes(l[r], plus);
+                    const int h = h0 + 8 * r;
+                    if ((lane & 3) == 0) {
+                        if (part >= 0 && hg * G + h < a.heads)
+                            *reinterpret_cast<float2*>(a.part_ml + (static_cast<int64_t>(part) * a.heads + hg * G + h) * 2) =
+                                make_float2(den == 0.f ? ninf : m[r], den);
+                        f_s[h] = den == 0.f ? 0.f : part < 0 ? 1.f / den : 1.f;
+                    }
+                }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(efull);
+                ++seg;
+                p.next();
+            }
+            p.next();
+        }
+    } else if (warp >= 8) {
+        // queries into tensor memory, and finished rows out of it while the next row's first tile is on its way
+        const int quad = warp & 3;
+        const uint32_t lane_base = static_cast<uint32_t>(quad * 32) << 16;
+        int b = start.row, j = start.tile, segs = 0;
+        RowTiles t = n_tiles > 0 ? slot_tiles(a, start.slot) : RowTiles{};
+        Place p;
+        // lanes 0-15: dims 0-287 of 16 heads, lanes 16-31: dims 288-511 and the rope's
+        auto load_queries = [&] {
+            if (!mbar_wait_warp(qland(segs & 1), segs >> 1 & 1, abort_flag, 97)) return false;
+            const uint32_t head = 16 * quad + (lane & 15);
+            const uint8_t* line = base_ptr + p.at * kPTileBytes + head * 128;      // of the first block of 64 dims
+            const uint32_t first = lane < 16 ? 0 : 36;
+            if (segs > 0 && !mbar_wait_warp(qfree, (segs - 1) & 1, abort_flag, 83)) return false;
+            tc_fence_after();
+#pragma unroll
+            for (int c = 0; c < 36; c += 4) {
+                uint32_t r[16];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const uint32_t piece = first + c + i;
+                    const uint4 v = *reinterpret_cast<const uint4*>(line + (piece >> 3) * (G * 128) + (((piece ^ head) & 7) << 4));
+                    r[4 * i] = v.x;
+                    r[4 * i + 1] = v.y;
+                    r[4 * i + 2] = v.z;
+                    r[4 * i + 3] = v.w;
+                }
+                tmem_st_32x16(tmem_base + lane_base + kTmemQ + 4 * c, r);
+            }
+            tmem_st_wait();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) {
+                mbar_arrive(qread(segs & 1));
+                mbar_arrive(qfull);
+            }
+            if (warp == 8) {                                   // the place is free for a tile
+                if (!mbar_wait_warp(qread(segs & 1), segs >> 1 & 1, abort_flag, 98)) return false;
+                if (lane == 0) {
+                    mbar_arrive(kfree(p.at, 0));
+                    mbar_arrive(kfree(p.at, 1));
+                }
+            }
+            p.next();
+            ++segs;
+            return true;
+        };
+        bool ok = n_tiles == 0 || load_queries();
+        if (hg == 0) clear_empty_rows(a, range);
+        for (int seg = 0, left = n_tiles; ok && left > 0; ++seg) {
+            const int row = b, tiles = min(t.n - j, left);
+            const int part = part_slot((j == 0 ? 4 : 0) | (j + tiles == t.n ? 8 : 0), range);
+            left -= tiles;
+            j = 0;
+            if (left > 0) {
+                do t = row_tiles(a, ++b);
+                while (t.n == 0);
+                for (int i = 0; i < tiles; ++i) p.next();
+                if (!(ok = load_queries())) break;
+            }
+            if (!(ok = mbar_wait_warp(efull, seg & 1, abort_flag, 94))) break;
+            if (!(ok = mbar_wait_warp(odone, seg & 1, abort_flag, 88))) break;
+            tc_fence_after();
+            write_row<G>(a, part, row, hg * G, tmem_base + lane_base, f_s);
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(ofree);
@@ -878,7 +1389,7 @@ int paged_attn_error_take() {
 // Heads of a CTA (the fewest groups, then the narrowest that holds its share), and the ranges that the tiles
 // are cut into.
 static int paged_group(int64_t heads) {
-    const int64_t groups = (heads + kPMaxG - 1) / kPMaxG, share = (heads + groups - 1) / groups;
+    const int64_t groups = (heads + kWideG - 1) / kWideG, share = (heads + groups - 1) / groups;
     return share <= 16 ? 16 : share <= 32 ? 32 : 64;
 }
 static int paged_ranges(int64_t heads) {
@@ -887,15 +1398,13 @@ static int paged_ranges(int64_t heads) {
     return static_cast<int>(r < 1 ? 1 : r < kJoinMaxParts ? r : kJoinMaxParts);
 }
 
-template <int G>
-static int launch_paged(const CUtensorMap& tm_qa, const CUtensorMap& tm_qp, const CUtensorMap& tm_kv,
+static int launch_paged(int group, const CUtensorMap& tm_qa, const CUtensorMap& tm_qp, const CUtensorMap& tm_kv,
                         const CUtensorMap& tm_pe, const PagedArgs& a, cudaStream_t s) {
-    if (int rc = ensure_dynamic_smem(reinterpret_cast<const void*>(&mla_paged_kernel<G>), static_cast<int>(kPSmemBytes),
-                                     "rt_mla_paged_decode"))
-        return rc;
-    const int groups = (a.heads + G - 1) / G;
-    mla_paged_kernel<G><<<static_cast<unsigned>(a.n_ranges * groups), kPThreads, kPSmemBytes, s>>>(tm_qa, tm_qp, tm_kv,
-                                                                                                    tm_pe, a);
+    auto* kernel = group == 16 ? &mla_paged_kernel<16> : group == 32 ? &mla_paged_kernel<32> : &mla_paged_wide_kernel;
+    const int smem = static_cast<int>(group == kWideG ? kWideSmemBytes : kPSmemBytes);
+    if (int rc = ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), smem, "rt_mla_paged_decode")) return rc;
+    const int groups = (a.heads + group - 1) / group;
+    kernel<<<static_cast<unsigned>(a.n_ranges * groups), kPThreads, smem, s>>>(tm_qa, tm_qp, tm_kv, tm_pe, a);
     count_launch();
     return check_launch("mla_paged_kernel");
 }
@@ -985,10 +1494,7 @@ extern "C" int rt_mla_paged_decode(const void* q_abs, const void* q_pe, const vo
         if (int rc = tc::make_tmap_bf16(&tm_pe, pe, 3, dims, st, box)) return rc;
     }
     cudaStream_t s = as_stream(stream);
-    if (int rc = group == 16   ? tc::launch_paged<16>(tm_qa, tm_qp, tm_kv, tm_pe, a, s)
-                 : group == 32 ? tc::launch_paged<32>(tm_qa, tm_qp, tm_kv, tm_pe, a, s)
-                               : tc::launch_paged<64>(tm_qa, tm_qp, tm_kv, tm_pe, a, s))
-        return rc;
+    if (int rc = tc::launch_paged(group, tm_qa, tm_qp, tm_kv, tm_pe, a, s)) return rc;
     if (a.n_ranges == 1) return RT_OK;
     dim3 grid(static_cast<unsigned>(heads), static_cast<unsigned>(a.n_ranges - 1));
     // launched while the last CTAs of the kernel before still run; it waits for their parts itself
