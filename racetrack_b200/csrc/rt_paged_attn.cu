@@ -10,13 +10,14 @@
 // A row of 1152 bytes serves 2 * 1088 flops for each head, 242 flop/B at 128 heads: with few heads the
 // kernel is bound by reading the cache once, with all of them memory and tensor cores take about the same.
 // Measured on one B200, kernels and join, calls in a row on inputs of three sets (copy rate 6546 GB/s):
-//   16 heads, 48 sequences of up to 32768 (0.56 GB)  97 us, 5740 GB/s; 64 of 4096 (0.30 GB) 60 us
-//   32 heads, 128 under a window of 1024 (0.11 GB)   40 us; 64 of 4096 67 us
-//   128 heads, 64 of 4096                            96 us, 760 TFLOP/s; 64 heads 75 us
-//   one sequence of 17 positions, 16 heads           10 us; of 131072 41 us
+//   16 heads, 48 sequences of up to 32768 (0.56 GB)  96 us, 5800 GB/s; 64 of 4096 (0.30 GB) 58 us
+//   32 heads, 128 under a window of 1024 (0.11 GB)   38 us; 64 of 4096 65 us
+//   128 heads, 64 of 4096                            92 us, 790 TFLOP/s; 64 heads 69.5 us
+//   one sequence of 17 positions, 16 heads           8.7 us; of 131072 37 us
 // Two kernels share the walk over the tiles and the join. mla_paged_kernel serves groups of up to 32 heads,
-// mla_paged_wide_kernel of 64; each served all groups once: the first takes 124 us for 64 x 4096 at 128 heads
-// (80 at 64), the second 45 for the window's case and 100 for the ragged one.
+// mla_paged_wide_kernel of 64; each served all groups once, with an earlier join: the first takes 124 us for
+// 64 x 4096 at 128 heads where the second took 97 (80 and 75 at 64), the second 44 for the window's case and 99
+// for the ragged one where the first took 40 and 97.
 #include "rt_tc.cuh"
 
 namespace rt {
@@ -477,7 +478,6 @@ __global__ void __launch_bounds__(kPThreads, 1) mla_paged_kernel(const __grid_co
     tc_fence_after();
     const uint32_t tmem_base = *slot_ptr;
     const int n_tiles = start.count;
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");     // the join kernel may be set up
 
     if (warp == 0) {
         if (n_tiles > 0 && elect_one()) {
@@ -806,6 +806,7 @@ __global__ void __launch_bounds__(kPThreads, 1) mla_paged_kernel(const __grid_co
     }
     tc_fence_before();
     __syncthreads();
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");     // the join kernel may be set up
     if (warp == 0) {
         tc_fence_after();
         tmem_dealloc(tmem_base, kTmemCols);
@@ -827,10 +828,12 @@ __global__ void __launch_bounds__(kPThreads, 1) mla_paged_kernel(const __grid_co
 //             lanes. All warps still vote whether any head's maximum grew, since a warp that scales O holds all
 //             heads of its dims;
 //   P         K-major [head][position] in shared memory, the B operand of O^T += V^T P^T.
-// 2100 to 2400 cycles a tile at 128 heads (64 x 4096: 96 us); what bounds it is the tensor core's time for 52
-// small instructions a tile, 1080 + 850 cycles, and the loads behind it (without asking the next tile into L2:
-// 101 us). Measured and not kept: the two halves of the scores as buffers of their own (107 against 104 then),
-// queries that the warps read from global memory (1 x 4096: 24 us against 23 then).
+// 2100 to 2400 cycles a tile at 128 heads, kernel alone 85 to 90 us for 64 x 4096 where the first form takes 117. The
+// tensor core is busy for 63 % of them; the rest is the way of the scores (36 instructions of 29 cycles, 450 until
+// they are seen, 265 to read them, 250 until the next may begin: one buffer is all that tensor memory holds)
+// and loads behind it (without asking the next tile into L2: 4 us more). Measured and not kept: the scores'
+// halves as buffers of their own (4 us more), eight softmax warps (4 us more, with both 18), the halves' instructions
+// in turn (no difference), queries read from global memory by the warps (1 x 4096: 1 us more).
 constexpr int kWideG = 64;
 constexpr int kWideStages = 3;
 constexpr uint32_t kWidePOff = kWideStages * kPTileBytes;    // P: [64 heads][64 positions] bf16
@@ -926,7 +929,6 @@ __global__ void __launch_bounds__(kPThreads, 1) mla_paged_wide_kernel(const __gr
     tc_fence_after();
     const uint32_t tmem_base = *slot_ptr;
     const int n_tiles = start.count;
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");     // the join kernel may be set up
 
     if (warp == 0) {
         // scores
@@ -1284,6 +1286,7 @@ __global__ void __launch_bounds__(kPThreads, 1) mla_paged_wide_kernel(const __gr
     }
     tc_fence_before();
     __syncthreads();
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");     // the join kernel may be set up
     if (warp == 0) {
         tc_fence_after();
         tmem_dealloc(tmem_base, kTmemCols);
@@ -1291,82 +1294,100 @@ __global__ void __launch_bounds__(kPThreads, 1) mla_paged_wide_kernel(const __gr
 }
 
 // Joins the parts of every row that crosses ranges: out = sum_s o_s 2^(m_s - M) / sum_s l_s 2^(m_s - M). A row
-// of P parts crosses P - 1 range borders, and blockIdx.y + 1 is a range, so the row has P - 1 blocks a head:
-// the first S of them (a power of two, at most 16) take 512 / S dims each, with S groups of threads that sum
-// every S-th part; the groups' sums are added in order, so the result does not depend on timing. A row
-// that is cut once is one block of 128 threads, one cut 147 times is 16 blocks of 16 x 8.
+// of P parts crosses P - 1 range borders, and blockIdx.x + 1 is a range, so the row has P - 1 blocks: the first S of
+// them (the largest power of two, at most 64) take 512 / S dims each. A warp has one head: its lanes cover the
+// dims with one, two or four pieces of four, and beyond S = 4 they are S / 4 groups that sum every S / 4-th part.
+// So a lane has at most eight pieces of parts to read (P up to 128), all under way at once, whether a row is
+// cut once or 127 times; the groups' sums are added in order, so the result does not depend on timing.
+// Measured with the kernel before it: 64 x 4096 at 64 heads 69.5 us, at 128 92; 1 x 4096 at 128 heads 17.9, at 16 11.4;
+// 1 x 131072 37.4. Blocks of one head and slice that met twice at a barrier took 75.6, 97, 20.5, 10.8 and 40.6; blocks that
+// walk several heads 78.8 and 98. The kernel before lets this one's blocks in when a CTA of it has finished: let
+// in from the start they fill the first SMs that come free and work there side by side (1 x 131072 40.7 us).
 constexpr int kJoinThreads = 128;
 constexpr int kJoinMaxParts = 160;
 __global__ void __launch_bounds__(kJoinThreads) mla_paged_join_kernel(const PagedArgs a) {
     asm volatile("griddepcontrol.wait;" ::: "memory");        // the parts are complete
-    const int r = blockIdx.y + 1, head = blockIdx.x;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int r = blockIdx.x + 1, head = blockIdx.y * (kJoinThreads / 32) + warp;
     const int4 rg = a.ranges[r];
-    if (rg.x < 0 || rg.y == 0) return;
+    if (rg.x < 0 || rg.y == 0 || head >= a.heads) return;
     const int per = rg.w, t0 = r * per - rg.y, r0 = t0 / per, r1 = (t0 + rg.z - 1) / per, parts = r1 - r0 + 1;
-    const int slices = 1 << min(4, 31 - __clz(parts - 1)), slice = r - r0 - 1;
-    if (slice >= slices) return;
-    __shared__ float w_s[kJoinMaxParts], red[4][2];
-    __shared__ float4 acc_s[kJoinThreads];
+    const int log_s = min(6, 31 - __clz(parts - 1)), slice = r - r0 - 1;
+    if (slice >> log_s) return;
+    __shared__ float w_all[kJoinThreads / 32][kJoinMaxParts];
+    float* const w_s = w_all[warp];
     const float ninf = __int_as_float(0xff800000);
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     auto row_of = [&](int s) { return static_cast<int64_t>(s == 0 ? 2 * r0 + 1 : 2 * (r0 + s)) * a.heads + head; };
-    const int wide = 128 / slices, c = slice * wide + (tid & (wide - 1)), q = tid / wide;
-    // the first parts' sums are under way while the weights are found
-    float4 o[4];
+    // pieces of a lane and lanes of a group; the lane's first piece and its group
+    const int log_p = max(0, 2 - log_s), log_w = min(5, 7 - log_s), groups = 32 >> log_w;
+    const int c = (slice << (7 - log_s)) + (lane & ((1 << log_w) - 1)), q = lane >> log_w;
+    auto part_of = [&](int i, int s0) {                        // load i: piece i % pieces of part s0 + (i / pieces) * groups
+        const int s = min(s0 + (i >> log_p) * groups, parts - 1);
+        return *(reinterpret_cast<const float4*>(a.part_o + row_of(s) * 512) + c + ((i & ((1 << log_p) - 1)) << 5));
+    };
+    float4 o[8];
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-        o[i] = *(reinterpret_cast<const float4*>(a.part_o + row_of(min(q + i * slices, parts - 1)) * 512) + c);
-    float2 ml[2];
+    for (int i = 0; i < 8; ++i) o[i] = part_of(i, q);
+    float2 ml[kJoinMaxParts / 32];
+    float m = ninf;
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const int s = tid + i * kJoinThreads;
+    for (int i = 0; i < kJoinMaxParts / 32; ++i) {
+        const int s = lane + 32 * i;
         ml[i] = s < parts ? *reinterpret_cast<const float2*>(a.part_ml + row_of(s) * 2) : make_float2(ninf, 0.f);
+        m = fmaxf(m, ml[i].x);
     }
-    float m = warp_max(fmaxf(ml[0].x, ml[1].x));
-    if (lane == 0) red[warp][0] = m;
-    __syncthreads();
-    m = fmaxf(fmaxf(red[0][0], red[1][0]), fmaxf(red[2][0], red[3][0]));
+    m = warp_max(m);
     float den = 0.f;
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < kJoinMaxParts / 32; ++i) {
         // a part without a maximum has no weight, or (NaN scores alone) NaN
         const float w = ml[i].x == ninf ? (ml[i].y != 0.f ? ml[i].y : 0.f) : exp2f(ml[i].x - m);
-        const int s = tid + i * kJoinThreads;
-        if (s < parts) w_s[s] = w;
+        if (lane + 32 * i < parts) w_s[lane + 32 * i] = w;
         den += ml[i].y * w;
     }
     den = warp_sum(den);
-    if (lane == 0) red[warp][1] = den;
-    __syncthreads();
-    den = (red[0][1] + red[1][1]) + (red[2][1] + red[3][1]);
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int s0 = q; s0 < parts; s0 += 4 * slices) {
+    __syncwarp();
+    float4 acc[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) acc[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+    const int step = groups << (3 - log_p);                    // parts of a round
+    for (int s0 = q; s0 < parts; s0 += step) {
         if (s0 != q) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-                o[i] = *(reinterpret_cast<const float4*>(a.part_o + row_of(min(s0 + i * slices, parts - 1)) * 512) + c);
+            for (int i = 0; i < 8; ++i) o[i] = part_of(i, s0);
         }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            if (s0 + i * slices < parts) {
-                const float w = w_s[s0 + i * slices];
-                acc.x += o[i].x * w; acc.y += o[i].y * w; acc.z += o[i].z * w; acc.w += o[i].w * w;
+        auto add = [&](float4& to, int i) {
+            const int s = s0 + (i >> log_p) * groups;
+            if (s < parts) {
+                const float w = w_s[s];
+                to.x += o[i].x * w; to.y += o[i].y * w; to.z += o[i].z * w; to.w += o[i].w * w;
             }
+        };
+        if (log_p == 0) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) add(acc[0], i);
+        } else if (log_p == 1) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) add(acc[i & 1], i);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) add(acc[i & 3], i);
         }
     }
-    if (slices > 1) {
-        acc_s[tid] = acc;
-        __syncthreads();
-        if (q != 0) return;
-        for (int i = 1; i < slices; ++i) {
-            const float4 v = acc_s[tid + i * wide];
-            acc.x += v.x; acc.y += v.y; acc.z += v.z; acc.w += v.w;
-        }
+    for (int b = 1 << log_w; b < 32; b <<= 1) {
+        acc[0].x += __shfl_xor_sync(0xffffffffu, acc[0].x, b);
+        acc[0].y += __shfl_xor_sync(0xffffffffu, acc[0].y, b);
+        acc[0].z += __shfl_xor_sync(0xffffffffu, acc[0].z, b);
+        acc[0].w += __shfl_xor_sync(0xffffffffu, acc[0].w, b);
     }
+    if (q != 0) return;
     const float inv = 1.f / den;
-    uint2 v = make_uint2(pack_bf16x2(acc.x * inv, acc.y * inv), pack_bf16x2(acc.z * inv, acc.w * inv));
-    if (den == 0.f) v = make_uint2(0u, 0u);
-    *reinterpret_cast<uint2*>(a.out + (static_cast<int64_t>(rg.x) * a.heads + head) * 512 + c * 4) = v;
+    uint2* const to = reinterpret_cast<uint2*>(a.out + (static_cast<int64_t>(rg.x) * a.heads + head) * 512) + c;
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+        if (k >> log_p == 0)
+            to[32 * k] = den == 0.f ? make_uint2(0u, 0u) : make_uint2(pack_bf16x2(acc[k].x * inv, acc[k].y * inv),
+                                                                    pack_bf16x2(acc[k].z * inv, acc[k].w * inv));
 }
 
 int sm_count();                                      // rt_gemm.cu
@@ -1496,7 +1517,7 @@ extern "C" int rt_mla_paged_decode(const void* q_abs, const void* q_pe, const vo
     cudaStream_t s = as_stream(stream);
     if (int rc = tc::launch_paged(group, tm_qa, tm_qp, tm_kv, tm_pe, a, s)) return rc;
     if (a.n_ranges == 1) return RT_OK;
-    dim3 grid(static_cast<unsigned>(heads), static_cast<unsigned>(a.n_ranges - 1));
+    dim3 grid(static_cast<unsigned>(a.n_ranges - 1), static_cast<unsigned>((heads + 3) / 4));
     // launched while the last CTAs of the kernel before still run; it waits for their parts itself
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = grid;
