@@ -698,7 +698,7 @@ int rt_page_extend(int32_t* table, int64_t table_stride, int32_t* lens, int32_t*
                    void* stream);
 
 /* Row t of rows[b] (row_strides[b] bytes apart) goes to slots[t] of buffer b; slots outside the pool are
- * skipped. */
+ * skipped, and none may be named twice: the order is not defined. */
 int rt_page_write(void* const* bases, const int64_t* page_strides, const int64_t* row_bytes,
                   const void* const* rows, const int64_t* row_strides, int64_t n_buffers,
                   const int32_t* slots, int64_t tokens, int64_t pages, int64_t page_size, void* stream);

@@ -528,8 +528,8 @@ def page_extend(block_table: torch.Tensor, seq_lens: torch.Tensor, refcount: tor
 
 
 def page_write(pages, rows, slots: torch.Tensor) -> None:
-    """rows[b][t] into row slots[t] of every buffer pages[b]; slots outside the pool are skipped.
-    rows[b] is [tokens, ...] of the buffer's type, its rows at any pitch."""
+    """rows[b][t] into row slots[t] of every buffer pages[b]; slots outside the pool are skipped, and none inside
+    is named twice. rows[b] is [tokens, ...] of the buffer's type, its rows at any pitch."""
     _native().page_write(list(pages), list(rows), slots)
 
 
