@@ -1481,6 +1481,9 @@ extern "C" int rt_mla_paged_decode(const void* q_abs, const void* q_pe, const vo
     a.scale_log2 = softmax_scale * 1.4426950408889634f;
     const int group = tc::paged_group(heads);
     a.n_ranges = tc::paged_ranges(heads);
+    // (the host knows no length, but what the table holds at most: fewer tiles than CTAs leave the join less to look
+    // at, one tile nothing; 1 x 4096 in a table of 64 pages 11.5 -> 11.0 us at 16 heads)
+    if (a.n_ranges > batch * tiles) a.n_ranges = batch * tiles > 0 ? static_cast<int>(batch * tiles) : 1;
     a.ranges = static_cast<int4*>(workspace);
     a.part_ml = reinterpret_cast<float*>(a.ranges + a.n_ranges);
     a.part_o = a.part_ml + 2ll * a.n_ranges * heads * 2;

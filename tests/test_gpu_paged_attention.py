@@ -162,6 +162,17 @@ def test_nothing_to_attend_to(heads):
     assert not got.any()
 
 
+@pytest.mark.parametrize("heads", [16, 128])
+@pytest.mark.parametrize("page, width", [(16, 1), (64, 1), (64, 2), (128, 1), (16, 9)])
+@pytest.mark.parametrize("length", [0, 1, 15, 16])
+def test_tables_of_few_tiles(heads, page, width, length):
+    """Less than a CTA each: with one tile there is nothing to join."""
+    lengths = [length if width == 1 else length * page * width // 16]
+    kv, pe, table, q_abs, q_pe = make(lengths, heads, page, width=width, seed=length)
+    got = ops.mla_paged_decode(q_abs, q_pe, kv, pe, ints(table), ints(lengths), SCALE)
+    check(got, kv, pe, table, lengths, q_abs, q_pe)
+
+
 def test_lengths_beyond_the_table_are_cut():
     lengths = [128, 64]
     kv, pe, table, q_abs, q_pe = make(lengths, 16, 64, width=2)
