@@ -154,9 +154,9 @@ __device__ RangeStart find_range(const PagedArgs& a, int range, volatile int* sc
 //             rows as [8-row groups][8 blocks of 64 dims][8 rows][128 B] (128-byte swizzle), one the rope keys: a
 //             page of any size lands in the same layout, of which both products read their operand (the group
 //             stride is a field of the descriptor), so the rows are staged once. Two tiles are staged (144 KB);
-//             the one behind them is asked into L2 (without: 64 x 4096 x 128 heads 128 us instead of 123, ragged
-//             104 instead of 99; two or three tiles ahead are no better). Boxes of half or a quarter of the dims
-//             instead of the positions: 134 and 142 us;
+//             the one behind them is asked into L2 (the ragged batch above 99 us, without 104; two tiles ahead
+//             101, three 105). Boxes of half or a quarter of the dims instead of the positions: 64 x 4096 x 128
+//             heads, when this kernel served them, 134 and 142 us instead of 125;
 //   S = K Q^T 36 tcgen05.mma (M = 64 positions, N = G heads, K = 16 dims), both K-major;
 //   softmax   warps 4-7. An M = 64 product lies in lanes 0-15 of each quarter of tensor memory; read in 16 x 256
 //             bit blocks a thread holds two positions of G / 4 heads, so all lanes work. The maxima change only
