@@ -753,7 +753,7 @@ int rt_page_copy(void* const* bases, const int64_t* page_strides, const int64_t*
  * one rope key per token shared by all heads (MLA: the k_pe broadcast of the reference's
  * torch.cat is never materialised); rope_dim == 0 means the key is k_nope alone (k_pe may be
  * NULL). fp32 scores / softmax / accumulation, probabilities rounded to bf16 before they
- * multiply v, as the reference's probs.to(v.dtype).
+ * multiply v, as the reference's probs.to(v.dtype). softmax_scale: of either sign, or 0.
  * nope_dim <= 128, rope_dim <= 64, v_dim <= 128, each a multiple of 8.
  * ref: racetrack/runtime/torch_ops.py:97-110 (causal_attention),
  *      racetrack/realistic_bench.py:304-313 (q / k / v of the synthetic layer),

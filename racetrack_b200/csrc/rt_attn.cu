@@ -539,7 +539,8 @@ struct PrefillArgs {
     int v_dim;
     int one_op;                  // bit i set: operand i (q_nope, q_pe, k_nope, k_pe, v) arrives as ONE box
     int pe_shared;               // k_pe has one row per token for all heads
-    float scale_log2;
+    float scale_log2;            // 0 or more; hidden scores are -infinity before they meet it
+    float sign;                  // 1, or what signed_scores multiplies the scores with first
     // optional (v_dim 128): the output as act_quant leaves it, FP8 e4m3 codes
     // [tokens, heads * 128] and one fp32 scale per token and head (= per 128-wide group)
     uint8_t* out_codes;
@@ -623,6 +624,18 @@ __device__ __forceinline__ void softmax_chunk(const uint32_t (&r)[32], uint32_t 
         }
         sum[i & 1] = add_f32x2(sum[i & 1], pack_f32x2(p0, p1));
         pk[i] = pack_bf16x2(p0, p1);
+    }
+}
+
+// The kernels hide a score by -infinity and take a row's maximum before the scale, so the scale they use is
+// positive: a negative one gives its sign to the scores, and 0 (of which -infinity would make NaN) makes them 0 and
+// leaves 1 as the scale. Behind one uniform branch: a call with a positive scale skips the 64 products.
+__device__ __forceinline__ void signed_scores(float sign, uint32_t (&r0)[32], uint32_t (&r1)[32]) {
+    if (sign == 1.f) return;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) {
+        r0[i] = __float_as_uint(__uint_as_float(r0[i]) * sign);
+        r1[i] = __float_as_uint(__uint_as_float(r1[i]) * sign);
     }
 }
 
@@ -846,6 +859,7 @@ __global__ void __launch_bounds__(kFThreads, 1) attn_prefill_kernel(
             tmem_ld_wait(r0);
             tmem_ld_wait(r1);
             if (threadIdx.x == 64) RT_FTRACE(7, j);
+            signed_scores(a.sign, r0, r1);
             if constexpr (kWindow) {
                 const int k0 = 128 * key_tile(j), r0_abs = q0 + 128 * t;
                 if (j == n_t - 1 || !(k0 > r0_abs + 127 - a.window || k0 + 127 < a.sinks)) {
@@ -1232,6 +1246,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFThreads, 1) attn_p
             __syncwarp();
             if (lane == 0) mbar_arrive_cluster(s_free_leader);
             if (threadIdx.x == 64) RT_FTRACE(7, j);
+            signed_scores(a.sign, r0, r1);
             if (j == n - 1) {                                 // diagonal tile: keys beyond the row's own are masked
                 const int c0 = 64 * cq;
 #pragma unroll
@@ -1660,7 +1675,8 @@ static int attn_causal_prefill(const void* q, const void* k_nope, const void* k_
     a.cv = static_cast<int>((v_dim + 63) / 64);
     a.v_dim = static_cast<int>(v_dim);
     a.pe_shared = pe_shared ? 1 : 0;
-    a.scale_log2 = softmax_scale * 1.4426950408889634f;
+    a.sign = softmax_scale < 0.f ? -1.f : softmax_scale == 0.f ? 0.f : 1.f;
+    a.scale_log2 = softmax_scale == 0.f ? 1.f : fabsf(softmax_scale) * 1.4426950408889634f;
     a.out_codes = static_cast<uint8_t*>(out_codes);
     a.out_scales = out_scales;
     if (window >= tokens) window = 0;                  // every query sees all keys before it

@@ -593,7 +593,8 @@ def attention_prefill(q: torch.Tensor, k_nope: torch.Tensor, k_pe: Optional[torc
     racetrack/realistic_bench.py:304-313): q bf16 [T, H, nope + rope]; the key of head h is
     [k_nope[:, h] | k_pe] with k_nope [T, H, nope] and k_pe [T, rope] (one rope key per token for
     all heads, never broadcast in memory) or [T, H, rope], or None; v [T, H, v_dim]. Operands may
-    be strided views (column slices of projection outputs). Returns bf16 [T, H, v_dim].
+    be strided views (column slices of projection outputs). softmax_scale: (nope + rope) ** -0.5 by
+    default, of either sign or 0. Returns bf16 [T, H, v_dim].
 
     quantized=True returns act_quant of that output instead, (FP8 codes [T, H * v_dim], fp32 scales
     [T, H]), bit for bit what fused_act_quant makes of it; for the 128 + 64 / 128 head shape the

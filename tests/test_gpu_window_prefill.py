@@ -171,3 +171,34 @@ def test_what_is_refused(kw, says):
     q, kn, kp, v = inputs(20, 2, 5)
     with pytest.raises(RuntimeError, match=says):
         ops.attention_prefill(q, kn, kp, v, **kw)
+
+
+@pytest.mark.parametrize("scale", [-192 ** -0.5, -0.3, 0.0, -0.0])
+@pytest.mark.parametrize("tokens, heads, window, sinks", [(300, 2, 100, 3), (300, 60, 100, 3), (300, 60, 30, 140)])
+def test_scales_that_are_not_positive(tokens, heads, window, sinks, scale):
+    """A negative scale turns the order of the scores, 0 weighs what is seen alike; 2 and 60 heads are the two
+    tilings. Hidden keys weigh nothing, NaN included."""
+    q, kn, kp, v = inputs(tokens, heads, 11)
+    got = ops.attention_prefill(q, kn, kp, v, scale, window=window, sinks=sinks)
+    check(got, q, kn, kp, v, window, sinks, scale)
+    at = 200
+    kn2 = kn.clone()
+    kn2[at] = float("nan")
+    blind = ~seen(tokens, window, sinks)[:, at]
+    again = ops.attention_prefill(q, kn2, kp, v, scale, window=window, sinks=sinks)
+    assert torch.equal(again[blind].view(torch.int16), got[blind].view(torch.int16))
+    codes, scales = ops.attention_prefill(q, kn, kp, v, scale, window=window, sinks=sinks, quantized=True)
+    want, want_scales = ops.fused_act_quant(got.view(tokens, -1))
+    assert torch.equal(codes.view(torch.uint8), want.view(torch.uint8)) and torch.equal(scales, want_scales)
+
+
+@pytest.mark.parametrize("scale", [-192 ** -0.5, -0.3, 0.0])
+@pytest.mark.parametrize("schedule", [1, 2])
+def test_scales_that_are_not_positive_without_a_window(schedule, scale):
+    q, kn, kp, v = inputs(300, 3, 12)
+    previous = ops.attention_prefill_schedule(schedule)
+    try:
+        got = ops.attention_prefill(q, kn, kp, v, scale)
+    finally:
+        ops.attention_prefill_schedule(previous)
+    check(got, q, kn, kp, v, 300, 0, scale)
