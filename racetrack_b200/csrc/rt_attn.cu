@@ -1559,7 +1559,7 @@ extern "C" int rt_attn_causal_prefill(const void* q, const void* k_nope, const v
                                       int64_t kp_head_stride, int64_t v_token_stride,
                                       int64_t v_head_stride, int64_t o_token_stride,
                                       int64_t o_head_stride, float softmax_scale, void* stream) {
-    RT_REQUIRE(out, RT_ERR_BAD_ARG, "rt_attn_causal_prefill: null pointer");
+    RT_REQUIRE(out || tokens == 0, RT_ERR_BAD_ARG, "rt_attn_causal_prefill: null pointer");
     return attn_causal_prefill(q, k_nope, k_pe, v, out, nullptr, nullptr, tokens, heads, heads, nope_dim, rope_dim,
                                v_dim, q_token_stride, q_head_stride, kn_token_stride, kn_head_stride,
                                kp_token_stride, kp_head_stride, v_token_stride, v_head_stride,
@@ -1589,7 +1589,7 @@ extern "C" int rt_attn_causal_prefill_share(const void* q, const void* k_nope, c
                                             int64_t v_token_stride, int64_t v_head_stride, int64_t o_token_stride,
                                             int64_t o_head_stride, float softmax_scale, void* stream) {
     RT_REQUIRE(layer_heads >= heads, RT_ERR_BAD_ARG, "rt_attn_causal_prefill_share: layer_heads below heads");
-    if (out == nullptr) {
+    if (out == nullptr && tokens != 0) {                // (an empty tensor has no address)
         RT_REQUIRE(out_codes && out_scales, RT_ERR_BAD_ARG, "rt_attn_causal_prefill_fp8: null pointer");
         RT_REQUIRE(nope_dim == 128 && rope_dim == 64 && v_dim == 128, RT_ERR_UNSUPPORTED,
                    "rt_attn_causal_prefill_fp8: the FP8 epilogue exists for the 128 + 64 / 128 head shape");
@@ -1613,7 +1613,7 @@ extern "C" int rt_attn_window_prefill(const void* q, const void* k_nope, const v
     RT_REQUIRE(window > 0 && sinks >= 0, RT_ERR_BAD_ARG,
                "rt_attn_window_prefill: window must be positive and sinks not negative");
     RT_REQUIRE(layer_heads >= heads, RT_ERR_BAD_ARG, "rt_attn_window_prefill: layer_heads below heads");
-    if (out == nullptr) {
+    if (out == nullptr && tokens != 0) {                // (an empty tensor has no address)
         RT_REQUIRE(out_codes && out_scales, RT_ERR_BAD_ARG, "rt_attn_window_prefill: null pointer");
         RT_REQUIRE(nope_dim == 128 && rope_dim == 64 && v_dim == 128, RT_ERR_UNSUPPORTED,
                    "rt_attn_window_prefill: the FP8 epilogue exists for the 128 + 64 / 128 head shape");

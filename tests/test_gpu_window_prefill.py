@@ -202,3 +202,14 @@ def test_scales_that_are_not_positive_without_a_window(schedule, scale):
     finally:
         ops.attention_prefill_schedule(previous)
     check(got, q, kn, kp, v, 300, 0, scale)
+
+
+@pytest.mark.parametrize("window, sinks", [(None, 0), (5, 1)])
+@pytest.mark.parametrize("nope, rope, v_dim", [(128, 64, 128), (64, 32, 64)])
+def test_a_prompt_without_tokens(nope, rope, v_dim, window, sinks):
+    q, kn, kp, v = inputs(0, 4, 1, nope, rope, v_dim)
+    got = ops.attention_prefill(q, kn, kp, v, window=window, sinks=sinks)
+    assert got.shape == (0, 4, v_dim) and got.dtype == torch.bfloat16
+    codes, scales = ops.attention_prefill(q, kn, kp, v, window=window, sinks=sinks, quantized=True)
+    assert codes.shape == (0, 4 * v_dim) and codes.dtype == torch.float8_e4m3fn
+    assert scales.shape == (0, 4 * v_dim // 128) and scales.dtype == torch.float32

@@ -95,3 +95,16 @@ def test_windowed_prefill(lib, memory, change, code, says):
 
 def test_a_prefill_without_tokens_does_nothing(lib, memory):
     assert call(lib.rt_attn_window_prefill, PREFILL, memory[0], dict(tokens=0)) == 0
+
+
+@pytest.mark.parametrize("change", [{}, dict(out=None, out_codes=None, out_scales=None),
+                                    dict(q=None, k_nope=None, k_pe=None, v=None, out=None), dict(out=None, nope=64, v_dim=64)])
+def test_a_prefill_without_tokens_needs_no_memory(lib, memory, change):
+    """Tensors without elements have no address: no tokens is no error, under a window or without one."""
+    args = dict(change, tokens=0)
+    assert call(lib.rt_attn_window_prefill, PREFILL, memory[0], args) == 0
+    share = {k: v for k, v in PREFILL.items() if k not in ("window", "sinks")}
+    assert call(lib.rt_attn_causal_prefill_share, share, memory[0], args) == 0
+    causal = {k: v for k, v in share.items() if k not in ("out_codes", "out_scales", "layer_heads")}
+    args = {k: v for k, v in args.items() if k in causal}
+    assert call(lib.rt_attn_causal_prefill, causal, memory[0], args) == 0
