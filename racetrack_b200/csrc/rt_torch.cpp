@@ -816,8 +816,6 @@ Prefill prefill_operands(const Tensor& q, const Tensor& k_nope, const OptTensor&
     require_cuda({&q, &k_nope, &v});
     if (window && *window < 1) fail(who + ": window must be positive");
     if (sinks < 0 || (sinks > 0 && !window)) fail(who + ": sinks go with a window and must not be negative");
-    if (k_nope.device() != q.device() || v.device() != q.device() || (k_pe && k_pe->device() != q.device()))
-        fail(who + ": operands must be on one device");
     Prefill p;
     bool ok = q.dim() == 3 && k_nope.dim() == 3 && v.dim() == 3;
     if (ok) {
@@ -832,6 +830,9 @@ Prefill prefill_operands(const Tensor& q, const Tensor& k_nope, const OptTensor&
     }
     if (!ok)
         fail(who + ": expected q [T,H,nope+rope], k_nope [T,H,nope], k_pe [T,rope] or [T,H,rope], v [T,H,v]");
+    // (without rope dims k_pe is not looked at)
+    if (k_nope.device() != q.device() || v.device() != q.device() || (p.rope > 0 && k_pe->device() != q.device()))
+        fail(who + ": operands must be on one device");
     auto view = [&](const Tensor& t, const char* name) {
         if (t.scalar_type() != at::kBFloat16) fail(who + ": " + name + " must be bfloat16");
         bool fits = t.stride(-1) == 1 && aligned16(t);

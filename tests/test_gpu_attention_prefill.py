@@ -264,3 +264,13 @@ def test_both_sides_of_the_schedule_rule(ops, tokens, heads):
     ops.tc_error_state()
     assert torch.equal(outs[0], outs[1]) or torch.equal(outs[0], outs[2])
     assert rel_err(outs[1], outs[2]) <= 1e-2
+
+
+def test_a_rope_key_is_not_looked_at_without_rope_dims(ops):
+    q, kn, _, v = (t.cuda() for t in _qkv(50, 2, 128, 8, 128, 77))
+    q = q[..., :128]
+    want = ops.attention_prefill(q, kn, None, v)
+    for k_pe in (torch.empty(50, 0), torch.empty(50, 0, device="cuda"), torch.zeros(3)):
+        assert torch.equal(ops.attention_prefill(q, kn, k_pe, v), want)
+    with pytest.raises(RuntimeError, match="one device"):
+        ops.attention_prefill(torch.cat((q, q[..., :8]), -1), kn, torch.zeros(50, 8).bfloat16(), v)
