@@ -211,10 +211,14 @@ class PagedDecodeLayer(_AbsorbedLayer):
 
     def prefill(self, hidden: torch.Tensor, seq: torch.Tensor, layers: int) -> torch.Tensor:
         """hidden [T, H] bf16, the prompt of the empty sequence seq (int32 [1]) -> hidden after `layers`
-        applications of the layer; the prompt's rows are left in the caches."""
-        tokens = hidden.shape[0]
+        applications of the layer; the prompt's rows are left in the caches. A sequence that holds tokens already is
+        refused as one out of range is: it stays as it was, caches.check() tells of it, and what is returned
+        belongs to no sequence."""
+        tokens, lens = hidden.shape[0], self.caches.seq_lens
+        held = lens.index_select(0, seq.clamp(min=0, max=lens.shape[0] - 1))
+        served = torch.where((seq < 0) | (held == 0), seq, lens.shape[0])
         offsets = torch.arange(2, device=hidden.device, dtype=torch.int32) * tokens
-        self._slots = self.caches.extend(tokens, seq, offsets=offsets)
+        self._slots = self.caches.extend(tokens, served, offsets=offsets)
         try:
             return self.forward_stack(hidden, torch.arange(tokens, device=hidden.device, dtype=torch.int64), layers)
         finally:

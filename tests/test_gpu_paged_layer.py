@@ -164,3 +164,48 @@ def test_a_pool_that_is_full_is_reported():
     with pytest.raises(RuntimeError, match="1 pages were lacking"):
         m.caches.check()
     assert m.caches.seq_lens.tolist()[0] == 64
+
+
+def test_a_prompt_for_a_sequence_that_holds_tokens_is_refused():
+    """Positions and attention of a prompt begin at 0, so a second one has no place behind the first."""
+    m, twin = model(), model()
+    for x in (m, twin):
+        x.prefill(prompt(40, 1), ints([1]), 1)
+        x.prefill(prompt(20, 3), ints([0]), 1)
+    m.prefill(prompt(24, 2), ints([1]), 1)
+    with pytest.raises(RuntimeError, match="1 entries were refused .0 pages"):
+        m.caches.check()
+    for name in ("kv", "pe", "block_table", "seq_lens", "refcount"):
+        a, b = getattr(m.caches, name), getattr(twin.caches, name)
+        assert torch.equal(a, b), name
+    # padding is not refused, a number out of range is; a sequence that was given back takes a new prompt
+    m.prefill(prompt(24, 2), ints([-1]), 1)
+    m.caches.check()
+    m.prefill(prompt(24, 2), ints([6]), 1)
+    with pytest.raises(RuntimeError, match="1 entries were refused"):
+        m.caches.check()
+    m.caches.free(ints([1]))
+    again = m.prefill(prompt(24, 2), ints([1]), 1)
+    m.caches.check()
+    assert m.caches.seq_lens.tolist() == [20, 24, 0, 0, 0, 0]
+    assert torch.equal(again, twin.prefill(prompt(24, 2), ints([4]), 1))
+
+
+def test_a_captured_prompt_is_refused_on_its_second_replay():
+    m = model()
+    hidden, seq = prompt(33, 1), ints([2])
+    m.prefill(hidden, ints([3]), 1)
+    m.caches.free(ints([3]))
+    side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    with torch.cuda.stream(side):
+        side.wait_stream(torch.cuda.default_stream())
+        with torch.cuda.graph(graph, stream=side):
+            m.prefill(hidden, seq, 1)
+    torch.cuda.synchronize()
+    graph.replay()
+    m.caches.check()
+    assert m.caches.seq_lens.tolist() == [0, 0, 33, 0, 0, 0]
+    graph.replay()
+    with pytest.raises(RuntimeError, match="1 entries were refused"):
+        m.caches.check()
+    assert m.caches.seq_lens.tolist() == [0, 0, 33, 0, 0, 0]
