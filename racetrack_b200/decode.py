@@ -97,7 +97,7 @@ class _AbsorbedLayer(RealisticLayer):
         """Latent attention output [B, h, kv_lora] -> this rank's partial sum in `out` (an exchange buffer the
         other ranks read), or the all-reduced [B, H]."""
         s = self.shape
-        heads_out = ops.linear_bf16_batched(latent, self.w_uv).reshape(latent.shape[0], -1)     # [B, h * v]
+        heads_out = ops.linear_bf16_batched(latent, self.w_uv).flatten(1)     # [B, h * v]
         if out is not None:
             return self.w_o(heads_out, out=out)
         return self._all_reduce(self.w_o(heads_out))

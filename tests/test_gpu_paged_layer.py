@@ -209,3 +209,13 @@ def test_a_captured_prompt_is_refused_on_its_second_replay():
     with pytest.raises(RuntimeError, match="1 entries were refused"):
         m.caches.check()
     assert m.caches.seq_lens.tolist() == [0, 0, 33, 0, 0, 0]
+
+
+def test_the_attention_half_of_a_step_without_sequences():
+    m = model()
+    none = ints([])
+    normed = ops.fused_rms_norm(prompt(1, 1), m.ones_h, eps=SHAPE.eps)[:0]
+    out = m.decode_attention(normed, none, m.caches.extend(0, none), torch.zeros(0, device="cuda", dtype=torch.int64))
+    assert out.shape == (0, SHAPE.hidden)
+    m.caches.check()
+    assert not m.caches.seq_lens.any()
