@@ -14,8 +14,8 @@
 //   32 heads, 128 under a window of 1024 (0.11 GB)   38 us; 64 of 4096 65 us
 //   128 heads, 64 of 4096                            92 us, 790 TFLOP/s; 64 heads 69.5 us
 //   one sequence of 17 positions, 16 heads           8.7 us; of 131072 37 us
-// Two kernels share the walk over the tiles and the join. mla_paged_kernel serves groups of up to 32 heads,
-// mla_paged_wide_kernel of 64; each served all groups once, with an earlier join: the first takes 124 us for
+// Two kernels share the walk over the tiles and the join. mla_paged_kernel serves up to 32 heads,
+// mla_paged_wide_kernel more of them in groups of 64; each served all groups once, with an earlier join: the first takes 124 us for
 // 64 x 4096 at 128 heads where the second took 97 (80 and 75 at 64), the second 44 for the window's case and 99
 // for the ragged one where the first took 40 and 97.
 #include "rt_tc.cuh"
@@ -144,10 +144,9 @@ __device__ RangeStart find_range(const PagedArgs& a, int range, volatile int* sc
     return r;
 }
 
-// ---- up to 32 heads a group -------------------------------------------------------------------
-// Work of a CTA: its range of tiles for one group of G heads, 16 or 32 (more heads are several groups, whose CTAs
-// run side by side and share the tiles in L2). Positions and dims are the rows of the products, heads the
-// columns: with few heads what the tensor core reads from shared memory is then little more than the tile
+// ---- up to 32 heads ---------------------------------------------------------------------------
+// Work of a CTA: its range of tiles for all heads, padded to G = 16 or 32. Positions and dims are the rows of the
+// products, heads the columns: with few heads what the tensor core reads from shared memory is then little more than the tile
 // itself. (Heads as rows, padded to 128, took 2300 + 1400 cycles a tile for 16 heads: 4 KB of mostly empty
 // query rows for each instruction. This form takes about half.) Per tile of 64 positions:
 //   producer  one TMA box a page (32 positions at most, which are also given back together) brings the latent
@@ -443,8 +442,7 @@ __global__ void __launch_bounds__(kPThreads, 1) mla_paged_kernel(const __grid_co
     float* const f_s = w_s + 256;                                            // what a finished row's O is multiplied with
 
     const int warp = uniform_warp_id(), lane = threadIdx.x & 31;
-    const int groups = (a.heads + G - 1) / G;
-    const int hg = blockIdx.x % groups, range = blockIdx.x / groups;
+    const int range = blockIdx.x;
 
     if (threadIdx.x == 0) {
         *abort_flag = 0;
@@ -583,8 +581,8 @@ __global__ void __launch_bounds__(kPThreads, 1) mla_paged_kernel(const __grid_co
                         if (w.flags & 1) {
                             const uint32_t qd = base + qb * (G * kPQRow);
                             mbar_arrive_expect_tx(qfull(qb), G * kPQRow);
-                            tma_load_4d(qd, &tm_qa, 0, hg * G, 0, w.b, qfull(qb));
-                            tma_load_3d(qd + G * 1024, &tm_qp, 0, hg * G, w.b, qfull(qb));
+                            tma_load_4d(qd, &tm_qa, 0, 0, 0, w.b, qfull(qb));
+                            tma_load_3d(qd + G * 1024, &tm_qp, 0, 0, w.b, qfull(qb));
                         }
                         info_s[st].mask = w.mask;
                         info_s[st].row = w.b;
@@ -772,8 +770,8 @@ __global__ void __launch_bounds__(kPThreads, 1) mla_paged_kernel(const __grid_co
                 // all, every page out of the pool or every score -infinity: it is zero)
                 if (tid < G) {
                     const float den = (w_s[tid] + w_s[64 + tid]) + (w_s[128 + tid] + w_s[192 + tid]);
-                    if (part >= 0 && hg * G + tid < a.heads)
-                        *reinterpret_cast<float2*>(a.part_ml + (static_cast<int64_t>(part) * a.heads + hg * G + tid) * 2) =
+                    if (part >= 0 && tid < a.heads)
+                        *reinterpret_cast<float2*>(a.part_ml + (static_cast<int64_t>(part) * a.heads + tid) * 2) =
                             make_float2(den == 0.f ? ninf : m_own, den);
                     f_s[tid] = den == 0.f ? 0.f : part < 0 ? 1.f / den : 1.f;
                 }
@@ -791,14 +789,14 @@ __global__ void __launch_bounds__(kPThreads, 1) mla_paged_kernel(const __grid_co
         // finished rows out of tensor memory, while the next row's first tile is on its way
         const int quad = warp & 3;
         const uint32_t lane_base = static_cast<uint32_t>(quad * 32) << 16;
-        if (hg == 0) clear_empty_rows(a, range);
+        clear_empty_rows(a, range);
         for (int seg = 0, left = n_tiles; left > 0; ++seg) {
             if (!mbar_wait_warp(efull, seg & 1, abort_flag, 94)) break;
             const int b = done_s[0], part = done_s[1], tiles = done_s[2];
             if (!mbar_wait_warp(odone, seg & 1, abort_flag, 88)) break;
             tc_fence_after();
             left -= tiles;
-            write_row<G>(a, part, b, hg * G, tmem_base + lane_base, f_s);
+            write_row<G>(a, part, b, 0, tmem_base + lane_base, f_s);
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(ofree);
@@ -814,7 +812,7 @@ __global__ void __launch_bounds__(kPThreads, 1) mla_paged_kernel(const __grid_co
 }
 
 // ---- 33 heads and more ------------------------------------------------------------------------
-// Groups of 64 heads, the same mathematics. With 64 query rows in shared memory only two tiles fit beside them,
+// Groups of 64 heads, whose CTAs run side by side and share the tiles in L2; the same mathematics. With 64 query rows in shared memory only two tiles fit beside them,
 // and a tile's way (load 2000 cycles, scores 1400, softmax 1400, P V 1100) took 3100 cycles over two places. Here
 // the queries lie in tensor memory, as the A operand of the scores: 64 heads are its rows, dims 0-287 of the
 // rows 16 i .. 16 i + 15 in lanes 32 i .. of 144 columns, dims 288-575 in lanes 32 i + 16 .. of the same columns,
@@ -1407,8 +1405,8 @@ int paged_attn_error_take() {
     return v;
 }
 
-// Heads of a CTA (the fewest groups, then the narrowest that holds its share), and the ranges that the tiles
-// are cut into.
+// Heads of a CTA (the fewest groups, then the narrowest that holds its share: below 64 there is one group), and the
+// ranges that the tiles are cut into.
 static int paged_group(int64_t heads) {
     const int64_t groups = (heads + kWideG - 1) / kWideG, share = (heads + groups - 1) / groups;
     return share <= 16 ? 16 : share <= 32 ? 32 : 64;
@@ -1424,7 +1422,7 @@ static int launch_paged(int group, const CUtensorMap& tm_qa, const CUtensorMap& 
     auto* kernel = group == 16 ? &mla_paged_kernel<16> : group == 32 ? &mla_paged_kernel<32> : &mla_paged_wide_kernel;
     const int smem = static_cast<int>(group == kWideG ? kWideSmemBytes : kPSmemBytes);
     if (int rc = ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), smem, "rt_mla_paged_decode")) return rc;
-    const int groups = (a.heads + group - 1) / group;
+    const int groups = (a.heads + group - 1) / group;          // one below groups of 64
     kernel<<<static_cast<unsigned>(a.n_ranges * groups), kPThreads, smem, s>>>(tm_qa, tm_qp, tm_kv, tm_pe, a);
     count_launch();
     return check_launch("mla_paged_kernel");
