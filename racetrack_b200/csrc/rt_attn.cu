@@ -540,7 +540,7 @@ struct PrefillArgs {
     int one_op;                  // bit i set: operand i (q_nope, q_pe, k_nope, k_pe, v) arrives as ONE box
     int pe_shared;               // k_pe has one row per token for all heads
     float scale_log2;            // 0 or more; hidden scores are -infinity before they meet it
-    float sign;                  // 1, or what signed_scores multiplies the scores with first
+    float sign;                  // the signed form: what the scores are multiplied with first
     // optional (v_dim 128): the output as act_quant leaves it, FP8 e4m3 codes
     // [tokens, heads * 128] and one fp32 scale per token and head (= per 128-wide group)
     uint8_t* out_codes;
@@ -627,18 +627,6 @@ __device__ __forceinline__ void softmax_chunk(const uint32_t (&r)[32], uint32_t 
     }
 }
 
-// The kernels hide a score by -infinity and take a row's maximum before the scale, so the scale they use is
-// positive: a negative one gives its sign to the scores, and 0 (of which -infinity would make NaN) makes them 0 and
-// leaves 1 as the scale. Behind one uniform branch: a call with a positive scale skips the 64 products.
-__device__ __forceinline__ void signed_scores(float sign, uint32_t (&r0)[32], uint32_t (&r1)[32]) {
-    if (sign == 1.f) return;
-#pragma unroll
-    for (int i = 0; i < 32; ++i) {
-        r0[i] = __float_as_uint(__uint_as_float(r0[i]) * sign);
-        r1[i] = __float_as_uint(__uint_as_float(r1[i]) * sign);
-    }
-}
-
 // kWindow: under a sliding window with sinks a block of 256 queries walks the key tiles that hold sinks and
 // then those from the first key its first query sees on; both query tiles walk the same list. A tile that
 // not every query of a query tile sees whole is masked by 64 bits a thread; a row may meet a tile that it
@@ -647,7 +635,11 @@ __device__ __forceinline__ void signed_scores(float sign, uint32_t (&r0)[32], ui
 // tokens x 32 heads under 1024 with 64 sinks 214 -> 206 us).
 // kTiles 1: 128 queries a CTA, for a grid of twice the CTAs that still runs in one wave (777 x 16 heads under
 // 200 18 -> 14 us).
-template <bool kWindow, int kTiles = 2>
+// kSigned: for scales of 0 and below. A score is hidden by -infinity and a row's maximum taken before the scale, which
+// therefore has to be positive: a negative one gives its sign to the scores first, and 0 (of which -infinity would make
+// NaN) makes them 0 and leaves 1 as the scale. A form of its own, which takes all such calls, a window of all tokens
+// standing for none: behind a branch in the others the products cost 64 heads x 4096 about 1 % (361 us).
+template <bool kWindow, int kTiles = 2, bool kSigned = false>
 __global__ void __launch_bounds__(kFThreads, 1) attn_prefill_kernel(
     const __grid_constant__ CUtensorMap tm_qn, const __grid_constant__ CUtensorMap tm_qp,
     const __grid_constant__ CUtensorMap tm_kn, const __grid_constant__ CUtensorMap tm_kp,
@@ -859,7 +851,13 @@ __global__ void __launch_bounds__(kFThreads, 1) attn_prefill_kernel(
             tmem_ld_wait(r0);
             tmem_ld_wait(r1);
             if (threadIdx.x == 64) RT_FTRACE(7, j);
-            signed_scores(a.sign, r0, r1);
+            if constexpr (kSigned) {
+#pragma unroll
+                for (int i = 0; i < 32; ++i) {
+                    r0[i] = __float_as_uint(__uint_as_float(r0[i]) * a.sign);
+                    r1[i] = __float_as_uint(__uint_as_float(r1[i]) * a.sign);
+                }
+            }
             if constexpr (kWindow) {
                 const int k0 = 128 * key_tile(j), r0_abs = q0 + 128 * t;
                 if (j == n_t - 1 || !(k0 > r0_abs + 127 - a.window || k0 + 127 < a.sinks)) {
@@ -1246,7 +1244,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFThreads, 1) attn_p
             __syncwarp();
             if (lane == 0) mbar_arrive_cluster(s_free_leader);
             if (threadIdx.x == 64) RT_FTRACE(7, j);
-            signed_scores(a.sign, r0, r1);
             if (j == n - 1) {                                 // diagonal tile: keys beyond the row's own are masked
                 const int c0 = 64 * cq;
 #pragma unroll
@@ -1675,11 +1672,16 @@ static int attn_causal_prefill(const void* q, const void* k_nope, const void* k_
     a.cv = static_cast<int>((v_dim + 63) / 64);
     a.v_dim = static_cast<int>(v_dim);
     a.pe_shared = pe_shared ? 1 : 0;
-    a.sign = softmax_scale < 0.f ? -1.f : softmax_scale == 0.f ? 0.f : 1.f;
+    const bool other = softmax_scale <= 0.f;
+    a.sign = softmax_scale == 0.f ? 0.f : -1.f;
     a.scale_log2 = softmax_scale == 0.f ? 1.f : fabsf(softmax_scale) * 1.4426950408889634f;
     a.out_codes = static_cast<uint8_t*>(out_codes);
     a.out_scales = out_scales;
     if (window >= tokens) window = 0;                  // every query sees all keys before it
+    if (other && window == 0) {
+        window = tokens;
+        sinks = 0;
+    }
     a.window = static_cast<int>(window);
     a.sinks = static_cast<int>(sinks < tokens ? sinks : tokens);
     CUtensorMap tm_qn, tm_qp, tm_kn, tm_kp, tm_v;
@@ -1706,8 +1708,9 @@ static int attn_causal_prefill(const void* q, const void* k_nope, const void* k_
     a.one_op = (one[0] ? 1 : 0) | (one[1] ? 2 : 0) | (one[2] ? 4 : 0) | (one[3] ? 8 : 0) | (one[4] ? 16 : 0);
     const bool mla_shape = nope_dim == 128 && rope_dim == 64 && v_dim == 128;
     if (window > 0) {
-        const bool one = (tokens + 127) / 128 * heads <= tc::sm_count();
-        const auto kernel = one ? &tc::attn_prefill_kernel<true, 1> : &tc::attn_prefill_kernel<true, 2>;
+        const bool one = !other && (tokens + 127) / 128 * heads <= tc::sm_count();
+        const auto kernel = other ? &tc::attn_prefill_kernel<true, 2, true>
+                                  : one ? &tc::attn_prefill_kernel<true, 1> : &tc::attn_prefill_kernel<true, 2>;
         if (int rc = ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), static_cast<int>(tc::kFSmemBytes),
                                          "rt_attn_window_prefill"))
             return rc;
