@@ -491,7 +491,7 @@ __global__ void __launch_bounds__(128) mla_merge_kernel(const float* __restrict_
 //                      clocks whoever issues them; two warps per scheduler keep it busy), each
 //                      with 64 of the row's scores in registers after one tcgen05.ld pass: causal
 //                      mask on the diagonal tile, the two half-row maxima exchanged through shared
-//                      memory (as bf16, so both threads use the same value), running maximum with a
+//                      memory (as bf16, under a window in 24 bits, so both threads use the same value), running maximum with a
 //                      lazy rescale (the accumulator is rescaled only when the maximum grows by
 //                      more than 2^8), P = exp2(s - m) written back as bf16 INTO THE SCORE COLUMNS
 //                      (two per column);
@@ -514,7 +514,8 @@ constexpr uint32_t kFVOff = 12 * kFChunk;                  // 2 chunks
 constexpr uint32_t kFBarOff = 14 * kFChunk;
 constexpr int kFBars = 12;     // q_full[2] k_full[2] k_empty[2] v_full v_empty s_full[2] p_full[2] + o_full[2] below
 constexpr uint32_t kFXmOff = kFBarOff + (kFBars + 2) * 8 + 16;        // row maxima exchanged as bf16 [2][128][2]
-constexpr uint32_t kFSmemBytes = kFXmOff + 2 * 128 * 2 * 2 + 1024;
+constexpr uint32_t kFXlOff = kFXmOff + 2 * 128 * 2 * 2;               // under a window: eight bits more of each
+constexpr uint32_t kFSmemBytes = kFXlOff + 2 * 128 * 2 + 1024;
 static_assert(kFSmemBytes <= 232448, "shared memory budget");
 
 // Optional pipeline trace (never compiled into the library): with -DRT_FA_TRACE the CTA of the
@@ -831,6 +832,7 @@ __global__ void __launch_bounds__(kFThreads, 1) attn_prefill_kernel(
         const float ninf = __int_as_float(0xff800000);
         const int o_half = a.cv;                              // 32-column accumulator chunks per thread
         __nv_bfloat16* xm = reinterpret_cast<__nv_bfloat16*>(base_ptr + kFXmOff) + (t * 128 + row) * 2;
+        uint8_t* const xl8 = base_ptr + kFXlOff + (t * 128 + row) * 2;
         float m_ref = ninf, l = 0.f;
         bool ok = n_t > 0;
         for (int j = 0; ok && j < n_t; ++j) {
@@ -891,11 +893,25 @@ __global__ void __launch_bounds__(kFThreads, 1) attn_prefill_kernel(
                 mx2 = fmaxf(mx2, __uint_as_float(r1[i]));
                 mx3 = fmaxf(mx3, __uint_as_float(r1[16 + i]));
             }
-            // both threads of a row round both half maxima to bf16, so they agree on the maximum
-            const __nv_bfloat16 mine = __float2bfloat16_rn(fmaxf(fmaxf(mx0, mx1), fmaxf(mx2, mx3)) * a.scale_log2);
-            xm[hh] = mine;
-            asm volatile("bar.sync %0, 64;" ::"r"(pair_bar) : "memory");
-            const float mt = fmaxf(__bfloat162float(mine), __bfloat162float(xm[hh ^ 1]));
+            float mt = fmaxf(fmaxf(mx0, mx1), fmaxf(mx2, mx3)) * a.scale_log2;
+            if constexpr (kWindow) {
+                // both half maxima to 24 bits (32 do not fit), the same to the row's two threads: with a maximum m off
+                // by 2^-16 m the probability of a row's only key is 1 in bf16 and 1 to 2^-9 in the sum, and so its value
+                // comes back as it is, up to |m| = 184 (2^-9 / (ln 2 2^-16)). From a maximum in bf16 it came back off
+                // by up to 2^-8.
+                const uint32_t mine = (__float_as_uint(mt) + 0x80u) >> 8;
+                uint16_t* const hi = reinterpret_cast<uint16_t*>(xm);
+                hi[hh] = static_cast<uint16_t>(mine >> 8);
+                xl8[hh] = static_cast<uint8_t>(mine);
+                asm volatile("bar.sync %0, 64;" ::"r"(pair_bar) : "memory");
+                mt = fmaxf(__uint_as_float(mine << 8), __uint_as_float(static_cast<uint32_t>(hi[hh ^ 1]) << 16 | static_cast<uint32_t>(xl8[hh ^ 1]) << 8));
+            } else {
+                // both threads of a row round both half maxima to bf16, so they agree on the maximum
+                const __nv_bfloat16 mine = __float2bfloat16_rn(mt);
+                xm[hh] = mine;
+                asm volatile("bar.sync %0, 64;" ::"r"(pair_bar) : "memory");
+                mt = fmaxf(__bfloat162float(mine), __bfloat162float(xm[hh ^ 1]));
+            }
             const bool grow = mt > m_ref + 8.f;
             const float m_new = grow ? mt : m_ref;
             if (nth > 0 && __any_sync(0xffffffffu, grow)) {

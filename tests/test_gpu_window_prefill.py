@@ -213,3 +213,16 @@ def test_a_prompt_without_tokens(nope, rope, v_dim, window, sinks):
     codes, scales = ops.attention_prefill(q, kn, kp, v, window=window, sinks=sinks, quantized=True)
     assert codes.shape == (0, 4 * v_dim) and codes.dtype == torch.float8_e4m3fn
     assert scales.shape == (0, 4 * v_dim // 128) and scales.dtype == torch.float32
+
+
+@pytest.mark.parametrize("tokens, heads", [(1, 3), (300, 2), (300, 60)])
+@pytest.mark.parametrize("spread", [0.1, 1.0, 2.0])
+@pytest.mark.parametrize("window, sinks", [(1, 0), (2, 0), (40, 3)])
+def test_a_key_that_is_seen_alone_gives_its_value(tokens, heads, spread, window, sinks):
+    """Its probability is 1: the output is the value itself, to the bit (scores up to 100 in size). Two and 60 heads
+    are the two tilings; a single token takes the causal call, so it is asked for under a window in two."""
+    q, kn, kp, v = inputs(max(tokens, 2), heads, tokens + 13, spread=spread)
+    got = ops.attention_prefill(q, kn, kp, v, window=1 if tokens == 1 else window, sinks=sinks)
+    alone = seen(max(tokens, 2), 1 if tokens == 1 else window, sinks).sum(1) == 1
+    assert alone[0] and (window > 1 or sinks or bool(alone.all()))
+    assert torch.equal(got[alone].view(torch.int16), v[alone].view(torch.int16))
