@@ -808,8 +808,10 @@ int rt_attn_causal_prefill_share(const void* q, const void* k_nope, const void* 
  * rt_attn_causal_prefill_share under a sliding window with sinks: query i sees the keys j <= i with j > i -
  * window or j < sinks, and only key tiles that hold such keys are loaded and multiplied. window >= tokens is
  * the causal call. The key of a token that a query does not see weighs nothing, NaN included; an infinite or
- * NaN value of such a token may reach it (0 * inf), as in a product with a masked softmax. There is one
- * schedule, so the bits do not depend on layer_heads below the window.
+ * NaN value of such a token may reach it (0 * inf), as in a product with a masked softmax. A CTA takes 128 or
+ * 256 queries, by the tokens and heads of the call itself; both forms walk the same key tiles of a query in the
+ * same order, so a share of the heads has the bits of the whole call below the window too, and layer_heads
+ * decides nothing there.
  */
 int rt_attn_window_prefill(const void* q, const void* k_nope, const void* k_pe, const void* v, void* out,
                            void* out_codes, float* out_scales, int64_t tokens, int64_t heads,

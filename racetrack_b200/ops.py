@@ -602,7 +602,8 @@ def attention_prefill(q: torch.Tensor, k_nope: torch.Tensor, k_pe: Optional[torc
     ``out`` = (codes, scales) to write into (contiguous, 1-byte codes).
 
     layer_heads: the heads of the whole layer where a rank holds a share of them (default: H). The schedule
-    is the one the whole layer would take, so the share has the bits a call with every head gives.
+    is the one the whole layer would take, so the share has the bits a call with every head gives. (Under a
+    window all schedules give the same bits.)
 
     window: query i sees only the last `window` keys up to its own and the first `sinks` of all; key tiles
     without such a key are neither loaded nor multiplied. A window of T or more is the causal call. Hidden

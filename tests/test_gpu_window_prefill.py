@@ -226,3 +226,23 @@ def test_a_key_that_is_seen_alone_gives_its_value(tokens, heads, spread, window,
     alone = seen(max(tokens, 2), 1 if tokens == 1 else window, sinks).sum(1) == 1
     assert alone[0] and (window > 1 or sinks or bool(alone.all()))
     assert torch.equal(got[alone].view(torch.int16), v[alone].view(torch.int16))
+
+
+@pytest.mark.parametrize("scale", [None, -0.05])
+@pytest.mark.parametrize("window, sinks", [(200, 0), (200, 4), (300, 300), (129, 129), (128, 128), (1, 0), (600, 128)])
+@pytest.mark.parametrize("tokens, heads, share", [(777, 32, 4), (700, 40, 1)])
+def test_a_share_of_the_heads_has_the_bits_of_the_whole(tokens, heads, share, window, sinks, scale):
+    """All heads fill more than one wave with blocks of 256 queries, a share takes blocks of 128: the same bits,
+    whatever the share says of its layer."""
+    q, kn, kp, v = inputs(tokens, heads, 17)
+    kw = dict(softmax_scale=scale, window=window, sinks=sinks)
+    whole = ops.attention_prefill(q, kn, kp, v, **kw)
+    codes, scales = ops.attention_prefill(q, kn, kp, v, quantized=True, **kw)
+    for lo in (0, heads - share):
+        mine = slice(lo, lo + share)
+        for layer_heads in (heads, share):
+            part = ops.attention_prefill(q[:, mine], kn[:, mine], kp, v[:, mine], layer_heads=layer_heads, **kw)
+            assert torch.equal(part.view(torch.int16), whole[:, mine].contiguous().view(torch.int16))
+            c, s = ops.attention_prefill(q[:, mine], kn[:, mine], kp, v[:, mine], quantized=True, layer_heads=layer_heads, **kw)
+            assert torch.equal(c.view(torch.uint8), codes.view(torch.uint8)[:, lo * 128:(lo + share) * 128])
+            assert torch.equal(s, scales[:, mine])
