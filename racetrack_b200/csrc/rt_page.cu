@@ -221,8 +221,12 @@ __device__ void extend(const ExtendArgs& a) {
     for (int r = threadIdx.x; r < got; r += kPlanThreads) {
         const int i = last_not_above(cum, a.n, r), old = old_len[i];
         if (old < 0) continue;
-        const int s = a.seqs ? a.seqs[i] : i;
-        a.table[s * a.table_stride + ceil_div(old, a.page) + (r - cum[i])] = found[r];
+        int s, first, count;
+        extend_entry(a, i, s, first, count);
+        // (offsets that overlap can take the prefix sums past 31 bits: no entry takes more pages than it needs)
+        const int have = ceil_div(old, a.page), k = r - cum[i];
+        if (static_cast<unsigned>(k) >= static_cast<unsigned>(ceil_div(old + count, a.page) - have)) continue;
+        a.table[s * a.table_stride + have + k] = found[r];
         a.refs[found[r]] = 1;
     }
     __syncthreads();

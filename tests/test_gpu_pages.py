@@ -344,3 +344,22 @@ def test_what_is_refused(call, says):
     with pytest.raises(RuntimeError, match=says):
         call(c)
     same(c, m)
+
+
+@pytest.mark.parametrize("seed", range(6))
+def test_lists_whose_offsets_overlap_keep_tables_and_counts_together(seed):
+    """Offsets that do not ascend are nobody's list, but every page that is named is counted, none is named twice,
+    and no sequence has more entries than its length asks for."""
+    r = random.Random(seed)
+    c, _ = make(200, 16, 40, 12, extra=None)
+    c.append(rows(c, 60, seed), ints(range(40)[::2]), offsets=ints([3 * i for i in range(21)]))
+    n, tokens = 40, r.choice([30, 64, 500])
+    offsets = [r.randrange(-20, tokens + 40) for _ in range(n + 1)]
+    order = r.sample(range(40), n)
+    c.append(rows(c, tokens, seed + 1), ints(order), offsets=ints(offsets))
+    table, lens = c.block_table.cpu(), c.seq_lens.tolist()
+    named = table[table >= 0]
+    assert torch.equal(torch.bincount(named, minlength=200), c.refcount.cpu().long())
+    assert len(set(named.tolist())) == named.numel()
+    for s in range(40):
+        assert int((table[s] >= 0).sum()) <= -(-lens[s] // 16) and lens[s] <= 12 * 16
