@@ -686,7 +686,7 @@ int rt_mla_paged_decode(const void* q_abs, const void* q_pe, const void* kv, con
 
 /*
  * Sequence seqs[i] (NULL: i) grows by offsets[i + 1] - offsets[i] tokens (NULL: one each), tokens
- * [offsets[i], offsets[i + 1]) of the list: takes the lowest free pages, in the order of the list, and
+ * [offsets[i], offsets[i + 1]) of the list (offsets ascend from 0 to at most tokens): takes the lowest free pages, in the order of the list, and
  * writes where the rows of the tokens go: slots int32 [tokens], page * page_size + row, -1 for the tokens of
  * entries that were not served (a number out of range, one that an earlier entry has named, more than
  * width pages, no free page left) and for padding. workspace: rt_page_extend_workspace_ints(n, tokens) ints.

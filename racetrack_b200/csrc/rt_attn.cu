@@ -633,9 +633,9 @@ __device__ __forceinline__ void softmax_chunk(const uint32_t (&r)[32], uint32_t 
 // not every query of a query tile sees whole is masked by 64 bits a thread; a row may meet a tile that it
 // sees nothing of before its first key, so its maximum may still be -infinity. The first tile behind the sinks
 // may lie outside the windows of all of query tile 1, which then leaves it out (one of some ten: 8192
-// tokens x 32 heads under 1024 with 64 sinks 214 -> 206 us).
+// tokens x 32 heads under 1024 with 64 sinks 214 -> 206 us in short runs; in long ones among other work 236 to 242).
 // kTiles 1: 128 queries a CTA, for a grid of twice the CTAs that still runs in one wave (777 x 16 heads under
-// 200 18 -> 14 us).
+// 200 18 -> 14 us; the whole call 16.2).
 // kSigned: for scales of 0 and below. A score is hidden by -infinity and a row's maximum taken before the scale, which
 // therefore has to be positive: a negative one gives its sign to the scores first, and 0 (of which -infinity would make
 // NaN) makes them 0 and leaves 1 as the scale. A form of its own, which takes all such calls, a window of all tokens
@@ -765,11 +765,11 @@ __global__ void __launch_bounds__(kFThreads, 1) attn_prefill_kernel(
                 }
                 mma_commit(s_full(t));
             };
-            auto issue_pv = [&](int t, int first) {            // first: nothing to add to yet
+            auto issue_pv = [&](int t, int nth) {              // nth: of the key tiles taken; the first has nothing to add to
 #pragma unroll
                 for (int k = 0; k < 8; ++k) {
                     const uint64_t bdesc = smem_desc_sw128_mn(base + kFVOff + k * 2048, kFChunk);
-                    mma_f16_ts(t_o(t), t_s(t) + 8u * k, bdesc, idesc_o, (first | k) != 0 ? 1u : 0u);
+                    mma_f16_ts(t_o(t), t_s(t) + 8u * k, bdesc, idesc_o, (nth | k) != 0 ? 1u : 0u);
                 }
             };
             bool ok = mbar_wait(q_full(0), 0, abort_flag, 73) && mbar_wait(k_full(0), 0, abort_flag, 74);

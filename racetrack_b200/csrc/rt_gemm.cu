@@ -1888,8 +1888,6 @@ int make_tmap_rows128_batched(CUtensorMap* map, const void* ptr, uint64_t rows, 
     return RT_OK;
 }
 
-// 4-D bf16 tensor map with the 128-byte swizzle for the attention kernels (rt_attn.cu): dims and
-// box are given fastest dimension first, strides in bytes for dimensions 1..3.
 // Tensor map of bf16 data, 128-byte swizzle, reads outside it as zeros: `rank` dims (the first contiguous),
 // strides in bytes of the others.
 int make_tmap_bf16(CUtensorMap* map, const void* ptr, int rank, const uint64_t* dims_in, const uint64_t* strides_in,

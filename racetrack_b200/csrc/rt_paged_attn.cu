@@ -9,15 +9,16 @@
 //
 // A row of 1152 bytes serves 2 * 1088 flops for each head, 242 flop/B at 128 heads: with few heads the
 // kernel is bound by reading the cache once, with all of them memory and tensor cores take about the same.
-// Measured on one B200, kernels and join, calls in a row on inputs of three sets (copy rate 6546 GB/s):
-//   16 heads, 48 sequences of up to 32768 (0.56 GB)  96 us, 5800 GB/s; 64 of 4096 (0.30 GB) 58 us
-//   32 heads, 128 under a window of 1024 (0.11 GB)   38 us; 64 of 4096 65 us
-//   128 heads, 64 of 4096                            92 us, 790 TFLOP/s; 64 heads 69.5 us
-//   one sequence of 17 positions, 16 heads           8.7 us; of 131072 37 us
+// Measured on one B200, kernels and join, short runs of calls in a row on inputs of three sets (copy rate 6546 GB/s); in
+// brackets the whole call in long runs among other work, host and power cap included:
+//   16 heads, 48 sequences of up to 32768 (0.56 GB)  96 us, 5800 GB/s (98-105); 64 of 4096 (0.30 GB) 58 us
+//   32 heads, 128 under a window of 1024 (0.11 GB)   38 us (39-40); 64 of 4096 65 us
+//   128 heads, 64 of 4096                            92 us, 790 TFLOP/s (106-112); 64 heads 69.5 us
+//   one sequence of 17 positions, 16 heads           8.7 us (10); of 131072 37 us
 // Two kernels share the walk over the tiles and the join. mla_paged_kernel serves up to 32 heads,
-// mla_paged_wide_kernel more of them in groups of 64; each served all groups once, with an earlier join: the first takes 124 us for
-// 64 x 4096 at 128 heads where the second took 97 (80 and 75 at 64), the second 44 for the window's case and 99
-// for the ragged one where the first took 40 and 97.
+// mla_paged_wide_kernel more of them in groups of 64; each served all groups once, with an earlier join: the first
+// took 124 us for 64 x 4096 at 128 heads where the second took 97 (80 and 75 at 64), the second 44 for the
+// window's case and 99 for the ragged one where the first took 40 and 97.
 #include "rt_tc.cuh"
 
 namespace rt {
@@ -153,8 +154,8 @@ __device__ RangeStart find_range(const PagedArgs& a, int range, volatile int* sc
 //             rows as [8-row groups][8 blocks of 64 dims][8 rows][128 B] (128-byte swizzle), one the rope keys: a
 //             page of any size lands in the same layout, of which both products read their operand (the group
 //             stride is a field of the descriptor), so the rows are staged once. Two tiles are staged (144 KB);
-//             the one behind them is asked into L2 (the ragged batch above 99 us, without 104; two tiles ahead
-//             101, three 105). Boxes of half or a quarter of the dims instead of the positions: 64 x 4096 x 128
+//             the one behind them is asked into L2 (when it came the ragged batch above took 99 us with it, 104
+//             without, 101 two tiles ahead, 105 three). Boxes of half or a quarter of the dims instead of the positions: 64 x 4096 x 128
 //             heads, when this kernel served them, 134 and 142 us instead of 125;
 //   S = K Q^T 36 tcgen05.mma (M = 64 positions, N = G heads, K = 16 dims), both K-major;
 //   softmax   warps 4-7. An M = 64 product lies in lanes 0-15 of each quarter of tensor memory; read in 16 x 256
@@ -826,10 +827,10 @@ __global__ void __launch_bounds__(kPThreads, 1) mla_paged_kernel(const __grid_co
 //             lanes. All warps still vote whether any head's maximum grew, since a warp that scales O holds all
 //             heads of its dims;
 //   P         K-major [head][position] in shared memory, the B operand of O^T += V^T P^T.
-// 2100 to 2400 cycles a tile at 128 heads, kernel alone 85 to 90 us for 64 x 4096 where the first form takes 117. The
-// tensor core is busy for 63 % of them; the rest is the way of the scores (36 instructions of 29 cycles, 450 until
-// they are seen, 265 to read them, 250 until the next may begin: one buffer is all that tensor memory holds)
-// and loads behind it (without asking the next tile into L2: 4 us more). Measured and not kept: the scores'
+// 2100 to 2400 cycles a tile at 128 heads, kernel alone 83 to 90 us for 64 x 4096 where the first form took 117. The
+// tensor core is busy for 66 % of them; the rest is the way of the scores (36 instructions of 29 cycles, about half
+// the rate of M = 128 ones; 450 until they are seen, 265 to read them, 250 until the next may begin: with all
+// 576 dims of the queries in tensor memory it holds one buffer of scores) and loads behind it (without asking the next tile into L2: 4 us more). Measured and not kept: the scores'
 // halves as buffers of their own (4 us more), eight softmax warps (4 us more, with both 18), the halves' instructions
 // in turn (no difference), queries read from global memory by the warps (1 x 4096: 1 us more).
 constexpr int kWideG = 64;
