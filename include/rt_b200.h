@@ -668,7 +668,8 @@ int rt_mla_sparse_decode(const void* q_abs, const void* q_pe, const void* kv, co
  * positions it does not see, NaN included, does not reach the output. An infinite or NaN value of a row that is
  * seen may reach all 512 dims of the output.
  * q_abs bf16 [batch, heads, 512], q_pe bf16 [batch, heads, 64], kv bf16 [pages, page_size, 512], pe bf16
- * [pages, page_size, 64] (strides in elements, multiples of 8, pointers 16-byte aligned), table int32 [slots,
+ * [pages, page_size, 64] (strides in elements, multiples of 8, rows that do not overlap, pointers 16-byte
+ * aligned), table int32 [slots,
  * width], out bf16 [batch, heads, 512] contiguous. page_size: a power of two, 16 or more; heads up to 1024;
  * batch up to 65535. The sequences' tiles are cut evenly over the SMs on the device; a second kernel joins
  * what was cut, in the order of the positions. workspace: rt_mla_paged_decode_workspace_bytes(heads), 16-byte

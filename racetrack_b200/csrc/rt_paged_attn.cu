@@ -1460,6 +1460,11 @@ extern "C" int rt_mla_paged_decode(const void* q_abs, const void* q_pe, const vo
     for (int64_t s : strides)
         RT_REQUIRE(s >= 0 && s % 8 == 0 && s < (1ll << 38), RT_ERR_BAD_ARG,
                    "rt_mla_paged_decode: strides must be non-negative multiples of 8 elements");
+    // (a tensor map's strides are those of rows that lie apart; one of a dimension of 1 is not looked at)
+    RT_REQUIRE(kv_row_stride >= 512 && pe_row_stride >= 64 && (pages <= 1 || (kv_page_stride >= 512 && pe_page_stride >= 64)) &&
+                   (heads == 1 || (qa_head_stride >= 512 && qp_head_stride >= 64)) &&
+                   (batch == 1 || (qa_batch_stride >= 512 && qp_batch_stride >= 64)),
+               RT_ERR_BAD_ARG, "rt_mla_paged_decode: rows must not overlap");
     RT_REQUIRE(window >= 0 && sinks >= 0, RT_ERR_BAD_ARG, "rt_mla_paged_decode: window and sinks must not be negative");
     RT_REQUIRE(pages > 0, RT_ERR_BAD_ARG, "rt_mla_paged_decode: the pool has no page");
     const int64_t tiles = (width * page_size + tc::kPTile - 1) / tc::kPTile;

@@ -1156,11 +1156,14 @@ Tensor mla_paged_decode(const Tensor& q_abs_in, const Tensor& q_pe_in, const Ten
         if (t->stride(2) != 1 || (pages > 1 && (t->stride(0) % 8 != 0 || t->stride(0) < 0)) || t->stride(1) % 8 != 0 ||
             t->stride(1) < 0 || !aligned16(*t))
             fail(who + ": kv_pages and pe_pages must have contiguous, 16-byte aligned rows");
+    for (const Tensor* t : {&kv, &pe})
+        if (t->stride(1) < t->size(2) || (pages > 1 && t->stride(0) < t->size(2)))
+            fail(who + ": rows of kv_pages and pe_pages must not overlap");
     const c10::cuda::CUDAGuard guard(q_abs_in.device());
     // queries are a few rows: what the kernel cannot take as it lies is copied
     auto rows = [](const Tensor& t) {
-        const bool fits = t.stride(2) == 1 && t.stride(0) % 8 == 0 && t.stride(1) % 8 == 0 && t.stride(0) > 0 &&
-                          t.stride(1) > 0 && aligned16(t);
+        const bool fits = t.stride(2) == 1 && t.stride(0) % 8 == 0 && t.stride(1) % 8 == 0 && t.stride(0) >= t.size(2) &&
+                          t.stride(1) >= t.size(2) && aligned16(t);
         return fits ? t : t.clone(at::MemoryFormat::Contiguous);
     };
     const Tensor q_abs = rows(q_abs_in), q_pe = rows(q_pe_in);

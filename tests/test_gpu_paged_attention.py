@@ -402,3 +402,22 @@ def _call(**change):
 def test_what_is_refused(change, says):
     with pytest.raises(RuntimeError, match=says):
         _call(**change)
+
+
+@pytest.mark.parametrize("name, width", [("kv_pages", 512), ("pe_pages", 64)])
+def test_pages_whose_rows_overlap_are_refused(name, width):
+    for view in (lambda t: t[:1].expand(t.shape[0], -1, -1), lambda t: t[:, :1].expand(-1, t.shape[1], -1),
+                 lambda t: t.as_strided(t.shape, (t.stride(0), width - 8, 1))):
+        with pytest.raises(RuntimeError, match="overlap"):
+            _call(**{name: view})
+
+
+@pytest.mark.parametrize("heads", [1, 16, 128])
+def test_rows_of_one_head_or_sequence_and_pages_of_interleaved_rows(heads):
+    """What a dimension of 1 has for a stride does not matter; page p's row r may lie at row r * pages + p."""
+    lengths = [130]
+    kv, pe, table, q_abs, q_pe = make(lengths, heads, 64)
+    turned = lambda t: t.transpose(0, 1).contiguous().transpose(0, 1)
+    odd = lambda t: t.as_strided(t.shape, (3, t.stride(1) if heads > 1 else 5, 1))
+    got = ops.mla_paged_decode(odd(q_abs), odd(q_pe), turned(kv), turned(pe), ints(table), ints(lengths), SCALE)
+    check(got, kv, pe, table, lengths, q_abs, q_pe)

@@ -108,3 +108,10 @@ def test_a_prefill_without_tokens_needs_no_memory(lib, memory, change):
     causal = {k: v for k, v in share.items() if k not in ("out_codes", "out_scales", "layer_heads")}
     args = {k: v for k, v in args.items() if k in causal}
     assert call(lib.rt_attn_causal_prefill, causal, memory[0], args) == 0
+
+
+@pytest.mark.parametrize("change", [dict(kv_row=0), dict(kv_row=504), dict(pe_row=0), dict(kv_page=0), dict(pe_page=56),
+                                    dict(qa_head=0), dict(qp_head=0), dict(batch=2, qa_batch=0), dict(batch=2, qp_batch=8)])
+def test_decode_refuses_rows_that_overlap(lib, memory, change):
+    assert call(lib.rt_mla_paged_decode, DECODE, memory[0], change) == BAD
+    assert b"overlap" in lib.rt_last_error()
